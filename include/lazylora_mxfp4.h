@@ -54,6 +54,7 @@ extern "C" {
 #define MXFP4_BF16 1
 #define MXFP4_I32 2
 #define MXFP4_I64 3
+#define MXFP4_F16 4 /* dense operators only */
 
 /* Flags for the routed layer. */
 #define MXFP4_MOE_SAVE 1          /* forward keeps gate|up and routing in the workspace */
@@ -246,6 +247,63 @@ int mxfp4_router_topk(int64_t *topk_idx, float *topk_w, const float *logits, con
 int mxfp4_router_topk_backward(float *grad_logits, const int64_t *topk_idx, const float *grad_w,
                                const float *logits, int N, int E, int top_k,
                                float routed_scaling_factor, int renormalize, hipStream_t stream);
+
+/* ---- dense operators: the other half of the latent MoE block -------------------------------
+ * Row-major contiguous arrays of `dtype` elements, 16-byte aligned where 16-bit tensors are said to be
+ * (the norms and the dropout take any alignment). Sums, statistics and activation functions are fp32;
+ * every result is rounded to its type once, to nearest even. No atomics: a call's results do not depend
+ * on timing. */
+
+/* Gated feed-forward block (the shared expert, lazy_lora/trainer/lazy_trainer.py:702-708):
+ *   gate = x Wg^T (+ gate_delta), up = x Wu^T (+ up_delta), h = GLU(gate, up), y = h Wd^T.
+ * x [M, D], w_gate and w_up [F, D], w_down [Do, F], gate_delta and up_delta [M, F] (the adapters' terms;
+ * each may be NULL), y [M, Do], h [M, F] (written; the hidden activations, rounded to dtype, are what the
+ * down product reads), all of dtype MXFP4_BF16 or MXFP4_F16. gu: [M, 2F] fp32, gate | up of each row kept
+ * for the backward, or NULL. act_kind as in the routed layer. D, F and Do are multiples of 8 and at most
+ * 2^20, M at most 2^24; all pointers 16-byte aligned. M = 0 is valid. The workspace (256-byte
+ * aligned; both calls) holds partial sums while the call runs. */
+size_t mxfp4_ffn_workspace_size(int M, int D, int F, int Do);
+int mxfp4_ffn_forward(void *y, void *h, float *gu, const void *x, const void *w_gate, const void *w_up,
+                      const void *w_down, const void *gate_delta, const void *up_delta, int dtype, int M,
+                      int D, int F, int Do, int act_kind, void *workspace, size_t workspace_bytes,
+                      hipStream_t stream);
+
+/* Its backward: with dh = dy Wd (+ grad_h, the gradient that reaches h from elsewhere, [M, F] or NULL),
+ * dgu [M, 2F] = dL/dgate | dL/dup of each row (always written; also the gradients of the deltas), and,
+ * each unless its pointer is NULL, dx [M, D], dw_gate and dw_up [F, D] (both or neither) and
+ * dw_down [Do, F]. h and gu are the forward's. With M = 0 the weight gradients are zero. */
+int mxfp4_ffn_backward(void *dx, void *dw_gate, void *dw_up, void *dw_down, void *dgu, const void *dy,
+                       const void *grad_h, const void *x, const void *h, const float *gu,
+                       const void *w_gate, const void *w_up, const void *w_down, int dtype, int M, int D,
+                       int F, int Do, int act_kind, void *workspace, size_t workspace_bytes,
+                       hipStream_t stream);
+
+/* Layer norm and RMS norm over the last axis (RMSNormFunction,
+ * lazy_lora/streaming/trunk_streamer.py:23-34, is the RMS form):
+ *   m = mean(x) (0 for MXFP4_NORM_RMS), r = 1 / sqrt(mean((x - m)^2) + eps),
+ *   y = (x - m) r * weight + bias.
+ * x and y [M, D] of dtype MXFP4_F32, _BF16 or _F16; weight and bias [D] fp32, each may be NULL.
+ * stats: 2 M floats (r, then m for layer norm) for the backward, or NULL. */
+#define MXFP4_NORM_RMS 0
+#define MXFP4_NORM_LAYER 1
+int mxfp4_norm_forward(void *y, float *stats, const void *x, const float *weight, const float *bias,
+                       int M, int D, float eps, int kind, int dtype, hipStream_t stream);
+/* dx [M, D], and dweight = sum over rows of dy (x - m) r and dbias = sum of dy, [D] fp32, each unless
+ * NULL (zeros when M = 0). stats from the forward. */
+size_t mxfp4_norm_workspace_size(int M, int D);
+int mxfp4_norm_backward(void *dx, float *dweight, float *dbias, const void *dy, const void *x,
+                        const float *weight, const float *stats, int M, int D, int kind, int dtype,
+                        void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Dropout whose mask is a function of (seed, stream_id, element number) and is stored nowhere
+ * (the adapters' dropout, lazy_lora/core/lora_layer.py:104-139): with word i = word i % 4 of Philox4x32-7
+ * at counter (i / 4 as 64 bits, stream_id as 64 bits) under the 64-bit key `seed`,
+ *   y[i] = word i < floor(p 2^32) ? 0 : x[i] / (1 - p).
+ * The gradient is the same call on dy. n elements of dtype MXFP4_F32, _BF16 or _F16; 0 <= p <= 1;
+ * y may be x. seed_device: when not NULL, one 64-bit seed in device memory read by the kernel instead
+ * of `seed` (a captured graph draws a new mask when it changes between replays). */
+int mxfp4_dropout(void *y, const void *x, long long n, double p, uint64_t seed,
+                  const uint64_t *seed_device, uint64_t stream_id, int dtype, hipStream_t stream);
 
 /* Phase timing of the routed-layer calls made on the calling thread, the counterpart of the
  * reference's LAZYLORA_PROFILE timings (lazy_lora/trainer/lazy_trainer.py:192-194). While

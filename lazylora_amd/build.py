@@ -12,7 +12,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblazylora_mxfp4.so")
-SOURCES = ["capi.hip", "mx_forward.hip", "mx_backward.hip", "mx_misc.hip", "mx_router.hip", "mx_lora.hip"]
+SOURCES = ["capi.hip", "mx_forward.hip", "mx_backward.hip", "mx_misc.hip", "mx_router.hip", "mx_lora.hip",
+           "mx_dense.hip", "mx_rows.hip"]
 
 # per-file flags: the transposed products keep their accumulators in VGPRs (the MFMA's VGPR
 # form); with the default heuristics the compiler splits them over AGPRs and VGPRs and shuffles

@@ -8,6 +8,7 @@
 #include <type_traits>
 
 #include "../../include/lazylora_mxfp4.h"
+#include "mx_dense.h"
 #include "mx_device.h"
 #include "mx_kernels.h"
 
@@ -1042,6 +1043,180 @@ int mxfp4_router_topk_backward(float* grad_logits, const int64_t* topk_idx, cons
   MX_TRY(mx::launch_router_topk_bwd(grad_logits, reinterpret_cast<const long long*>(topk_idx), grad_w, logits, N, E,
                                     top_k, routed_scaling_factor, renormalize, stream),
          "router_topk_backward");
+  return MXFP4_OK;
+}
+
+// ---------------------------------------------------------------- dense operators
+namespace {
+
+constexpr int kDenseMaxWidth = 1 << 20, kDenseMaxRows = 1 << 24;
+
+int check_ffn(const char* who, int dtype, int M, int D, int F, int Do, int act_kind)
+{
+  static thread_local char msg[160];
+  const auto bad = [&](const char* what) {
+    snprintf(msg, sizeof(msg), "%s: %s", who, what);
+    return fail(MXFP4_EINVAL, "%s", msg);
+  };
+  if (dtype != MXFP4_BF16 && dtype != MXFP4_F16) return bad("dtype must be MXFP4_BF16 or MXFP4_F16");
+  if (act_kind != MXFP4_ACT_SWIGLU && act_kind != MXFP4_ACT_SITU) return bad("unknown activation");
+  if (M < 0 || M > kDenseMaxRows) return bad("M must lie in [0, 2^24]");
+  for (int v : {D, F, Do})
+    if (v <= 0 || v > kDenseMaxWidth || v % 8) return bad("D, F and Do must be multiples of 8 in [8, 2^20]");
+  return MXFP4_OK;
+}
+bool all_aligned16(std::initializer_list<const void*> ps)
+{
+  for (const void* p : ps)
+    if (!aligned16(p)) return false;
+  return true;
+}
+
+}  // namespace
+
+size_t mxfp4_ffn_workspace_size(int M, int D, int F, int Do)
+{
+  (void)M; (void)D; (void)F; (void)Do;
+  return 0;
+}
+
+int mxfp4_ffn_forward(void* y, void* h, float* gu, const void* x, const void* w_gate, const void* w_up,
+                      const void* w_down, const void* gate_delta, const void* up_delta, int dtype, int M, int D, int F,
+                      int Do, int act_kind, void* workspace, size_t workspace_bytes, hipStream_t stream)
+{
+  const int rc = check_ffn("ffn_forward", dtype, M, D, F, Do, act_kind);
+  if (rc != MXFP4_OK) return rc;
+  if (workspace_bytes < mxfp4_ffn_workspace_size(M, D, F, Do))
+    return fail(MXFP4_EWORKSPACE, "ffn_forward: workspace too small%s");
+  if (M == 0) return MXFP4_OK;
+  if (!y || !h || !x || !w_gate || !w_up || !w_down) return fail(MXFP4_EINVAL, "ffn_forward: null pointer%s");
+  if (!all_aligned16({y, h, gu, x, w_gate, w_up, w_down, gate_delta, up_delta, workspace}))
+    return fail(MXFP4_EINVAL, "ffn_forward: pointers must be 16-byte aligned%s");
+  mx::DenseArgs a = {};
+  a.a[0] = a.a[1] = x; a.lda = D;
+  a.b[0] = w_gate; a.b[1] = w_up; a.ldb = D;
+  a.M = M; a.N = F; a.K = D; a.nseg = 1;
+  a.out = h; a.ldo = F; a.split_m = M;
+  a.add0 = gate_delta; a.add1 = up_delta; a.gu = gu; a.act = act_kind;
+  MX_TRY(mx::launch_dense_forward(a, dtype, mx::kDenseGlu, stream), "ffn_forward: gate/up");
+  a = {};
+  a.a[0] = a.a[1] = h; a.lda = F;
+  a.b[0] = a.b[1] = w_down; a.ldb = F;
+  a.M = M; a.N = Do; a.K = F; a.nseg = 1;
+  a.out = y; a.ldo = Do; a.split_m = M;
+  MX_TRY(mx::launch_dense_forward(a, dtype, mx::kDenseStore, stream), "ffn_forward: down");
+  return MXFP4_OK;
+}
+
+int mxfp4_ffn_backward(void* dx, void* dw_gate, void* dw_up, void* dw_down, void* dgu, const void* dy,
+                       const void* grad_h, const void* x, const void* h, const float* gu, const void* w_gate,
+                       const void* w_up, const void* w_down, int dtype, int M, int D, int F, int Do, int act_kind,
+                       void* workspace, size_t workspace_bytes, hipStream_t stream)
+{
+  const int rc = check_ffn("ffn_backward", dtype, M, D, F, Do, act_kind);
+  if (rc != MXFP4_OK) return rc;
+  if (workspace_bytes < mxfp4_ffn_workspace_size(M, D, F, Do))
+    return fail(MXFP4_EWORKSPACE, "ffn_backward: workspace too small%s");
+  if (!dw_gate != !dw_up) return fail(MXFP4_EINVAL, "ffn_backward: dw_gate and dw_up go together%s");
+  if (M > 0 && (!dgu || !dy || !gu || !w_gate || !w_up || !w_down || (dw_gate && !x) || (dw_down && !h)))
+    return fail(MXFP4_EINVAL, "ffn_backward: null pointer%s");
+  if (!all_aligned16({dx, dw_gate, dw_up, dw_down, dgu, dy, grad_h, x, h, gu, w_gate, w_up, w_down, workspace}))
+    return fail(MXFP4_EINVAL, "ffn_backward: pointers must be 16-byte aligned%s");
+  const char* dg = static_cast<const char*>(dgu);
+  mx::DenseArgs a = {};
+  if (M > 0) {
+    a.a[0] = a.a[1] = dy; a.lda = Do;
+    a.b[0] = a.b[1] = w_down; a.ldb = F;
+    a.M = M; a.N = F; a.K = Do; a.nseg = 1;
+    a.out = dgu; a.split_m = M;
+    a.add0 = grad_h; a.gu = const_cast<float*>(gu); a.act = act_kind;
+    MX_TRY(mx::launch_dense_dgrad(a, dtype, mx::kDenseDGlu, stream), "ffn_backward: gate/up gradient");
+  }
+  if (dx && M > 0) {
+    a = {};
+    a.a[0] = dg; a.a[1] = dg + 2LL * F; a.lda = 2LL * F;
+    a.b[0] = w_gate; a.b[1] = w_up; a.ldb = D;
+    a.M = M; a.N = D; a.K = F; a.nseg = 2;
+    a.out = dx; a.ldo = D; a.split_m = M;
+    MX_TRY(mx::launch_dense_dgrad(a, dtype, mx::kDenseStore, stream), "ffn_backward: dx");
+  }
+  if (dw_gate) {
+    a = {};
+    a.a[0] = a.a[1] = dg; a.lda = 2LL * F;
+    a.b[0] = a.b[1] = x; a.ldb = D;
+    a.M = 2 * F; a.N = D; a.K = M; a.nseg = 1;
+    a.out = dw_gate; a.out2 = dw_up; a.split_m = F; a.ldo = D;
+    MX_TRY(mx::launch_dense_wgrad(a, dtype, stream), "ffn_backward: gate/up weights");
+  }
+  if (dw_down) {
+    a = {};
+    a.a[0] = a.a[1] = dy; a.lda = Do;
+    a.b[0] = a.b[1] = h; a.ldb = F;
+    a.M = Do; a.N = F; a.K = M; a.nseg = 1;
+    a.out = dw_down; a.ldo = F; a.split_m = Do;
+    MX_TRY(mx::launch_dense_wgrad(a, dtype, stream), "ffn_backward: down weight");
+  }
+  return MXFP4_OK;
+}
+
+static int check_rows(const char* who, int M, int D, int kind, int dtype)
+{
+  static thread_local char msg[160];
+  const auto bad = [&](const char* what) {
+    snprintf(msg, sizeof(msg), "%s: %s", who, what);
+    return fail(MXFP4_EINVAL, "%s", msg);
+  };
+  if (dtype != MXFP4_F32 && dtype != MXFP4_BF16 && dtype != MXFP4_F16) return bad("dtype must be F32, BF16 or F16");
+  if (kind != MXFP4_NORM_RMS && kind != MXFP4_NORM_LAYER) return bad("unknown norm");
+  if (M < 0 || D < 1 || D > kDenseMaxWidth) return bad("need M >= 0 and D in [1, 2^20]");
+  return MXFP4_OK;
+}
+
+int mxfp4_norm_forward(void* y, float* stats, const void* x, const float* weight, const float* bias, int M, int D,
+                       float eps, int kind, int dtype, hipStream_t stream)
+{
+  const int rc = check_rows("norm_forward", M, D, kind, dtype);
+  if (rc != MXFP4_OK) return rc;
+  if (M == 0) return MXFP4_OK;
+  if (!y || !x) return fail(MXFP4_EINVAL, "norm_forward: null pointer%s");
+  MX_TRY(mx::launch_norm_forward(y, stats, x, weight, bias, M, D, eps, kind, dtype, stream), "norm_forward");
+  return MXFP4_OK;
+}
+
+size_t mxfp4_norm_workspace_size(int M, int D) { return M > 0 && D > 0 ? mx::norm_backward_workspace(M, D) : 0; }
+
+int mxfp4_norm_backward(void* dx, float* dweight, float* dbias, const void* dy, const void* x, const float* weight,
+                        const float* stats, int M, int D, int kind, int dtype, void* workspace, size_t workspace_bytes,
+                        hipStream_t stream)
+{
+  const int rc = check_rows("norm_backward", M, D, kind, dtype);
+  if (rc != MXFP4_OK) return rc;
+  if (M > 0 && (!dx || !dy || !x || !stats)) return fail(MXFP4_EINVAL, "norm_backward: null pointer%s");
+  if (dweight || dbias) {
+    if (workspace_bytes < mxfp4_norm_workspace_size(M, D))
+      return fail(MXFP4_EWORKSPACE, "norm_backward: workspace too small%s");
+    if (M > 0 && (!workspace || !aligned16(workspace)))
+      return fail(MXFP4_EINVAL, "norm_backward: the workspace must be 16-byte aligned%s");
+  }
+  MX_TRY(mx::launch_norm_backward(dx, dweight, dbias, dy, x, weight, stats, M, D, kind, dtype,
+                                  static_cast<float*>(workspace), stream),
+         "norm_backward");
+  return MXFP4_OK;
+}
+
+int mxfp4_dropout(void* y, const void* x, long long n, double p, uint64_t seed, const uint64_t* seed_device,
+                  uint64_t stream_id, int dtype, hipStream_t stream)
+{
+  if (dtype != MXFP4_F32 && dtype != MXFP4_BF16 && dtype != MXFP4_F16)
+    return fail(MXFP4_EINVAL, "dropout: dtype must be F32, BF16 or F16%s");
+  if (!(p >= 0.0 && p <= 1.0)) return fail(MXFP4_EINVAL, "dropout: p must lie in [0, 1]%s");
+  if (n < 0 || n > (1LL << 40)) return fail(MXFP4_EINVAL, "dropout: n must lie in [0, 2^40]%s");
+  if (n == 0) return MXFP4_OK;
+  if (!y || !x) return fail(MXFP4_EINVAL, "dropout: null pointer%s");
+  // p = 1 drops every word (threshold 2^32); its scale is never used
+  const float scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f;
+  MX_TRY(mx::launch_dropout(y, x, n, (uint64_t)(p * 4294967296.0), scale, seed, seed_device, stream_id, dtype, stream),
+         "dropout");
   return MXFP4_OK;
 }
 

@@ -19,6 +19,7 @@ Differences from the reference, all deliberate:
     Nothing here falls back to a CPU implementation: the MXFP4Kernel methods run on the GPU
     or raise.
 """
+import contextlib
 import ctypes
 import os
 import sys
@@ -33,7 +34,9 @@ ACT_SWIGLU = 0
 ACT_SITU = 1
 _ACTS = {"swiglu": ACT_SWIGLU, "situ": ACT_SITU, "situ_glu": ACT_SITU, ACT_SWIGLU: ACT_SWIGLU, ACT_SITU: ACT_SITU}
 
-F32, BF16, I32, I64 = 0, 1, 2, 3
+F32, BF16, I32, I64, F16 = 0, 1, 2, 3, 4
+NORM_RMS, NORM_LAYER = 0, 1
+_FLOATS = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 MOE_SAVE = 1
 MOE_REUSE_FORWARD = 2
 MOE_BWD_LAYOUT = 4
@@ -105,6 +108,21 @@ def _load_library() -> ctypes.CDLL:
     lib.mxfp4_router_topk.argtypes = [vp, vp, vp, vp, ci, ci, ci, ctypes.c_float, ci, vp]
     lib.mxfp4_router_topk_backward.restype = ci
     lib.mxfp4_router_topk_backward.argtypes = [vp, vp, vp, vp, ci, ci, ci, ctypes.c_float, ci, vp]
+    cll, cu64 = ctypes.c_longlong, ctypes.c_uint64
+    lib.mxfp4_ffn_workspace_size.restype = sz
+    lib.mxfp4_ffn_workspace_size.argtypes = [ci, ci, ci, ci]
+    lib.mxfp4_ffn_forward.restype = ci
+    lib.mxfp4_ffn_forward.argtypes = [vp] * 9 + [ci] * 6 + [vp, sz, vp]
+    lib.mxfp4_ffn_backward.restype = ci
+    lib.mxfp4_ffn_backward.argtypes = [vp] * 13 + [ci] * 6 + [vp, sz, vp]
+    lib.mxfp4_norm_forward.restype = ci
+    lib.mxfp4_norm_forward.argtypes = [vp] * 5 + [ci, ci, ctypes.c_float, ci, ci, vp]
+    lib.mxfp4_norm_workspace_size.restype = sz
+    lib.mxfp4_norm_workspace_size.argtypes = [ci, ci]
+    lib.mxfp4_norm_backward.restype = ci
+    lib.mxfp4_norm_backward.argtypes = [vp] * 7 + [ci] * 4 + [vp, sz, vp]
+    lib.mxfp4_dropout.restype = ci
+    lib.mxfp4_dropout.argtypes = [vp, vp, cll, ctypes.c_double, cu64, vp, cu64, ci, vp]
     lib.mxfp4_moe_timing.restype = ci
     lib.mxfp4_moe_timing.argtypes = [ci]
     lib.mxfp4_moe_timed_calls.restype = ci
@@ -386,6 +404,123 @@ class MXFP4Kernel:
         if not 1 <= top_k <= min(E, 64):
             raise ValueError(f"top_k must lie in [1, min(E, 64)] = [1, {min(E, 64)}], got {top_k}")
 
+    # -- dense operators ---------------------------------------------------------------------
+    # Device tensors only (ValueError otherwise); lazylora_amd.dense wraps these in autograd.
+    def ffn_forward(self, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+                    act="swiglu", gate_delta: Optional[torch.Tensor] = None,
+                    up_delta: Optional[torch.Tensor] = None, save_for_backward: bool = False):
+        """(y [M, Do], h [M, F], gu) of the gated feed-forward block for x [M, D], all bfloat16 or all
+        float16: gate = x Wg^T (+ gate_delta), up = x Wu^T (+ up_delta), h = GLU(gate, up),
+        y = h Wd^T with w_gate, w_up [F, D] and w_down [Do, F] (mxfp4_ffn_forward). gu is the fp32
+        gate | up [M, 2F] that ffn_backward takes, or None without save_for_backward."""
+        c = _FfnCall(x, w_gate, w_up, w_down, act)
+        gd, ud = c.like_h(gate_delta, "gate_delta"), c.like_h(up_delta, "up_delta")
+        y, h = c.new(c.M, c.Do), c.new(c.M, c.F)
+        gu = torch.empty((c.M, 2 * c.F), dtype=torch.float32, device=c.dev) if save_for_backward else None
+        if c.M:
+            ws, nws = c.workspace(self.lib)
+            with _on(c.dev):
+                _check(self.lib.mxfp4_ffn_forward(y.data_ptr(), h.data_ptr(), _ptr(gu), c.x.data_ptr(),
+                                                  *[w.data_ptr() for w in c.w], _ptr(gd), _ptr(ud), c.dtype, c.M, c.D,
+                                                  c.F, c.Do, c.act, _ptr(ws), nws, _stream(c.dev)), self.lib)
+        return y, h, gu
+
+    def ffn_backward(self, grad_y: torch.Tensor, gu: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                     w_down: torch.Tensor, act="swiglu", grad_h: Optional[torch.Tensor] = None,
+                     x: Optional[torch.Tensor] = None, h: Optional[torch.Tensor] = None, need_x: bool = True,
+                     need_w_in: bool = False, need_w_down: bool = False):
+        """(dgu, dx, dw_gate, dw_up, dw_down) for dL/dy and, if h was used elsewhere, dL/dh = grad_h
+        (mxfp4_ffn_backward). dgu [M, 2F] = dL/dgate | dL/dup, also the gradients of the deltas. The others
+        are None unless asked for: dx; dw_gate and dw_up (need_w_in, takes the forward's x); dw_down
+        (need_w_down, takes its h)."""
+        if need_w_in and x is None:
+            raise ValueError("need_w_in=True takes the forward's x")
+        if need_w_down and h is None:
+            raise ValueError("need_w_down=True takes the forward's h")
+        c = _FfnCall(x, w_gate, w_up, w_down, act, rows=grad_y)
+        gy = c.take(grad_y, "grad_y", (c.M, c.Do))
+        gh, h = c.like_h(grad_h, "grad_h"), c.like_h(h, "h")
+        if gu.dtype != torch.float32 or tuple(gu.shape) != (c.M, 2 * c.F) or gu.device != c.dev:
+            raise ValueError(f"gu must be the forward's float32 [{c.M}, {2 * c.F}]")
+        gu = _aligned(gu.contiguous())
+        dgu = c.new(c.M, 2 * c.F)
+        dx = c.new(c.M, c.D) if need_x else None
+        dwg, dwu = (c.new(c.F, c.D), c.new(c.F, c.D)) if need_w_in else (None, None)
+        dwd = c.new(c.Do, c.F) if need_w_down else None
+        ws, nws = c.workspace(self.lib)
+        with _on(c.dev):
+            _check(self.lib.mxfp4_ffn_backward(_ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd), dgu.data_ptr(),
+                                               gy.data_ptr(), _ptr(gh), _ptr(c.x), _ptr(h), gu.data_ptr(),
+                                               *[w.data_ptr() for w in c.w], c.dtype, c.M, c.D, c.F, c.Do, c.act,
+                                               _ptr(ws), nws, _stream(c.dev)), self.lib)
+        return dgu, dx, dwg, dwu, dwd
+
+    def norm_forward(self, x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                     bias: Optional[torch.Tensor] = None, eps: float = 1e-5, kind: int = NORM_RMS,
+                     save_for_backward: bool = False):
+        """(y, stats) of the RMS or layer norm of x [M, D] (float32, bfloat16 or float16) over its last
+        axis, weight and bias [D] float32 or None (mxfp4_norm_forward); stats [2, M] float32 is what
+        norm_backward takes, or None without save_for_backward."""
+        M, D, dt = _rows(x)
+        w, b = _vector(weight, D, x.device, "weight"), _vector(bias, D, x.device, "bias")
+        xc = x.contiguous()
+        y = torch.empty_like(xc)
+        stats = torch.empty((2, M), dtype=torch.float32, device=x.device) if save_for_backward else None
+        if M:
+            with _on(x.device):
+                _check(self.lib.mxfp4_norm_forward(y.data_ptr(), _ptr(stats), xc.data_ptr(), _ptr(w), _ptr(b), M, D,
+                                                   float(eps), kind, dt, _stream(x.device)), self.lib)
+        return y, stats
+
+    def norm_backward(self, grad_y: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor],
+                      stats: torch.Tensor, kind: int = NORM_RMS, need_weight: bool = False,
+                      need_bias: bool = False):
+        """(dx, dweight, dbias) for dL/dy (mxfp4_norm_backward); the column gradients are float32, None
+        unless asked for."""
+        M, D, dt = _rows(x)
+        if grad_y.shape != x.shape or grad_y.dtype != x.dtype or grad_y.device != x.device:
+            raise ValueError(f"grad_y must be {x.dtype} {tuple(x.shape)} on x's device")
+        if stats.dtype != torch.float32 or tuple(stats.shape) != (2, M) or stats.device != x.device:
+            raise ValueError(f"stats must be the forward's float32 [2, {M}]")
+        w = _vector(weight, D, x.device, "weight")
+        xc, gy, stats = x.contiguous(), grad_y.contiguous(), stats.contiguous()
+        dx = torch.empty_like(xc)
+        dw = torch.empty(D, dtype=torch.float32, device=x.device) if need_weight else None
+        db = torch.empty(D, dtype=torch.float32, device=x.device) if need_bias else None
+        nws = int(self.lib.mxfp4_norm_workspace_size(M, D)) if need_weight or need_bias else 0
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
+        with _on(x.device):
+            _check(self.lib.mxfp4_norm_backward(dx.data_ptr(), _ptr(dw), _ptr(db), gy.data_ptr(), xc.data_ptr(),
+                                                _ptr(w), stats.data_ptr(), M, D, kind, dt, _ptr(ws), nws,
+                                                _stream(x.device)), self.lib)
+        return dx, dw, db
+
+    def dropout(self, x: torch.Tensor, p: float, seed, stream: int = 0) -> torch.Tensor:
+        """x / (1 - p) where kept, 0 where dropped; the mask is a function of (seed, stream, element
+        number in row-major order) and is stored nowhere (mxfp4_dropout). seed: a whole number in
+        [0, 2^64), or a one-element int64 tensor on x's device, read by the kernel (for captured graphs).
+        stream: a second number in [0, 2^64) that tells calls under one seed apart."""
+        if not x.is_cuda or x.dtype not in _FLOATS:
+            raise ValueError("x must be a float32, bfloat16 or float16 tensor on the HIP device")
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must lie in [0, 1], got {p}")
+        if not 0 <= stream < 2 ** 64:
+            raise ValueError(f"stream must lie in [0, 2^64), got {stream}")
+        on_dev = torch.is_tensor(seed)
+        if on_dev:
+            if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device:
+                raise ValueError("a seed tensor must hold one int64 on x's device")
+        elif not 0 <= seed < 2 ** 64:
+            raise ValueError(f"seed must lie in [0, 2^64), got {seed}")
+        xc = x.contiguous()
+        y = torch.empty_like(xc)
+        if xc.numel():
+            with _on(x.device):
+                _check(self.lib.mxfp4_dropout(y.data_ptr(), xc.data_ptr(), xc.numel(), float(p),
+                                              0 if on_dev else int(seed), seed.data_ptr() if on_dev else None,
+                                              int(stream), _FLOATS[x.dtype], _stream(x.device)), self.lib)
+        return y
+
     def moe_workspace_bytes(self, N: int, k: int, E: int, D: int, F: int) -> int:
         return int(self.lib.mxfp4_moe_workspace_size(N, k, E, D, F))
 
@@ -422,6 +557,78 @@ def _check_weight(packed: torch.Tensor, scales: torch.Tensor, R: int, K: int) ->
         raise ValueError(f"K = {K} is not a multiple of the MX block size 32")
     if tuple(scales.shape) != (R, K // 32):
         raise ValueError(f"scales must be [{R}, {K // 32}], got {tuple(scales.shape)}")
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _on(dev: torch.device):
+    """Makes dev the current device for a launch on one of its streams."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _rows(x: torch.Tensor):
+    """(M, D, dtype code) of a norm's x."""
+    if x.dim() != 2 or x.shape[1] == 0 or not x.is_cuda or x.dtype not in _FLOATS:
+        raise ValueError("x must be a float32, bfloat16 or float16 tensor [M, D], D > 0, on the HIP device, got "
+                         f"{x.dtype} {tuple(x.shape)} on {x.device}")
+    return x.shape[0], x.shape[1], _FLOATS[x.dtype]
+
+
+def _vector(t: Optional[torch.Tensor], D: int, dev: torch.device, name: str):
+    if t is None:
+        return None
+    if tuple(t.shape) != (D,) or t.dtype != torch.float32 or t.device != dev:
+        raise ValueError(f"{name} must be float32 [{D}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.contiguous()
+
+
+class _FfnCall:
+    """Validated arguments of one call of the gated feed-forward block. Without x (a backward that needs
+    no weight gradients) the row count is that of `rows`."""
+
+    def __init__(self, x, w_gate, w_up, w_down, act, rows=None):
+        if act not in _ACTS:
+            raise ValueError(f"unknown activation {act!r}")
+        self.act = _ACTS[act]
+        first = x if x is not None else rows
+        self.torch_dtype, self.dev = first.dtype, first.device
+        if self.torch_dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"the feed-forward block takes bfloat16 or float16, got {self.torch_dtype}")
+        if self.dev.type != "cuda":
+            raise ValueError(f"the feed-forward block takes tensors on the HIP device, got {self.dev}")
+        if first.dim() != 2 or w_gate.dim() != 2 or w_down.dim() != 2:
+            raise ValueError("x and the weights must be 2-D")
+        self.M = first.shape[0]
+        self.F, self.D = w_gate.shape
+        self.Do = w_down.shape[0]
+        for name, n in (("D", self.D), ("F", self.F), ("Do", self.Do)):
+            if n == 0 or n % 8:
+                raise ValueError(f"{name} = {n} must be a positive multiple of 8")
+        self.x = None if x is None else self.take(x, "x", (self.M, self.D))
+        self.w = (self.take(w_gate, "w_gate", (self.F, self.D)), self.take(w_up, "w_up", (self.F, self.D)),
+                  self.take(w_down, "w_down", (self.Do, self.F)))
+
+    def take(self, t, name, shape):
+        if tuple(t.shape) != shape or t.dtype != self.torch_dtype or t.device != self.dev:
+            raise ValueError(f"{name} must be {self.torch_dtype} {list(shape)} on {self.dev}, got {t.dtype} "
+                             f"{list(t.shape)} on {t.device}")
+        return _aligned(t.contiguous())
+
+    def like_h(self, t, name):
+        return None if t is None else self.take(t, name, (self.M, self.F))
+
+    def new(self, *shape):
+        return torch.empty(shape, dtype=self.torch_dtype, device=self.dev)
+
+    @property
+    def dtype(self):
+        return _FLOATS[self.torch_dtype]
+
+    def workspace(self, lib):
+        n = int(lib.mxfp4_ffn_workspace_size(self.M, self.D, self.F, self.Do))
+        return (torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None), n
 
 
 class _RoutedCall:
