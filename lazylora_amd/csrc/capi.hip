@@ -1076,8 +1076,14 @@ bool all_aligned16(std::initializer_list<const void*> ps)
 
 size_t mxfp4_ffn_workspace_size(int M, int D, int F, int Do)
 {
-  (void)M; (void)D; (void)F; (void)Do;
-  return 0;
+  if (M <= 0 || D <= 0 || F <= 0 || Do <= 0) return 0;
+  // the products of a call run one after another and share the bytes
+  return std::max({mx::dense_partial_bytes(mx::kDenseForward, mx::kDenseGlu, M, F, D, 1),
+                   mx::dense_partial_bytes(mx::kDenseForward, mx::kDenseStore, M, Do, F, 1),
+                   mx::dense_partial_bytes(mx::kDenseDgrad, mx::kDenseDGlu, M, F, Do, 1),
+                   mx::dense_partial_bytes(mx::kDenseDgrad, mx::kDenseStore, M, D, F, 2),
+                   mx::dense_partial_bytes(mx::kDenseWgrad, mx::kDenseStore, 2 * F, D, M, 1),
+                   mx::dense_partial_bytes(mx::kDenseWgrad, mx::kDenseStore, Do, F, M, 1)});
 }
 
 int mxfp4_ffn_forward(void* y, void* h, float* gu, const void* x, const void* w_gate, const void* w_up,
@@ -1092,19 +1098,20 @@ int mxfp4_ffn_forward(void* y, void* h, float* gu, const void* x, const void* w_
   if (!y || !h || !x || !w_gate || !w_up || !w_down) return fail(MXFP4_EINVAL, "ffn_forward: null pointer%s");
   if (!all_aligned16({y, h, gu, x, w_gate, w_up, w_down, gate_delta, up_delta, workspace}))
     return fail(MXFP4_EINVAL, "ffn_forward: pointers must be 16-byte aligned%s");
+  float* part = static_cast<float*>(workspace);
   mx::DenseArgs a = {};
   a.a[0] = a.a[1] = x; a.lda = D;
   a.b[0] = w_gate; a.b[1] = w_up; a.ldb = D;
   a.M = M; a.N = F; a.K = D; a.nseg = 1;
   a.out = h; a.ldo = F; a.split_m = M;
   a.add0 = gate_delta; a.add1 = up_delta; a.gu = gu; a.act = act_kind;
-  MX_TRY(mx::launch_dense_forward(a, dtype, mx::kDenseGlu, stream), "ffn_forward: gate/up");
+  MX_TRY(mx::launch_dense(mx::kDenseForward, mx::kDenseGlu, a, dtype, part, stream), "ffn_forward: gate/up");
   a = {};
   a.a[0] = a.a[1] = h; a.lda = F;
   a.b[0] = a.b[1] = w_down; a.ldb = F;
   a.M = M; a.N = Do; a.K = F; a.nseg = 1;
   a.out = y; a.ldo = Do; a.split_m = M;
-  MX_TRY(mx::launch_dense_forward(a, dtype, mx::kDenseStore, stream), "ffn_forward: down");
+  MX_TRY(mx::launch_dense(mx::kDenseForward, mx::kDenseStore, a, dtype, part, stream), "ffn_forward: down");
   return MXFP4_OK;
 }
 
@@ -1123,6 +1130,7 @@ int mxfp4_ffn_backward(void* dx, void* dw_gate, void* dw_up, void* dw_down, void
   if (!all_aligned16({dx, dw_gate, dw_up, dw_down, dgu, dy, grad_h, x, h, gu, w_gate, w_up, w_down, workspace}))
     return fail(MXFP4_EINVAL, "ffn_backward: pointers must be 16-byte aligned%s");
   const char* dg = static_cast<const char*>(dgu);
+  float* part = static_cast<float*>(workspace);
   mx::DenseArgs a = {};
   if (M > 0) {
     a.a[0] = a.a[1] = dy; a.lda = Do;
@@ -1130,7 +1138,7 @@ int mxfp4_ffn_backward(void* dx, void* dw_gate, void* dw_up, void* dw_down, void
     a.M = M; a.N = F; a.K = Do; a.nseg = 1;
     a.out = dgu; a.split_m = M;
     a.add0 = grad_h; a.gu = const_cast<float*>(gu); a.act = act_kind;
-    MX_TRY(mx::launch_dense_dgrad(a, dtype, mx::kDenseDGlu, stream), "ffn_backward: gate/up gradient");
+    MX_TRY(mx::launch_dense(mx::kDenseDgrad, mx::kDenseDGlu, a, dtype, part, stream), "ffn_backward: gate/up gradient");
   }
   if (dx && M > 0) {
     a = {};
@@ -1138,7 +1146,7 @@ int mxfp4_ffn_backward(void* dx, void* dw_gate, void* dw_up, void* dw_down, void
     a.b[0] = w_gate; a.b[1] = w_up; a.ldb = D;
     a.M = M; a.N = D; a.K = F; a.nseg = 2;
     a.out = dx; a.ldo = D; a.split_m = M;
-    MX_TRY(mx::launch_dense_dgrad(a, dtype, mx::kDenseStore, stream), "ffn_backward: dx");
+    MX_TRY(mx::launch_dense(mx::kDenseDgrad, mx::kDenseStore, a, dtype, part, stream), "ffn_backward: dx");
   }
   if (dw_gate) {
     a = {};
@@ -1146,7 +1154,7 @@ int mxfp4_ffn_backward(void* dx, void* dw_gate, void* dw_up, void* dw_down, void
     a.b[0] = a.b[1] = x; a.ldb = D;
     a.M = 2 * F; a.N = D; a.K = M; a.nseg = 1;
     a.out = dw_gate; a.out2 = dw_up; a.split_m = F; a.ldo = D;
-    MX_TRY(mx::launch_dense_wgrad(a, dtype, stream), "ffn_backward: gate/up weights");
+    MX_TRY(mx::launch_dense(mx::kDenseWgrad, mx::kDenseStore, a, dtype, part, stream), "ffn_backward: gate/up weights");
   }
   if (dw_down) {
     a = {};
@@ -1154,7 +1162,7 @@ int mxfp4_ffn_backward(void* dx, void* dw_gate, void* dw_up, void* dw_down, void
     a.b[0] = a.b[1] = h; a.ldb = F;
     a.M = Do; a.N = F; a.K = M; a.nseg = 1;
     a.out = dw_down; a.ldo = F; a.split_m = Do;
-    MX_TRY(mx::launch_dense_wgrad(a, dtype, stream), "ffn_backward: down weight");
+    MX_TRY(mx::launch_dense(mx::kDenseWgrad, mx::kDenseStore, a, dtype, part, stream), "ffn_backward: down weight");
   }
   return MXFP4_OK;
 }

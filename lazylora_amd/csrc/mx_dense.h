@@ -31,14 +31,21 @@ struct DenseArgs {
   const void* add1;  // kDenseGlu: up delta or null
   float* gu;         // [M, 2N] fp32 gate | up: kDenseGlu writes it (null: not kept), kDenseDGlu reads it
   int act;
+  // set by the launcher: the tile grid, and the cut of K into `splits` runs of `run` steps, whose sums go to
+  // partial [splits][M][N] (kDenseGlu: [splits][M][2N], gate | up) and meet in a second kernel (null: one run)
   int tiles_m, tiles_n;
+  int splits, run;
+  float* partial;
 };
 
-// dtype: MXFP4_BF16 or MXFP4_F16. The three shapes the block needs: A and B K-major (forward
-// products), A K-major and B row-major (gradients of activations), both row-major (weight gradients).
-hipError_t launch_dense_forward(const DenseArgs& a, int dtype, DenseEpi epi, hipStream_t s);
-hipError_t launch_dense_dgrad(const DenseArgs& a, int dtype, DenseEpi epi, hipStream_t s);
-hipError_t launch_dense_wgrad(const DenseArgs& a, int dtype, hipStream_t s);
+// The three shapes of product the block needs: A and B K-major (forward products), A K-major and B
+// row-major (gradients of activations), both row-major (weight gradients).
+enum DenseShape : int { kDenseForward = 0, kDenseDgrad = 1, kDenseWgrad = 2 };
+
+// Bytes of partial sums that launch_dense may use for a product of these sizes, and the product
+// (dtype MXFP4_BF16 or MXFP4_F16; partial: that many bytes).
+size_t dense_partial_bytes(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg);
+hipError_t launch_dense(DenseShape shape, DenseEpi epi, const DenseArgs& a, int dtype, float* partial, hipStream_t s);
 
 // Layer / RMS norm over rows of D elements (dtype MXFP4_F32, _BF16 or _F16), fp32 statistics
 // stats[0:M] = 1 / sqrt(var + eps), stats[M:2M] = mean (layer norm). weight and bias fp32 or null.

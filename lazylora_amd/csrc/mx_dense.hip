@@ -5,6 +5,8 @@
 //              dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 // One tile kernel does them all: the GLU and its derivative are epilogues on the fp32 sums, so
 // neither g | u (except for a backward) nor dh is ever stored for a later pass to read.
+#include <algorithm>
+
 #include "../../include/lazylora_mxfp4.h"
 #include "mx_dense.h"
 #include "mx_device.h"
@@ -14,22 +16,23 @@ namespace mx {
 namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <typename T>
 struct Elem;
 template <>
 struct Elem<__bf16> {
-  static MX_DEV f32x4 mfma(i32x4 a, i32x4 b, f32x4 c)
+  static MX_DEV f32x16 mfma(i32x4 a, i32x4 b, f32x16 c)
   {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                    0, 0);
   }
 };
 template <>
 struct Elem<_Float16> {
-  static MX_DEV f32x4 mfma(i32x4 a, i32x4 b, f32x4 c)
+  static MX_DEV f32x16 mfma(i32x4 a, i32x4 b, f32x16 c)
   {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                   0);
   }
 };
@@ -51,6 +54,21 @@ MX_DEV void store_f(void* p, long long i, const float (&v)[NV])
 #pragma unroll
   for (int j = 0; j < NV; ++j) t[j] = (T)v[j];
   *reinterpret_cast<tv*>(static_cast<T*>(p) + i) = t;
+}
+
+MX_DEV void store_sums(float* p, const float (&v)[8])
+{
+  *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+  *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+}
+MX_DEV void add_sums(const float* p, float (&v)[8])
+{
+  const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[j] += a[j];
+    v[4 + j] += b[j];
+  }
 }
 
 // The epilogues, on NV neighbouring columns n.. of row m.
@@ -114,31 +132,30 @@ MX_DEV void epi_dglu(const DenseArgs& p, int m, int n, float (&v)[NV])
 }
 
 // ------------------------------------------------------------------ the tile kernel
-// A work-group of four waves (2 x 2) makes a tile of 32 FM rows x 32 FN columns, each wave FM x FN
-// blocks of v_mfma_f32_16x16x32. The weights' side is the MFMA's first operand, so a lane ends up
-// with 4 neighbouring columns of one row.
+// A work-group of WM x WN waves makes a tile of 32 FM WM rows x 32 FN WN columns, each wave FM x FN
+// blocks of v_mfma_f32_32x32x16 (twice the products per operand byte read of the 16 x 16 form: less power,
+// and half the instructions between which reads and copies have to fit). The weights' side is the
+// MFMA's first operand, so a lane ends up with runs of 4 neighbouring columns of one row.
 //
-// K goes in steps of 64 through two LDS stages, filled by 16-byte buffer loads that write LDS
+// K goes in steps of 64 through NS LDS stages, filled by 16-byte buffer loads that write LDS
 // directly. A lane whose element lies past a row, column or K edge gets an offset past its buffer's
 // count, so it loads zeros: odd sizes cost no branches in the loop. Stage layouts, 16-byte pieces
 // placed so that neither kind of read meets bank conflicts (LDS has 64 banks of 4 bytes):
-//  * K-major operand: rows of 128 bytes (64 K terms); piece c of row r at place c ^ key(r). A wave
-//    reads fragments of 16 rows x 32 terms with ds_read_b128, lane l row l % 16, terms 8 (l / 16)..+7;
-//    key gives the 16 rows of a fragment 8 values per row parity, 256 bytes in all.
-//    The columns of a B fragment pair are taken interleaved (columns 8 a + 4 f + j of 32 for fragment
-//    f, a = 0..3, j = 0..3), so that a lane holds 8 neighbouring columns of the result.
-//  * row-major operand: K terms of 64 FM bytes; 32-byte chunk c of term k at place c ^ g(k). The
-//    fragments come from ds_read_b64_tr_b16, which hands lane t of a 16-lane group the 4 terms of
-//    column t from 4 terms x 16 columns; the 8 terms that 32 lanes read at once get 8 places.
+//  * K-major operand: rows of 128 bytes (64 K terms); piece c of row r at place c ^ key_k(r). A wave
+//    reads fragments of 32 rows x 16 terms with ds_read_b128, lane l row l % 32, terms 8 (l / 32)..+7;
+//    the key takes 8 values over the 8 rows of each parity, so 16 rows' pieces fill 256 bytes.
+//  * row-major operand: K terms of 64 bytes per block; 32-byte chunk c of term k at place c ^ key_t(k).
+//    The fragments come from ds_read_b64_tr_b16, which hands lane t of a 16-lane group the 4 terms of
+//    column t from 4 terms x 16 columns; 32 lanes read 4 terms x 64 bytes at once, which the key puts
+//    side by side.
 constexpr int kDenseStep = 64;
 constexpr uint32_t kOob = 0x80000000u;  // at or past every buffer's count
 
-MX_DEV int key_a(int r) { return (r >> 1) & 7; }
-MX_DEV int key_b(int r) { return ((r >> 1) & 1) | ((r >> 2) & 2) | ((r >> 2) & 4); }
-template <int FX>
+MX_DEV int key_k(int r) { return (r >> 1) & 7; }
+template <int BLOCKS>
 MX_DEV int key_t(int k)
 {
-  return FX >= 4 ? (k & 3) + ((k >> 1) & 4) : ((k >> 1) & 1) + ((k >> 2) & 2);
+  return BLOCKS >= 4 ? (k & 3) << 1 : k & 2;
 }
 
 MX_DEV i32x4 rsrc_words(const void* base, uint32_t bytes)
@@ -159,68 +176,70 @@ MX_DEV void dma16_buf(i32x4 r, uint32_t voff, uint32_t soff, uint32_t lds)
 
 typedef __attribute__((address_space(3))) const i32x4 lds_i32x4;
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+typedef __attribute__((address_space(3))) const f32x4 lds_f32x4;
+typedef __attribute__((address_space(3))) f32x4 lds_f32x4_w;
 
-// One operand's side of the loop: copies into a stage and fragment reads from it. FX 16-row blocks per
-// wave, TR: row-major source. ROLE 0: A, 1: B, 2: B of the gate and up matrices (columns of a wave:
-// 8 FX of gate, then the same of up).
-template <int FX, bool TR, int ROLE>
+// One operand's side of the loop: copies into a stage and fragment reads from it. WX waves of FX 32-row
+// blocks each share the operand among NW waves, TR: row-major source, GLU: B of the gate and up
+// matrices (columns of a wave: 16 FX of gate, then the same of up).
+template <int FX, int WX, int NW, bool TR, bool GLU>
 struct Side {
-  static constexpr int kReads = TR ? 2 * FX : FX;  // LDS reads per fragment set
-  uint32_t voff[FX];  // this lane's source offset of each of its wave's FX copies per step
-  uint32_t raddr[TR ? FX : 2];
+  static constexpr int kBlocks = FX * WX;
+  static constexpr int kCopies = 4 * kBlocks / NW;     // 1 KiB copies of a wave per step
+  static constexpr int kReads = (TR ? 2 : 1) * 2 * FX;  // LDS reads of a half step's fragments
+  static_assert(4 * kBlocks % NW == 0 && kCopies > 0, "the waves share the copies evenly");
+  uint32_t voff[kCopies];  // this lane's source offset of each of its wave's copies
+  uint32_t raddr[TR ? FX : 1];
   const char* base[2];
   long long step_bytes;  // TR: bytes from one K term to the next
   long long col_bytes;   // TR: bytes from a term's start to this tile's first column
-  int kc0;               // K-major: first K term of this lane's piece of copy 0, before the copies' key bits
 
   // x0: first row (column) of the tile; X: rows (columns) there are
   MX_DEV void init(const void* const* src, long long ld, int x0, int X, int wave, int lane, int wx)
   {
-    const int w = wave;
     if constexpr (!TR) {
-      const int m = ROLE == 2 ? (w & 1) : 0;
-      base[0] = static_cast<const char*>(src[m]) + (long long)x0 * ld * 2;
-      base[1] = ROLE == 2 ? base[0] : static_cast<const char*>(src[1]) + (long long)x0 * ld * 2;
+      base[0] = static_cast<const char*>(src[0]) + (long long)x0 * ld * 2;
+      base[1] = static_cast<const char*>(src[1]) + (long long)x0 * ld * 2;
 #pragma unroll
-      for (int j = 0; j < FX; ++j) {
-        const int r = 8 * (w * FX + j) + (lane >> 3);
-        const int c = (lane & 7) ^ (ROLE == 0 ? key_a(r) : key_b(r));
-        const int row = ROLE == 2 ? (w >> 1) * 8 * FX + r % (8 * FX) : r;
+      for (int j = 0; j < kCopies; ++j) {
+        const int r = 8 * (wave * kCopies + j) + (lane >> 3);
+        const int c = (lane & 7) ^ key_k(r);
+        const int row = GLU ? r / (32 * FX) * 16 * FX + r % (16 * FX) : r;
         voff[j] = x0 + row < X ? (uint32_t)(row * ld * 2) + c * 16 : kOob;
       }
-      const int i = lane & 15, b = lane >> 4;
-      const int r = wx * 16 * FX + (ROLE == 0 ? i : 8 * (i >> 2) + (i & 3));
-      raddr[0] = r * 128 + ((b ^ (i >> 1)) << 4);
-      raddr[1] = raddr[0] ^ 64;
+      const int i = lane & 31;
+      raddr[0] = (wx * 32 * FX + i) * 128 + (((lane >> 5) ^ key_k(i)) << 4);
     } else {
-      constexpr int kRow = 64 * FX, kLanes = 4 * FX, kPer = 64 / kLanes;
+      constexpr int kRow = 64 * kBlocks, kLanes = 4 * kBlocks, kPer = 64 / kLanes;
       col_bytes = (long long)x0 * 2;
       step_bytes = ld * 2;
       base[0] = static_cast<const char*>(src[0]) + col_bytes;
       base[1] = static_cast<const char*>(src[1]) + col_bytes;
 #pragma unroll
-      for (int j = 0; j < FX; ++j) {
-        const int k = (w * FX + j) * kPer + lane / kLanes;
+      for (int j = 0; j < kCopies; ++j) {
+        const int k = (wave * kCopies + j) * kPer + lane / kLanes;
         const int pos = lane % kLanes;
-        const int c = ((pos >> 1) ^ key_t<FX>(k)) * 2 + (pos & 1);
+        const int c = ((pos >> 1) ^ key_t<kBlocks>(k)) * 2 + (pos & 1);
         voff[j] = x0 + c * 8 < X ? (uint32_t)(k * ld * 2) + c * 16 : kOob;
       }
-      const int t = lane & 15, b = lane >> 4;
-      const int k = 8 * b + (t >> 2);
+      const int t = lane & 15;
+      const int k = 8 * (lane >> 5) + (t >> 2);
 #pragma unroll
-      for (int f = 0; f < FX; ++f) raddr[f] = k * kRow + (((wx * FX + f) ^ key_t<FX>(k)) << 5) + (t & 3) * 8;
+      for (int f = 0; f < FX; ++f)
+        raddr[f] = k * kRow + (((2 * (wx * FX + f) + ((lane >> 4) & 1)) ^ key_t<kBlocks>(k)) << 5) + (t & 3) * 8;
     }
   }
 
   // Copies j of the step at terms k0 of segment seg (nothing but zeros from k0 >= K) to LDS address lds.
   MX_DEV void copy(int j, int seg, int k0, int K, uint32_t lds, int wave, int lane) const
   {
-    const uint32_t dst = lds + (wave * FX + j) * 1024;
+    const uint32_t dst = lds + (wave * kCopies + j) * 1024;
     if constexpr (!TR) {
-      const int r = 8 * (wave * FX + j) + (lane >> 3);
-      const int c = (lane & 7) ^ (ROLE == 0 ? key_a(r) : key_b(r));
+      const int q = wave * kCopies + j;
+      const int c = (lane & 7) ^ key_k(8 * q + (lane >> 3));
       const uint32_t v = k0 + 8 * c < K ? voff[j] : kOob;
-      dma16_buf(rsrc_words(seg ? base[1] : base[0], 0x7FFFFFFFu), v, (uint32_t)k0 * 2u, dst);
+      dma16_buf(rsrc_words((GLU ? (q / (2 * FX)) & 1 : seg) ? base[1] : base[0], 0x7FFFFFFFu), v, (uint32_t)k0 * 2u,
+                dst);
     } else {
       const int left = K - k0 < kDenseStep ? K - k0 : kDenseStep;
       const uint32_t n = left > 0 ? (uint32_t)(left * step_bytes - col_bytes) : 0u;
@@ -228,174 +247,363 @@ struct Side {
     }
   }
 
-  // Read i (0 .. kReads - 1) of the fragments of half h from the stage at lds.
-  MX_DEV void read(int i, int h, uint32_t lds, i32x4 (&f)[FX]) const
+  // Read i (0 .. kReads - 1) of the fragments of half h (terms 32 h..: two slices of 16) from the stage at lds.
+  template <int I, int H>
+  MX_DEV void read(uint32_t lds, i32x4 (&f)[2][FX]) const
   {
+    constexpr int S = I / (kReads / 2), J = I % (kReads / 2);
     if constexpr (!TR) {
-      const uint32_t imm = ROLE == 0 ? i * 2048 : (i >> 1) * 4096 + (i & 1) * 512;
-      f[i] = *reinterpret_cast<lds_i32x4*>(lds + raddr[h] + imm);
+      f[S][J] = *reinterpret_cast<lds_i32x4*>(lds + (raddr[0] ^ (64 * H + 32 * S)) + J * 4096);
     } else {
-      constexpr int kRow = 64 * FX;
-      const int n = i >> 1, jj = i & 1;
+      constexpr int kRow = 64 * kBlocks, N = J / 2, Q = J % 2;
       const i16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          reinterpret_cast<lds_i16x4*>(lds + raddr[n] + (32 * h + 4 * jj) * kRow));
+          reinterpret_cast<lds_i16x4*>(lds + raddr[N] + (32 * H + 16 * S + 4 * Q) * kRow));
       const u32x2 w = __builtin_bit_cast(u32x2, v);
-      f[n][2 * jj] = (int)w[0];
-      f[n][2 * jj + 1] = (int)w[1];
+      f[S][N][2 * Q] = (int)w[0];
+      f[S][N][2 * Q + 1] = (int)w[1];
     }
   }
 };
 
-// Every wave's LDS reads of the finished stage and copies into the next one are done.
-MX_DEV void stage_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
-template <typename T, int FM, int FN, bool ATR, bool BTR, DenseEpi EPI>
-__global__ __launch_bounds__(256) void dense_kernel(DenseArgs p)
+// Every wave's LDS reads so far, and all but its last N copies, are done.
+template <int N>
+MX_DEV void stage_barrier()
 {
-  constexpr int kStage = (FM + FN) * 4096;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStage];
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+template <typename T, int WM, int WN, int FM, int FN, int NS, bool ATR, bool BTR, DenseEpi EPI>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM * WN / 4))) void dense_kernel(DenseArgs p)
+{
+  constexpr int NW = WM * WN;
+  constexpr int kStageA = FM * WM * 4096, kStage = kStageA + FN * WN * 4096;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[NS * kStage];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / WN, wn = wave % WN;
 
-  // Work-groups go to the eight XCDs in turn: each XCD gets one run of neighbouring tiles, walked in
-  // columns of up to 8 tile rows, so that its own L2 holds what its tiles share.
+  // Work-groups go to the eight XCDs in turn: each XCD gets one run of neighbouring tiles of one run of K,
+  // walked in columns of up to 8 tile rows, so that its own L2 holds what its tiles share.
   const int total = gridDim.x, xcd = blockIdx.x & 7;
   int id = xcd * (total >> 3) + min(xcd, total & 7) + (blockIdx.x >> 3);
+  const int tiles = p.tiles_m * p.tiles_n, split = id / tiles;
+  id -= split * tiles;
   const int per_group = 8 * p.tiles_n, group = id / per_group;
   const int rows_here = min(8, p.tiles_m - group * 8);
   id -= group * per_group;
-  const int m0 = (group * 8 + id % rows_here) * 32 * FM;
-  constexpr int kCols = EPI == kDenseGlu ? 16 * FN : 32 * FN;
+  const int m0 = (group * 8 + id % rows_here) * 32 * FM * WM;
+  constexpr int kCols = (EPI == kDenseGlu ? 16 : 32) * FN * WN;
   const int n0 = id / rows_here * kCols;
 
-  Side<FM, ATR, 0> sa;
-  Side<FN, BTR, EPI == kDenseGlu ? 2 : 1> sb;
+  Side<FM, WM, NW, ATR, false> sa;
+  Side<FN, WN, NW, BTR, EPI == kDenseGlu> sb;
   sa.init(p.a, p.lda, m0, p.M, wave, lane, wm);
   sb.init(p.b, p.ldb, n0, p.N, wave, lane, wn);
 
   const int seg_steps = (p.K + kDenseStep - 1) / kDenseStep;
-  const int steps = seg_steps * p.nseg;
-  constexpr int kCopies = FM + FN;
+  const int first = split * p.run, steps = min(seg_steps * p.nseg, first + p.run);
+  constexpr int kCopiesA = decltype(sa)::kCopies, kCopies = kCopiesA + decltype(sb)::kCopies;
   auto copy = [&](int i, int step, int stage) {
     const int seg = step >= seg_steps;
-    const int k0 = (step - (seg ? seg_steps : 0)) * kDenseStep;
+    const int k0 = step < steps ? (step - (seg ? seg_steps : 0)) * kDenseStep : p.K;  // past the last: zeros
     const uint32_t l = lds + stage * kStage;
-    if (i < FM)
+    if (i < kCopiesA)
       sa.copy(i, seg, k0, p.K, l, wave, lane);
     else
-      sb.copy(i - FM, seg, k0, p.K, l + FM * 4096, wave, lane);
+      sb.copy(i - kCopiesA, seg, k0, p.K, l + kStageA, wave, lane);
   };
 
-  f32x4 acc[FM][FN];
+  f32x16 acc[FM][FN];
 #pragma unroll
   for (int m = 0; m < FM; ++m)
 #pragma unroll
-    for (int n = 0; n < FN; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < FN; ++n)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[m][n][j] = 0.f;
 
-  if (steps > 0) {
-    static_for<kCopies>([&](auto i) { copy(i, 0, 0); });
-    if (steps > 1) static_for<kCopies>([&](auto i) { copy(i, 1, 1); });
-  }
-  stage_barrier();
-  for (int step = 0; step < steps; ++step) {
-    const uint32_t l = lds + (step & 1) * kStage;
+  // Fragments of the half being multiplied and of the next one, which are read while the MFMAs of a half
+  // run; after the barrier in the second half of a step nobody reads its stage any more and the next step's copies have
+  // landed, and the MFMAs behind it also carry the copies of step + NS into the stage. The barrier stands
+  // behind the first kWait MFMAs of the second half, which run while the waves wait for each other.
+  i32x4 fa[2][2][FM], fb[2][2][FN];  // [half][slice][block]
+  constexpr int kMfma = 2 * FM * FN, kWait = kMfma / 4;
+  constexpr int kReadsA = decltype(sa)::kReads, kReads = kReadsA + decltype(sb)::kReads;
+  auto read = [&](auto i, auto h, uint32_t l) {
+    if constexpr (i < kReadsA)
+      sa.template read<i, h>(l, fa[h]);
+    else
+      sb.template read<i - kReadsA, h>(l + kStageA, fb[h]);
+  };
+  static_for<NS>([&](auto k) { static_for<kCopies>([&](auto i) { copy(i, first + k, k); }); });
+  stage_barrier<(NS - 1) * kCopies>();
+  static_for<kReads>([&](auto i) { read(i, std::integral_constant<int, 0>{}, lds); });
+  int stage = 0;
+  for (int step = first; step < steps; ++step) {
+    const int next = stage + 1 < NS ? stage + 1 : 0;
+    const uint32_t l0 = lds + stage * kStage, l1 = lds + next * kStage;
     static_for<2>([&](auto h) {
-      i32x4 fa[FM], fb[FN];
-      static_for<Side<FM, ATR, 0>::kReads>([&](auto i) { sa.read(i, h, l, fa); });
-      static_for<decltype(sb)::kReads>([&](auto i) { sb.read(i, h, l + FM * 4096, fb); });
-      static_for<FM * FN>([&](auto x) {
-        constexpr int m = x % FM, n = x / FM;
-        acc[m][n] = Elem<T>::mfma(fb[n], fa[m], acc[m][n]);
+      constexpr int H = h;
+      // LDS reads and copies one by one behind the MFMAs: issued in runs, they left the matrix cores idle
+      static_for<kMfma>([&](auto x) {
+        constexpr int sl = x / (FM * FN), m = x % FM, n = x / FM % FN;
+        acc[m][n] = Elem<T>::mfma(fb[H][sl][n], fa[H][sl][m], acc[m][n]);
+        constexpr int open = H == 0 ? 0 : kWait;  // reads and copies follow the MFMAs from here on
+        if constexpr (H == 1 && x == kWait - 1) stage_barrier<(NS - 2) * kCopies>();
+        static_for<kReads>([&](auto i) {
+          if constexpr (open + i * (kMfma - open) / kReads == x)
+            read(i, std::integral_constant<int, 1 - H>{}, H == 0 ? l0 : l1);
+        });
+        if constexpr (H == 1)
+          static_for<kCopies>([&](auto i) {
+            if constexpr (open + i * (kMfma - open) / kCopies == x) copy(i, step + NS, stage);
+          });
+        __builtin_amdgcn_sched_barrier(0);
       });
     });
-    stage_barrier();
-    if (step + 2 < steps) static_for<kCopies>([&](auto i) { copy(i, step + 2, step & 1); });
+    stage = next;
   }
+  stage_barrier<0>();  // the stages are free for the epilogue
 
-  const int row0 = m0 + wm * 16 * FM + (lane & 15), q = lane >> 4;
+  // The sums go through LDS, each wave its own FMP x FN blocks at a time, so that a lane takes 8
+  // neighbouring columns of a row (whole lines per row, and one short loop whatever the epilogue costs).
+  // fp32 rows of 32 FN columns; 16-byte piece c of row r at place c ^ key: the rows that a write
+  // instruction touches at once fall into different banks.
+  constexpr int kFit = NS * kStage / (FN * 4096 * NW);  // row blocks of a wave that fit
+  constexpr int FMP = kFit >= FM ? FM : kFit >= FM / 2 ? FM / 2 : FM / 4;
+  static_assert(FMP > 0 && FMP * FN * 4096 * NW <= NS * kStage, "a wave's sums do not fit its part of the stages");
+  const uint32_t own = lds + wave * FMP * FN * 4096;
+  auto place = [&](int r, int c) {
+    return own + r * 128 * FN + ((c ^ (FN >= 2 ? r & 15 : (r >> 1) & 7)) << 4);
+  };
+  auto eight = [&](int r, int c, float (&v)[8]) {
+    const f32x4 a = *reinterpret_cast<lds_f32x4*>(place(r, c)), b = *reinterpret_cast<lds_f32x4*>(place(r, c + 1));
 #pragma unroll
-  for (int m = 0; m < FM; ++m) {
-    const int row = row0 + 16 * m;
-    if (row >= p.M) continue;
-    if constexpr (EPI == kDenseGlu) {
-#pragma unroll
-      for (int n = 0; n < FN / 2; n += 2) {
-        const int col = n0 + wn * 8 * FN + 16 * n + 8 * q;
-        if (col >= p.N) continue;
-        float g[8], u[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          g[j] = acc[m][n + j / 4][j % 4];
-          u[j] = acc[m][n + FN / 2 + j / 4][j % 4];
+    for (int j = 0; j < 4; ++j) {
+      v[j] = a[j];
+      v[4 + j] = b[j];
+    }
+  };
+  constexpr int kCol8 = EPI == kDenseGlu ? 2 * FN : 4 * FN;  // groups of 8 result columns per wave
+  const int c8 = lane % kCol8;
+  const int col = n0 + wn * 8 * kCol8 + 8 * c8;
+  static_for<FM / FMP>([&](auto part) {
+    static_for<FMP>([&](auto m) {
+      static_for<FN * 4>([&](auto v) {
+        constexpr int n = v / 4, q = v % 4;
+        const f32x16& a = acc[part * FMP + m][n];
+        *reinterpret_cast<lds_f32x4_w*>(place(32 * m + (lane & 31), 8 * n + 2 * q + (lane >> 5))) =
+            f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+      });
+    });
+    wave_lds_fence();
+    const int row0 = m0 + wm * 32 * FM + part * 32 * FMP;
+#pragma unroll 1
+    for (int r = lane / kCol8; r < 32 * FMP; r += 64 / kCol8) {
+      const int row = row0 + r;
+      if (row >= p.M) break;
+      if (col >= p.N) continue;
+      float v[8];
+      eight(r, 2 * c8, v);
+      if constexpr (EPI == kDenseGlu) {
+        float u[8];
+        eight(r, 4 * FN + 2 * c8, u);
+        if (p.partial) {
+          float* q = p.partial + 2 * ((long long)split * p.M + row) * p.N + col;
+          store_sums(q, v);
+          store_sums(q + p.N, u);
+          continue;
         }
-        epi_glu<T, 8>(p, row, col, g, u);
-      }
-    } else if constexpr (!BTR) {
-#pragma unroll
-      for (int n = 0; n < FN; n += 2) {
-        const int col = n0 + wn * 16 * FN + 16 * n + 8 * q;
-        if (col >= p.N) continue;
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = acc[m][n + j / 4][j % 4];
-        epi_store<T, 8>(p, row, col, v);
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < FN; ++n) {
-        const int col = n0 + wn * 16 * FN + 16 * n + 4 * q;
-        if (col >= p.N) continue;
-        float v[4] = {acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]};
+        epi_glu<T, 8>(p, row, col, v, u);
+      } else if (p.partial) {
+        store_sums(p.partial + ((long long)split * p.M + row) * p.N + col, v);
+      } else {
         if constexpr (EPI == kDenseDGlu)
-          epi_dglu<T, 4>(p, row, col, v);
+          epi_dglu<T, 8>(p, row, col, v);
         else
-          epi_store<T, 4>(p, row, col, v);
+          epi_store<T, 8>(p, row, col, v);
       }
     }
-  }
+    wave_lds_fence();
+  });
 }
 
-template <typename T, int FM, int FN, bool ATR, bool BTR, DenseEpi EPI>
-hipError_t launch_tiles(DenseArgs a, hipStream_t s)
+// The runs' partial sums, added in order, and the epilogue: a thread per 8 columns of a row.
+template <typename T, DenseEpi EPI>
+__global__ __launch_bounds__(256) void dense_finish_kernel(DenseArgs p)
 {
-  const int cols = EPI == kDenseGlu ? 16 * FN : 32 * FN;
-  a.tiles_m = (a.M + 32 * FM - 1) / (32 * FM);
+  const int per_row = p.N / 8;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)p.M * per_row) return;
+  const int row = (int)(i / per_row), col = (int)(i % per_row) * 8;
+  float v[8] = {}, u[8] = {};
+  constexpr int W = EPI == kDenseGlu ? 2 : 1;
+  const long long stride = (long long)p.M * p.N * W;
+  const float* q = p.partial + (long long)row * p.N * W + col;
+  for (int k = 0; k < p.splits; ++k, q += stride) {
+    add_sums(q, v);
+    if constexpr (EPI == kDenseGlu) add_sums(q + p.N, u);
+  }
+  if constexpr (EPI == kDenseGlu)
+    epi_glu<T, 8>(p, row, col, v, u);
+  else if constexpr (EPI == kDenseDGlu)
+    epi_dglu<T, 8>(p, row, col, v);
+  else
+    epi_store<T, 8>(p, row, col, v);
+}
+
+// The tiles there are (kDenseGlu: half the columns are columns of h), one work-group per CU each, and what
+// they were measured to take (us; K = 7168, forward product, normally distributed operands): a step of 64
+// terms while few work-groups run, the same with every CU busy (the chip then lowers its clock; between the
+// two about in proportion), and a tile's start and epilogue.
+struct Tile {
+  int rows, cols;
+  float step, busy, ends;
+};
+constexpr Tile kTiles[] = {{256, 256, 1.13f, 1.80f, 8.f}, {128, 256, 0.66f, 1.02f, 7.f},
+                           {128, 128, 0.45f, 0.57f, 6.f}, {64, 128, 0.28f, 0.40f, 5.f}};
+constexpr int kNTiles = sizeof(kTiles) / sizeof(kTiles[0]);
+constexpr int kCUs = 256;
+constexpr int kMaxSplits = 16;
+
+struct Plan {
+  int tile, splits, run;
+  float us;
+};
+
+// The tile and the number of runs of K that the measurements above promise the shortest time for. Fewer tiles
+// than CUs leave CUs idle, which smaller tiles or more runs mend, each at its price: smaller tiles read their
+// operands more often (a step of four 128 x 128 tiles takes 1.2 x that of one 256 x 256), runs write and
+// read their sums (4 TB/s and a launch). 1000 rows, D = 7168, F = 2048: gate/up 64 us with 128 x 128 tiles
+// in one run, 129 with 256 x 256 in one, 73 in four.
+Plan plan_dense(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg)
+{
+  const float slow = shape == kDenseForward ? 1.f : 1.15f;  // row-major operands: twice the LDS reads
+  const long long cols = epi == kDenseGlu ? 2LL * N : N;
+  const int steps = (K + kDenseStep - 1) / kDenseStep * nseg;
+  const float stream = ((float)cols + M) * K * nseg * 2.f / 4.5e6f;  // the operands once from HBM
+  Plan best = {0, 1, steps, 1e30f};
+  for (int t = 0; t < kNTiles; ++t) {
+    const Tile& tile = kTiles[t];
+    const long long tiles = ((M + tile.rows - 1LL) / tile.rows) * ((cols + tile.cols - 1) / tile.cols);
+    for (int want = 1; want <= kMaxSplits && want <= std::max(steps, 1); ++want) {
+      const int run = (steps + want - 1) / want, splits = run > 0 ? (steps + run - 1) / run : 1;
+      if (splits != want) continue;
+      const long long full = tiles * splits / kCUs, rest = tiles * splits % kCUs;
+      float us = full * (run * tile.busy * slow + tile.ends);
+      if (rest) us += run * (tile.step + (tile.busy - tile.step) * rest / kCUs) * slow + tile.ends;
+      us = std::max(us, stream);
+      if (splits > 1) us += 4.f + (float)M * cols * splits * 1.5e-6f;
+      if (us < best.us) best = {t, splits, run, us};
+      if (tiles * splits >= 4 * kCUs) break;
+    }
+  }
+  return best;
+}
+
+template <typename T, int WM, int WN, int FM, int FN, int NS, DenseShape SH, DenseEpi EPI>
+void launch_tiles(const DenseArgs& a, int splits, hipStream_t s)
+{
+  hipLaunchKernelGGL((dense_kernel<T, WM, WN, FM, FN, NS, SH == kDenseWgrad, SH != kDenseForward, EPI>),
+                     dim3((unsigned)(a.tiles_m * a.tiles_n * splits)), dim3(64 * WM * WN), 0, s, a);
+}
+
+// A product whose last tile row is nearly empty takes its whole tile rows first and the rows behind them by
+// themselves, where the two are expected to be quicker (4099 rows, gate/up: 4096 in one round of 256 x 256
+// tiles and 3 rows, 225 us; two rounds 340).
+struct Cut {
+  int rows;  // of the first part; M: one part
+  Plan first, rest;
+};
+Cut cut_dense(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg)
+{
+  Cut cut = {M, plan_dense(shape, epi, M, N, K, nseg), {}};
+  float best = cut.first.us;
+  if (shape == kDenseWgrad) return cut;  // its rows are features: no odd counts worth a launch
+  for (int rows : {M / 256 * 256, M / 128 * 128}) {
+    if (rows == 0 || rows == M) continue;
+    const Plan a = plan_dense(shape, epi, rows, N, K, nseg), b = plan_dense(shape, epi, M - rows, N, K, nseg);
+    if (a.us + b.us + 3.f < best) {
+      best = a.us + b.us + 3.f;
+      cut = {rows, a, b};
+    }
+  }
+  return cut;
+}
+size_t plan_bytes(const Plan& p, DenseEpi epi, int M, int N)
+{
+  return p.splits > 1 ? sizeof(float) * p.splits * (size_t)M * N * (epi == kDenseGlu ? 2 : 1) : 0;
+}
+
+template <typename T, DenseShape SH, DenseEpi EPI>
+hipError_t launch_plan(const Plan& plan, DenseArgs a, float* partial, hipStream_t s)
+{
+  const Tile& tile = kTiles[plan.tile];
+  const int cols = EPI == kDenseGlu ? tile.cols / 2 : tile.cols;
+  a.tiles_m = (a.M + tile.rows - 1) / tile.rows;
   a.tiles_n = (a.N + cols - 1) / cols;
-  hipLaunchKernelGGL((dense_kernel<T, FM, FN, ATR, BTR, EPI>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(256), 0, s,
-                     a);
+  a.splits = plan.splits;
+  a.run = plan.run;
+  a.partial = plan.splits > 1 ? partial : nullptr;
+  switch (plan.tile) {
+    case 0: launch_tiles<T, 2, 4, 4, 2, 2, SH, EPI>(a, plan.splits, s); break;
+    case 1: launch_tiles<T, 2, 4, 2, 2, 3, SH, EPI>(a, plan.splits, s); break;
+    case 2: launch_tiles<T, 2, 2, 2, 2, 4, SH, EPI>(a, plan.splits, s); break;
+    default: launch_tiles<T, 2, 2, 1, 2, 5, SH, EPI>(a, plan.splits, s); break;
+  }
+  if (plan.splits > 1)
+    hipLaunchKernelGGL((dense_finish_kernel<T, EPI>), dim3((unsigned)(((long long)a.M * (a.N / 8) + 255) / 256)),
+                       dim3(256), 0, s, a);
   return hipGetLastError();
+}
+
+template <typename T, DenseShape SH, DenseEpi EPI>
+hipError_t launch_planned(DenseArgs a, float* partial, hipStream_t s)
+{
+  const Cut cut = cut_dense(SH, EPI, a.M, a.N, a.K, a.nseg);
+  if (cut.rows == a.M) return launch_plan<T, SH, EPI>(cut.first, a, partial, s);
+  const int rest = a.M - cut.rows;
+  a.M = cut.rows;
+  const hipError_t e = launch_plan<T, SH, EPI>(cut.first, a, partial, s);
+  if (e != hipSuccess) return e;
+  const auto down = [&](const void* p, long long ld) {
+    return p ? static_cast<const char*>(p) + 2 * cut.rows * ld : nullptr;
+  };
+  a.M = rest;
+  a.a[0] = down(a.a[0], a.lda);
+  a.a[1] = down(a.a[1], a.lda);
+  a.out = const_cast<char*>(down(a.out, EPI == kDenseStore ? a.ldo : EPI == kDenseGlu ? a.N : 2LL * a.N));
+  a.add0 = down(a.add0, a.N);
+  a.add1 = down(a.add1, a.N);
+  if (a.gu) a.gu += 2LL * cut.rows * a.N;
+  return launch_plan<T, SH, EPI>(cut.rest, a, partial, s);
+}
+
+template <typename T>
+hipError_t launch_typed(DenseShape shape, DenseEpi epi, const DenseArgs& a, float* partial, hipStream_t s)
+{
+  if (shape == kDenseForward)
+    return epi == kDenseGlu ? launch_planned<T, kDenseForward, kDenseGlu>(a, partial, s)
+                            : launch_planned<T, kDenseForward, kDenseStore>(a, partial, s);
+  if (shape == kDenseDgrad)
+    return epi == kDenseDGlu ? launch_planned<T, kDenseDgrad, kDenseDGlu>(a, partial, s)
+                             : launch_planned<T, kDenseDgrad, kDenseStore>(a, partial, s);
+  return launch_planned<T, kDenseWgrad, kDenseStore>(a, partial, s);
 }
 
 }  // namespace
 
-hipError_t launch_dense_forward(const DenseArgs& a, int dtype, DenseEpi epi, hipStream_t s)
+size_t dense_partial_bytes(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg)
 {
-  if (a.M <= 0 || a.N <= 0) return hipSuccess;
-  const bool bf = dtype == MXFP4_BF16;
-  if (epi == kDenseGlu)
-    return bf ? launch_tiles<__bf16, 4, 4, false, false, kDenseGlu>(a, s)
-              : launch_tiles<_Float16, 4, 4, false, false, kDenseGlu>(a, s);
-  return bf ? launch_tiles<__bf16, 4, 4, false, false, kDenseStore>(a, s)
-            : launch_tiles<_Float16, 4, 4, false, false, kDenseStore>(a, s);
+  if (M <= 0 || N <= 0) return 0;
+  const Cut cut = cut_dense(shape, epi, M, N, K, nseg);
+  return std::max(plan_bytes(cut.first, epi, cut.rows, N), plan_bytes(cut.rest, epi, M - cut.rows, N));
 }
 
-hipError_t launch_dense_dgrad(const DenseArgs& a, int dtype, DenseEpi epi, hipStream_t s)
+hipError_t launch_dense(DenseShape shape, DenseEpi epi, const DenseArgs& a, int dtype, float* partial, hipStream_t s)
 {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
-  const bool bf = dtype == MXFP4_BF16;
-  if (epi == kDenseDGlu)
-    return bf ? launch_tiles<__bf16, 4, 4, false, true, kDenseDGlu>(a, s)
-              : launch_tiles<_Float16, 4, 4, false, true, kDenseDGlu>(a, s);
-  return bf ? launch_tiles<__bf16, 4, 4, false, true, kDenseStore>(a, s)
-            : launch_tiles<_Float16, 4, 4, false, true, kDenseStore>(a, s);
-}
-
-hipError_t launch_dense_wgrad(const DenseArgs& a, int dtype, hipStream_t s)
-{
-  if (a.M <= 0 || a.N <= 0) return hipSuccess;
-  return dtype == MXFP4_BF16 ? launch_tiles<__bf16, 4, 4, true, true, kDenseStore>(a, s)
-                             : launch_tiles<_Float16, 4, 4, true, true, kDenseStore>(a, s);
+  return dtype == MXFP4_BF16 ? launch_typed<__bf16>(shape, epi, a, partial, s)
+                             : launch_typed<_Float16>(shape, epi, a, partial, s);
 }
 
 }  // namespace mx

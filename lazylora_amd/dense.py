@@ -17,7 +17,7 @@ from typing import Optional, Tuple, Union
 import torch
 from torch.autograd.function import once_differentiable
 
-from lazylora_amd.native import NORM_LAYER, NORM_RMS, kernel
+from lazylora_amd.native import _ACTS, _FLOATS, NORM_LAYER, NORM_RMS, _aligned, kernel
 
 
 def _native():
@@ -33,6 +33,33 @@ def _records(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _once(impl):
+    """A backward that autograd may run but not differentiate: once_differentiable where a graph of it
+    is asked for (create_graph=True), the plain function, which is quicker, elsewhere."""
+    guarded = once_differentiable(impl)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else impl(ctx, *grads)
+
+    return staticmethod(backward)
+
+
+def _ffn_grads(ctx, grad_y, grad_h=None):
+    x, w_gate, w_up, w_down, h, gu = ctx.saved_tensors
+    if grad_y is None and grad_h is None:
+        return (None,) * 8
+    need = ctx.needs_input_grad
+    if grad_y is None:  # only h was used
+        grad_y = grad_h.new_zeros((grad_h.shape[0], w_down.shape[0]))
+    tidy = lambda t: None if t is None else _aligned(t.contiguous())
+    dgu, dx, dwg, dwu, dwd = _native()._ffn_backward(
+        tidy(grad_y), gu, (tidy(w_gate), tidy(w_up), tidy(w_down)), _FLOATS[w_gate.dtype], _ACTS[ctx.act], tidy(grad_h),
+        tidy(x), tidy(h), need[0])
+    F = w_gate.shape[0]
+    return (dx, dwg if need[1] else None, dwu if need[2] else None, dwd, dgu[:, :F] if need[4] else None,
+            dgu[:, F:] if need[5] else None, None, None)
+
+
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, gate_delta, up_delta, act, return_hidden):
@@ -44,21 +71,7 @@ class _GatedFfn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return (y, h) if return_hidden else y
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y, grad_h=None):
-        x, w_gate, w_up, w_down, h, gu = ctx.saved_tensors
-        if grad_y is None and grad_h is None:
-            return (None,) * 8
-        need = ctx.needs_input_grad
-        if grad_y is None:  # only h was used
-            grad_y = grad_h.new_zeros((grad_h.shape[0], w_down.shape[0]))
-        dgu, dx, dwg, dwu, dwd = _native().ffn_backward(
-            grad_y, gu, w_gate, w_up, w_down, ctx.act, grad_h, x, h, need_x=need[0], need_w_in=need[1] or need[2],
-            need_w_down=need[3])
-        F = w_gate.shape[0]
-        return (dx, dwg if need[1] else None, dwu if need[2] else None, dwd, dgu[:, :F] if need[4] else None,
-                dgu[:, F:] if need[5] else None, None, None)
+    backward = _once(_ffn_grads)
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, act: str = "swiglu",
@@ -87,24 +100,24 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     return (y, h.reshape(lead + h.shape[-1:])) if return_hidden else y
 
 
+def _norm_grads(ctx, grad_y):
+    x, weight, stats = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    w = weight if weight is None else weight.float().contiguous()
+    dx, dw, db = _native()._norm_backward(grad_y, x.contiguous(), w, stats, ctx.kind, need[1], need[2])
+    return (dx, dw if dw is None else dw.to(weight.dtype), db if db is None else db.to(ctx.bias_dtype), None, None)
+
+
 class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, kind):
-        w, b = (None if t is None else t.float() for t in (weight, bias))
-        y, stats = _native().norm_forward(x, w, b, eps, kind, save_for_backward=True)
+        y, stats = _native().norm_forward(x, weight if weight is None else weight.float(),
+                                          bias if bias is None else bias.float(), eps, kind, True)
         ctx.save_for_backward(x, weight, stats)
         ctx.kind, ctx.bias_dtype = kind, None if bias is None else bias.dtype
         return y
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y):
-        x, weight, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = _native().norm_backward(grad_y, x, None if weight is None else weight.float(), stats, ctx.kind,
-                                             need_weight=need[1], need_bias=need[2])
-        return (dx if need[0] else None, dw.to(weight.dtype) if need[1] else None,
-                db.to(ctx.bias_dtype) if need[2] else None, None, None)
+    backward = _once(_norm_grads)
 
 
 def _norm(x, weight, bias, eps, kind):
@@ -133,20 +146,21 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
     return _norm(x, weight, None, eps, NORM_RMS)
 
 
+def _dropout_grad(ctx, grad_y):
+    seed = ctx.seed if ctx.seed is not None else ctx.saved_tensors[0]
+    return _native()._dropout(grad_y, ctx.p, seed, ctx.stream), None, None, None
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, stream):
-        ctx.on_dev = torch.is_tensor(seed)
-        if ctx.on_dev:  # saved, so that autograd notices a seed changed before the backward
+        ctx.p, ctx.seed, ctx.stream = p, seed, stream
+        if torch.is_tensor(seed):  # saved, so that autograd notices a seed changed before the backward
             ctx.save_for_backward(seed)
-        ctx.p, ctx.seed, ctx.stream = p, None if ctx.on_dev else seed, stream
+            ctx.seed = None
         return _native().dropout(x, p, seed, stream)
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y):
-        seed = ctx.saved_tensors[0] if ctx.on_dev else ctx.seed
-        return _native().dropout(grad_y, ctx.p, seed, ctx.stream), None, None, None
+    backward = _once(_dropout_grad)
 
 
 def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], stream: int = 0) -> torch.Tensor:

@@ -19,7 +19,6 @@ Differences from the reference, all deliberate:
     Nothing here falls back to a CPU implementation: the MXFP4Kernel methods run on the GPU
     or raise.
 """
-import contextlib
 import ctypes
 import os
 import sys
@@ -405,7 +404,9 @@ class MXFP4Kernel:
             raise ValueError(f"top_k must lie in [1, min(E, 64)] = [1, {min(E, 64)}], got {top_k}")
 
     # -- dense operators ---------------------------------------------------------------------
-    # Device tensors only (ValueError otherwise); lazylora_amd.dense wraps these in autograd.
+    # Device tensors only (ValueError otherwise); lazylora_amd.dense wraps these in autograd. Small calls
+    # are bound by host work, so each public method checks its arguments and an inner one, which the
+    # backward passes call with what their forward checked, launches.
     def ffn_forward(self, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
                     act="swiglu", gate_delta: Optional[torch.Tensor] = None,
                     up_delta: Optional[torch.Tensor] = None, save_for_backward: bool = False):
@@ -413,16 +414,22 @@ class MXFP4Kernel:
         float16: gate = x Wg^T (+ gate_delta), up = x Wu^T (+ up_delta), h = GLU(gate, up),
         y = h Wd^T with w_gate, w_up [F, D] and w_down [Do, F] (mxfp4_ffn_forward). gu is the fp32
         gate | up [M, 2F] that ffn_backward takes, or None without save_for_backward."""
-        c = _FfnCall(x, w_gate, w_up, w_down, act)
-        gd, ud = c.like_h(gate_delta, "gate_delta"), c.like_h(up_delta, "up_delta")
-        y, h = c.new(c.M, c.Do), c.new(c.M, c.F)
-        gu = torch.empty((c.M, 2 * c.F), dtype=torch.float32, device=c.dev) if save_for_backward else None
-        if c.M:
-            ws, nws = c.workspace(self.lib)
-            with _on(c.dev):
-                _check(self.lib.mxfp4_ffn_forward(y.data_ptr(), h.data_ptr(), _ptr(gu), c.x.data_ptr(),
-                                                  *[w.data_ptr() for w in c.w], _ptr(gd), _ptr(ud), c.dtype, c.M, c.D,
-                                                  c.F, c.Do, c.act, _ptr(ws), nws, _stream(c.dev)), self.lib)
+        dt, dev = x.dtype, x.device
+        code, kind, (D, F, Do) = _ffn_sizes(dt, dev, w_gate, w_down, act)
+        M = x.shape[0] if x.dim() == 2 else -1
+        x = _arg(x, "x", (M, D), dt, dev)
+        w_gate, w_up = _arg(w_gate, "w_gate", (F, D), dt, dev), _arg(w_up, "w_up", (F, D), dt, dev)
+        w_down = _arg(w_down, "w_down", (Do, F), dt, dev)
+        gd = gate_delta if gate_delta is None else _arg(gate_delta, "gate_delta", (M, F), dt, dev)
+        ud = up_delta if up_delta is None else _arg(up_delta, "up_delta", (M, F), dt, dev)
+        y = torch.empty((M, Do), dtype=dt, device=dev)
+        h = torch.empty((M, F), dtype=dt, device=dev)
+        gu = torch.empty((M, 2 * F), dtype=torch.float32, device=dev) if save_for_backward else None
+        if M:
+            ws, nws = self._ffn_workspace(M, D, F, Do, dev)
+            self._launch(dev, self.lib.mxfp4_ffn_forward, y.data_ptr(), h.data_ptr(), _ptr(gu), x.data_ptr(),
+                         w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), _ptr(gd), _ptr(ud), code, M, D, F, Do,
+                         kind, _ptr(ws), nws)
         return y, h, gu
 
     def ffn_backward(self, grad_y: torch.Tensor, gu: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
@@ -437,23 +444,38 @@ class MXFP4Kernel:
             raise ValueError("need_w_in=True takes the forward's x")
         if need_w_down and h is None:
             raise ValueError("need_w_down=True takes the forward's h")
-        c = _FfnCall(x, w_gate, w_up, w_down, act, rows=grad_y)
-        gy = c.take(grad_y, "grad_y", (c.M, c.Do))
-        gh, h = c.like_h(grad_h, "grad_h"), c.like_h(h, "h")
-        if gu.dtype != torch.float32 or tuple(gu.shape) != (c.M, 2 * c.F) or gu.device != c.dev:
-            raise ValueError(f"gu must be the forward's float32 [{c.M}, {2 * c.F}]")
-        gu = _aligned(gu.contiguous())
-        dgu = c.new(c.M, 2 * c.F)
-        dx = c.new(c.M, c.D) if need_x else None
-        dwg, dwu = (c.new(c.F, c.D), c.new(c.F, c.D)) if need_w_in else (None, None)
-        dwd = c.new(c.Do, c.F) if need_w_down else None
-        ws, nws = c.workspace(self.lib)
-        with _on(c.dev):
-            _check(self.lib.mxfp4_ffn_backward(_ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd), dgu.data_ptr(),
-                                               gy.data_ptr(), _ptr(gh), _ptr(c.x), _ptr(h), gu.data_ptr(),
-                                               *[w.data_ptr() for w in c.w], c.dtype, c.M, c.D, c.F, c.Do, c.act,
-                                               _ptr(ws), nws, _stream(c.dev)), self.lib)
+        dt, dev = grad_y.dtype, grad_y.device
+        code, kind, (D, F, Do) = _ffn_sizes(dt, dev, w_gate, w_down, act)
+        M = grad_y.shape[0] if grad_y.dim() == 2 else -1
+        grad_y = _arg(grad_y, "grad_y", (M, Do), dt, dev)
+        w = (_arg(w_gate, "w_gate", (F, D), dt, dev), _arg(w_up, "w_up", (F, D), dt, dev),
+             _arg(w_down, "w_down", (Do, F), dt, dev))
+        gu = _arg(gu, "gu", (M, 2 * F), torch.float32, dev)
+        grad_h = grad_h if grad_h is None else _arg(grad_h, "grad_h", (M, F), dt, dev)
+        x = _arg(x, "x", (M, D), dt, dev) if need_w_in else None
+        h = _arg(h, "h", (M, F), dt, dev) if need_w_down else None
+        return self._ffn_backward(grad_y, gu, w, code, kind, grad_h, x, h, need_x)
+
+    def _ffn_backward(self, grad_y, gu, w, code, kind, grad_h, x, h, need_x):
+        dt, dev = grad_y.dtype, grad_y.device
+        M, Do = grad_y.shape
+        F, D = w[0].shape
+        dgu = torch.empty((M, 2 * F), dtype=dt, device=dev)
+        dx = torch.empty((M, D), dtype=dt, device=dev) if need_x else None
+        dwg = dwu = dwd = None
+        if x is not None:
+            dwg, dwu = torch.empty((F, D), dtype=dt, device=dev), torch.empty((F, D), dtype=dt, device=dev)
+        if h is not None:
+            dwd = torch.empty((Do, F), dtype=dt, device=dev)
+        ws, nws = self._ffn_workspace(M, D, F, Do, dev)
+        self._launch(dev, self.lib.mxfp4_ffn_backward, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd), dgu.data_ptr(),
+                     grad_y.data_ptr(), _ptr(grad_h), _ptr(x), _ptr(h), gu.data_ptr(), w[0].data_ptr(),
+                     w[1].data_ptr(), w[2].data_ptr(), code, M, D, F, Do, kind, _ptr(ws), nws)
         return dgu, dx, dwg, dwu, dwd
+
+    def _ffn_workspace(self, M, D, F, Do, dev):
+        n = self.lib.mxfp4_ffn_workspace_size(M, D, F, Do)
+        return (torch.empty(n, dtype=torch.uint8, device=dev) if n else None), n
 
     def norm_forward(self, x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                      bias: Optional[torch.Tensor] = None, eps: float = 1e-5, kind: int = NORM_RMS,
@@ -461,15 +483,21 @@ class MXFP4Kernel:
         """(y, stats) of the RMS or layer norm of x [M, D] (float32, bfloat16 or float16) over its last
         axis, weight and bias [D] float32 or None (mxfp4_norm_forward); stats [2, M] float32 is what
         norm_backward takes, or None without save_for_backward."""
-        M, D, dt = _rows(x)
-        w, b = _vector(weight, D, x.device, "weight"), _vector(bias, D, x.device, "bias")
-        xc = x.contiguous()
-        y = torch.empty_like(xc)
-        stats = torch.empty((2, M), dtype=torch.float32, device=x.device) if save_for_backward else None
+        dev, code = x.device, _FLOATS.get(x.dtype)
+        if x.dim() != 2 or x.shape[1] == 0 or dev.type != "cuda" or code is None:
+            raise ValueError("x must be a float32, bfloat16 or float16 tensor [M, D], D > 0, on the HIP device, got "
+                             f"{x.dtype} {tuple(x.shape)} on {dev}")
+        M, D = x.shape
+        if weight is not None:
+            weight = _arg(weight, "weight", (D,), torch.float32, dev)
+        if bias is not None:
+            bias = _arg(bias, "bias", (D,), torch.float32, dev)
+        x = x.contiguous()
+        y = torch.empty_like(x)
+        stats = torch.empty((2, M), dtype=torch.float32, device=dev) if save_for_backward else None
         if M:
-            with _on(x.device):
-                _check(self.lib.mxfp4_norm_forward(y.data_ptr(), _ptr(stats), xc.data_ptr(), _ptr(w), _ptr(b), M, D,
-                                                   float(eps), kind, dt, _stream(x.device)), self.lib)
+            self._launch(dev, self.lib.mxfp4_norm_forward, y.data_ptr(), _ptr(stats), x.data_ptr(), _ptr(weight),
+                         _ptr(bias), M, D, eps, kind, code)
         return y, stats
 
     def norm_backward(self, grad_y: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor],
@@ -477,22 +505,28 @@ class MXFP4Kernel:
                       need_bias: bool = False):
         """(dx, dweight, dbias) for dL/dy (mxfp4_norm_backward); the column gradients are float32, None
         unless asked for."""
-        M, D, dt = _rows(x)
-        if grad_y.shape != x.shape or grad_y.dtype != x.dtype or grad_y.device != x.device:
-            raise ValueError(f"grad_y must be {x.dtype} {tuple(x.shape)} on x's device")
-        if stats.dtype != torch.float32 or tuple(stats.shape) != (2, M) or stats.device != x.device:
-            raise ValueError(f"stats must be the forward's float32 [2, {M}]")
-        w = _vector(weight, D, x.device, "weight")
-        xc, gy, stats = x.contiguous(), grad_y.contiguous(), stats.contiguous()
-        dx = torch.empty_like(xc)
-        dw = torch.empty(D, dtype=torch.float32, device=x.device) if need_weight else None
-        db = torch.empty(D, dtype=torch.float32, device=x.device) if need_bias else None
-        nws = int(self.lib.mxfp4_norm_workspace_size(M, D)) if need_weight or need_bias else 0
-        ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
-        with _on(x.device):
-            _check(self.lib.mxfp4_norm_backward(dx.data_ptr(), _ptr(dw), _ptr(db), gy.data_ptr(), xc.data_ptr(),
-                                                _ptr(w), stats.data_ptr(), M, D, kind, dt, _ptr(ws), nws,
-                                                _stream(x.device)), self.lib)
+        dt, dev = x.dtype, x.device
+        if x.dim() != 2 or x.shape[1] == 0 or dev.type != "cuda" or dt not in _FLOATS:
+            raise ValueError("x must be the forward's")
+        M, D = x.shape
+        if grad_y.shape != x.shape or grad_y.dtype != dt or grad_y.device != dev:
+            raise ValueError(f"grad_y must be {dt} {tuple(x.shape)} on x's device")
+        stats = _arg(stats, "stats", (2, M), torch.float32, dev)
+        if weight is not None:
+            weight = _arg(weight, "weight", (D,), torch.float32, dev)
+        return self._norm_backward(grad_y, x.contiguous(), weight, stats, kind, need_weight, need_bias)
+
+    def _norm_backward(self, grad_y, x, weight, stats, kind, need_weight, need_bias):
+        dev = x.device
+        M, D = x.shape
+        grad_y = grad_y.contiguous()
+        dx = torch.empty_like(x)
+        dw = torch.empty(D, dtype=torch.float32, device=dev) if need_weight else None
+        db = torch.empty(D, dtype=torch.float32, device=dev) if need_bias else None
+        nws = self.lib.mxfp4_norm_workspace_size(M, D) if need_weight or need_bias else 0
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+        self._launch(dev, self.lib.mxfp4_norm_backward, dx.data_ptr(), _ptr(dw), _ptr(db), grad_y.data_ptr(),
+                     x.data_ptr(), _ptr(weight), stats.data_ptr(), M, D, kind, _FLOATS[x.dtype], _ptr(ws), nws)
         return dx, dw, db
 
     def dropout(self, x: torch.Tensor, p: float, seed, stream: int = 0) -> torch.Tensor:
@@ -500,26 +534,37 @@ class MXFP4Kernel:
         number in row-major order) and is stored nowhere (mxfp4_dropout). seed: a whole number in
         [0, 2^64), or a one-element int64 tensor on x's device, read by the kernel (for captured graphs).
         stream: a second number in [0, 2^64) that tells calls under one seed apart."""
-        if not x.is_cuda or x.dtype not in _FLOATS:
+        if x.device.type != "cuda" or x.dtype not in _FLOATS:
             raise ValueError("x must be a float32, bfloat16 or float16 tensor on the HIP device")
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"p must lie in [0, 1], got {p}")
         if not 0 <= stream < 2 ** 64:
             raise ValueError(f"stream must lie in [0, 2^64), got {stream}")
-        on_dev = torch.is_tensor(seed)
-        if on_dev:
+        if torch.is_tensor(seed):
             if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device:
                 raise ValueError("a seed tensor must hold one int64 on x's device")
         elif not 0 <= seed < 2 ** 64:
             raise ValueError(f"seed must lie in [0, 2^64), got {seed}")
-        xc = x.contiguous()
-        y = torch.empty_like(xc)
-        if xc.numel():
-            with _on(x.device):
-                _check(self.lib.mxfp4_dropout(y.data_ptr(), xc.data_ptr(), xc.numel(), float(p),
-                                              0 if on_dev else int(seed), seed.data_ptr() if on_dev else None,
-                                              int(stream), _FLOATS[x.dtype], _stream(x.device)), self.lib)
+        return self._dropout(x, p, seed, stream)
+
+    def _dropout(self, x, p, seed, stream):
+        x = x.contiguous()
+        y = torch.empty_like(x)
+        number, where = (0, seed.data_ptr()) if isinstance(seed, torch.Tensor) else (seed, None)
+        self._launch(x.device, self.lib.mxfp4_dropout, y.data_ptr(), x.data_ptr(), x.numel(), p, number, where, stream,
+                     _FLOATS[x.dtype])
         return y
+
+    def _launch(self, dev, fn, *args):
+        """fn(*args, stream) on dev's current stream, with dev as the current device."""
+        stream = torch._C._cuda_getCurrentRawStream(dev.index)
+        if dev.index == torch.cuda.current_device():
+            rc = fn(*args, stream)
+        else:
+            with torch.cuda.device(dev):
+                rc = fn(*args, stream)
+        if rc:
+            _check(rc, self.lib)
 
     def moe_workspace_bytes(self, N: int, k: int, E: int, D: int, F: int) -> int:
         return int(self.lib.mxfp4_moe_workspace_size(N, k, E, D, F))
@@ -563,72 +608,28 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _on(dev: torch.device):
-    """Makes dev the current device for a launch on one of its streams."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _arg(t: torch.Tensor, name: str, shape, dt: torch.dtype, dev: torch.device) -> torch.Tensor:
+    """t, contiguous and 16-byte aligned (a copy where it is not), of this shape and type on dev."""
+    if t.shape != shape or t.dtype != dt or t.device != dev:
+        raise ValueError(f"{name} must be {dt} {list(shape)} on {dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+    return _aligned(t.contiguous())
 
 
-def _rows(x: torch.Tensor):
-    """(M, D, dtype code) of a norm's x."""
-    if x.dim() != 2 or x.shape[1] == 0 or not x.is_cuda or x.dtype not in _FLOATS:
-        raise ValueError("x must be a float32, bfloat16 or float16 tensor [M, D], D > 0, on the HIP device, got "
-                         f"{x.dtype} {tuple(x.shape)} on {x.device}")
-    return x.shape[0], x.shape[1], _FLOATS[x.dtype]
-
-
-def _vector(t: Optional[torch.Tensor], D: int, dev: torch.device, name: str):
-    if t is None:
-        return None
-    if tuple(t.shape) != (D,) or t.dtype != torch.float32 or t.device != dev:
-        raise ValueError(f"{name} must be float32 [{D}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.contiguous()
-
-
-class _FfnCall:
-    """Validated arguments of one call of the gated feed-forward block. Without x (a backward that needs
-    no weight gradients) the row count is that of `rows`."""
-
-    def __init__(self, x, w_gate, w_up, w_down, act, rows=None):
-        if act not in _ACTS:
-            raise ValueError(f"unknown activation {act!r}")
-        self.act = _ACTS[act]
-        first = x if x is not None else rows
-        self.torch_dtype, self.dev = first.dtype, first.device
-        if self.torch_dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError(f"the feed-forward block takes bfloat16 or float16, got {self.torch_dtype}")
-        if self.dev.type != "cuda":
-            raise ValueError(f"the feed-forward block takes tensors on the HIP device, got {self.dev}")
-        if first.dim() != 2 or w_gate.dim() != 2 or w_down.dim() != 2:
-            raise ValueError("x and the weights must be 2-D")
-        self.M = first.shape[0]
-        self.F, self.D = w_gate.shape
-        self.Do = w_down.shape[0]
-        for name, n in (("D", self.D), ("F", self.F), ("Do", self.Do)):
-            if n == 0 or n % 8:
-                raise ValueError(f"{name} = {n} must be a positive multiple of 8")
-        self.x = None if x is None else self.take(x, "x", (self.M, self.D))
-        self.w = (self.take(w_gate, "w_gate", (self.F, self.D)), self.take(w_up, "w_up", (self.F, self.D)),
-                  self.take(w_down, "w_down", (self.Do, self.F)))
-
-    def take(self, t, name, shape):
-        if tuple(t.shape) != shape or t.dtype != self.torch_dtype or t.device != self.dev:
-            raise ValueError(f"{name} must be {self.torch_dtype} {list(shape)} on {self.dev}, got {t.dtype} "
-                             f"{list(t.shape)} on {t.device}")
-        return _aligned(t.contiguous())
-
-    def like_h(self, t, name):
-        return None if t is None else self.take(t, name, (self.M, self.F))
-
-    def new(self, *shape):
-        return torch.empty(shape, dtype=self.torch_dtype, device=self.dev)
-
-    @property
-    def dtype(self):
-        return _FLOATS[self.torch_dtype]
-
-    def workspace(self, lib):
-        n = int(lib.mxfp4_ffn_workspace_size(self.M, self.D, self.F, self.Do))
-        return (torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None), n
+def _ffn_sizes(dt, dev, w_gate, w_down, act):
+    """(dtype code, activation code, (D, F, Do)) of a call of the gated feed-forward block."""
+    if dt != torch.bfloat16 and dt != torch.float16:
+        raise ValueError(f"the feed-forward block takes bfloat16 or float16, got {dt}")
+    if dev.type != "cuda":
+        raise ValueError(f"the feed-forward block takes tensors on the HIP device, got {dev}")
+    if act not in _ACTS:
+        raise ValueError(f"unknown activation {act!r}")
+    if w_gate.dim() != 2 or w_down.dim() != 2:
+        raise ValueError("the weights must be 2-D")
+    F, D = w_gate.shape
+    Do = w_down.shape[0]
+    if D % 8 or F % 8 or Do % 8 or not (D and F and Do):
+        raise ValueError(f"D = {D}, F = {F} and Do = {Do} must be positive multiples of 8")
+    return _FLOATS[dt], _ACTS[act], (D, F, Do)
 
 
 class _RoutedCall:
