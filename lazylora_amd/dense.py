@@ -33,6 +33,9 @@ def _records(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+# The backward functions run in autograd's own thread, where host work costs several times what it does in
+# the caller's (a step of a small norm: 123 us with the checks and conversions of a public call in its
+# backward, 91 without), so they take what their forward has checked and call the inner entry points.
 def _once(impl):
     """A backward that autograd may run but not differentiate: once_differentiable where a graph of it
     is asked for (create_graph=True), the plain function, which is quicker, elsewhere."""
@@ -44,6 +47,10 @@ def _once(impl):
     return staticmethod(backward)
 
 
+def _tidy(t):
+    return t if t is None else _aligned(t.contiguous())
+
+
 def _ffn_grads(ctx, grad_y, grad_h=None):
     x, w_gate, w_up, w_down, h, gu = ctx.saved_tensors
     if grad_y is None and grad_h is None:
@@ -51,10 +58,9 @@ def _ffn_grads(ctx, grad_y, grad_h=None):
     need = ctx.needs_input_grad
     if grad_y is None:  # only h was used
         grad_y = grad_h.new_zeros((grad_h.shape[0], w_down.shape[0]))
-    tidy = lambda t: None if t is None else _aligned(t.contiguous())
-    dgu, dx, dwg, dwu, dwd = _native()._ffn_backward(
-        tidy(grad_y), gu, (tidy(w_gate), tidy(w_up), tidy(w_down)), _FLOATS[w_gate.dtype], _ACTS[ctx.act], tidy(grad_h),
-        tidy(x), tidy(h), need[0])
+    dgu, dx, dwg, dwu, dwd = ctx.k._ffn_backward(
+        _tidy(grad_y), gu, (_tidy(w_gate), _tidy(w_up), _tidy(w_down)), _FLOATS[w_gate.dtype], _ACTS[ctx.act],
+        _tidy(grad_h), _tidy(x), _tidy(h), need[0])
     F = w_gate.shape[0]
     return (dx, dwg if need[1] else None, dwu if need[2] else None, dwd, dgu[:, :F] if need[4] else None,
             dgu[:, F:] if need[5] else None, None, None)
@@ -63,7 +69,8 @@ def _ffn_grads(ctx, grad_y, grad_h=None):
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, gate_delta, up_delta, act, return_hidden):
-        y, h, gu = _native().ffn_forward(x, w_gate, w_up, w_down, act, gate_delta, up_delta, save_for_backward=True)
+        ctx.k = _native()
+        y, h, gu = ctx.k.ffn_forward(x, w_gate, w_up, w_down, act, gate_delta, up_delta, save_for_backward=True)
         need = ctx.needs_input_grad
         # what the products of the wanted gradients read: x for the gate and up weights, h for the down weight
         ctx.save_for_backward(x if need[1] or need[2] else None, w_gate, w_up, w_down, h if need[3] else None, gu)
@@ -87,7 +94,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     (8 bytes per row and hidden feature): rounded to 16 bits they would add the same error again that
     the rounding of their gradients has."""
     lead = x.shape[:-1]
-    flat = lambda t: None if t is None else t.reshape(-1, t.shape[-1])
+    flat = lambda t: t if t is None or t.dim() == 2 else t.reshape(-1, t.shape[-1])
     if x.dim() == 0 or any(t is not None and t.shape[:-1] != lead for t in (gate_delta, up_delta)):
         raise ValueError("x and the deltas must agree in all axes but the last")
     x, gate_delta, up_delta = flat(x), flat(gate_delta), flat(up_delta)
@@ -96,25 +103,37 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
         y, h = out if return_hidden else (out, None)
     else:
         y, h, _ = _native().ffn_forward(x, w_gate, w_up, w_down, act, gate_delta, up_delta)
-    y = y.reshape(lead + y.shape[-1:])
-    return (y, h.reshape(lead + h.shape[-1:])) if return_hidden else y
+    if len(lead) != 1:
+        y = y.reshape(lead + y.shape[-1:])
+        h = h if h is None else h.reshape(lead + h.shape[-1:])
+    return (y, h) if return_hidden else y
 
 
 def _norm_grads(ctx, grad_y):
     x, weight, stats = ctx.saved_tensors
-    need = ctx.needs_input_grad
-    w = weight if weight is None else weight.float().contiguous()
-    dx, dw, db = _native()._norm_backward(grad_y, x.contiguous(), w, stats, ctx.kind, need[1], need[2])
-    return (dx, dw if dw is None else dw.to(weight.dtype), db if db is None else db.to(ctx.bias_dtype), None, None)
+    _, need_w, need_b, _, _ = ctx.needs_input_grad
+    dx, dw, db = ctx.k._norm_backward(grad_y, x, weight, stats, ctx.kind, need_w, need_b)
+    if need_w and ctx.weight_dtype != torch.float32:
+        dw = dw.to(ctx.weight_dtype)
+    if need_b and ctx.bias_dtype != torch.float32:
+        db = db.to(ctx.bias_dtype)
+    return dx, dw, db, None, None
 
 
 class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, kind):
-        y, stats = _native().norm_forward(x, weight if weight is None else weight.float(),
-                                          bias if bias is None else bias.float(), eps, kind, True)
+        ctx.k = _native()
+        if weight is not None:
+            ctx.weight_dtype = weight.dtype
+            weight = weight.float().contiguous()
+        if bias is not None:
+            ctx.bias_dtype = bias.dtype
+            bias = bias.float()
+        x = x.contiguous()
+        y, stats = ctx.k.norm_forward(x, weight, bias, eps, kind, True)
         ctx.save_for_backward(x, weight, stats)
-        ctx.kind, ctx.bias_dtype = kind, None if bias is None else bias.dtype
+        ctx.kind = kind
         return y
 
     backward = _once(_norm_grads)
@@ -123,13 +142,13 @@ class _Norm(torch.autograd.Function):
 def _norm(x, weight, bias, eps, kind):
     if x.dim() == 0:
         raise ValueError("x must have at least one axis")
-    x2 = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(0, 0)
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(0, 0)
     if _records(x2, weight, bias):
         y = _Norm.apply(x2, weight, bias, eps, kind)
     else:
         w, b = (None if t is None else t.float() for t in (weight, bias))
         y, _ = _native().norm_forward(x2, w, b, eps, kind)
-    return y.reshape(x.shape)
+    return y if x.dim() == 2 else y.reshape(x.shape)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -148,17 +167,17 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
 
 def _dropout_grad(ctx, grad_y):
     seed = ctx.seed if ctx.seed is not None else ctx.saved_tensors[0]
-    return _native()._dropout(grad_y, ctx.p, seed, ctx.stream), None, None, None
+    return ctx.k._dropout(grad_y, ctx.p, seed, ctx.stream), None, None, None
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, stream):
-        ctx.p, ctx.seed, ctx.stream = p, seed, stream
+        ctx.k, ctx.p, ctx.seed, ctx.stream = _native(), p, seed, stream
         if torch.is_tensor(seed):  # saved, so that autograd notices a seed changed before the backward
             ctx.save_for_backward(seed)
             ctx.seed = None
-        return _native().dropout(x, p, seed, stream)
+        return ctx.k.dropout(x, p, seed, stream)
 
     backward = _once(_dropout_grad)
 

@@ -517,9 +517,10 @@ class MXFP4Kernel:
         return self._norm_backward(grad_y, x.contiguous(), weight, stats, kind, need_weight, need_bias)
 
     def _norm_backward(self, grad_y, x, weight, stats, kind, need_weight, need_bias):
-        dev = x.device
         M, D = x.shape
-        grad_y = grad_y.contiguous()
+        dev = x.device
+        if not grad_y.is_contiguous():
+            grad_y = grad_y.contiguous()
         dx = torch.empty_like(x)
         dw = torch.empty(D, dtype=torch.float32, device=dev) if need_weight else None
         db = torch.empty(D, dtype=torch.float32, device=dev) if need_bias else None
