@@ -8,6 +8,10 @@
 #include "mx_dense.h"
 #include "mx_device.h"
 
+// Every fused multiply-add here is written out: left to the compiler, two forms of a kernel could round
+// differently, and a gradient would depend on which others were asked for.
+#pragma clang fp contract(off)
+
 namespace mx {
 
 namespace {
@@ -17,7 +21,8 @@ namespace {
 // alignment only (the memory pipeline takes them; whole rows stay contiguous).
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) Eight {
-  T v[8];
+  typedef T Vec __attribute__((ext_vector_type(8)));
+  Vec v;  // a vector: an array of 16-bit elements would take a register each
 };
 template <typename T>
 MX_DEV void load8(const T* p, int i, int n, float (&f)[8])
@@ -30,6 +35,18 @@ MX_DEV void load8(const T* p, int i, int n, float (&f)[8])
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = i + j < n ? (float)p[i + j] : 0.f;
   }
+}
+template <typename T>
+MX_DEV Eight<T> load_raw(const T* p, int i, int n)
+{
+  Eight<T> e;
+  if (i + 8 <= n) {
+    e = *reinterpret_cast<const Eight<T>*>(p + i);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e.v[j] = i + j < n ? p[i + j] : (T)0.f;
+  }
+  return e;
 }
 template <typename T>
 MX_DEV void store8(T* p, int i, int n, const float (&f)[8])
@@ -117,7 +134,7 @@ __global__ __launch_bounds__(NT) void norm_fwd_kernel(T* __restrict__ y, float* 
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float d = v[c][j] - mean;
-      if (8 * (lane + G * c) + j < n) q[0] += d * d;
+      if (8 * (lane + G * c) + j < n) q[0] = fmaf(d, d, q[0]);
     }
   team_sum<G, 1>(q, buf[1]);
   const float r = 1.0f / sqrtf(q[0] / (float)D + eps);
@@ -170,7 +187,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(T* __restrict__ y, 
     load8(xr, i, D, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (i + j < D) q[0] += (v[j] - mean) * (v[j] - mean);
+      if (i + j < D) q[0] = fmaf(v[j] - mean, v[j] - mean, q[0]);
   }
   team_sum<1024, 1>(q, buf[1]);
   const float r = 1.0f / sqrtf(q[0] / (float)D + eps);
@@ -196,9 +213,11 @@ __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(T* __restrict__ y, 
 // dx and, per work-group, the partial sums of dweight and dbias over the rows it takes:
 //   dx = r (t - mean t [layer] - xh mean(t xh)),  t = dy w,  xh = (x - mean) r.
 // A lane keeps the same columns for every row, so the column sums stay in registers to the end; the teams
-// then meet in LDS. partial: [gridDim.x][2][D] (dweight, dbias), added in order by norm_finish_kernel.
-template <typename T, int NT, int G, int V>
-__global__ __launch_bounds__(NT) void norm_bwd_kernel(T* __restrict__ dx, float* __restrict__ partial,
+// then meet in LDS. The next row's bytes are requested before this row's sums meet; rows are kept as they
+// were loaded and widened twice, which costs fewer registers than the widened values. FULL: layer norm, or
+// dbias wanted. partial: [gridDim.x][2][D] (dweight, dbias), added in order by norm_finish_kernel.
+template <typename T, int NT, int G, int V, bool FULL>
+__global__ __launch_bounds__(NT, 4) void norm_bwd_kernel(T* __restrict__ dx, float* __restrict__ partial,
                                                       const T* __restrict__ dy, const T* __restrict__ x,
                                                       const float* __restrict__ weight,
                                                       const float* __restrict__ stats, int M, int D, int layer,
@@ -209,51 +228,75 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(T* __restrict__ dx, float*
   constexpr int R = NT / G;
   const int lane = threadIdx.x % G, team = threadIdx.x / G;
   float w[V][8], sw[V][8], sb[V][8];
-#pragma unroll
-  for (int c = 0; c < V; ++c) {
+  const auto load_w = [&](int c) {
     if (weight) {
       load8(weight, 8 * (lane + G * c), D, w[c]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[c][j] = 1.f;
     }
+  };
+  constexpr bool kKeep = V == 1;  // the weight stays in registers; the widest form reads it (from L2) per row
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    if (kKeep) load_w(c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) sw[c][j] = sb[c][j] = 0.f;
   }
+  Eight<T> nx[V], ny[V];
+  float nr = 0.f, nm = 0.f;
+  const auto request = [&](long long row) {
+    const int n = row < M ? D : 0;
+    nr = n ? stats[row] : 0.f;
+    nm = FULL && n && layer ? stats[(long long)M + row] : 0.f;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      nx[c] = load_raw(x + row * D, 8 * (lane + G * c), n);
+      ny[c] = load_raw(dy + row * D, 8 * (lane + G * c), n);
+    }
+  };
+  constexpr bool kAhead = V == 1;  // the widest form has no registers for a second row
+  const long long step = (long long)gridDim.x * R;
   int phase = 0;
-  for (long long first = (long long)blockIdx.x * R; first < M; first += (long long)gridDim.x * R) {
+  if (kAhead) request((long long)blockIdx.x * R + team);
+  for (long long first = (long long)blockIdx.x * R; first < M; first += step) {
     const long long row = first + team;
     const bool live = row < M;
-    const int n = live ? D : 0;
-    const float r = live ? stats[row] : 0.f, mean = live && layer ? stats[(long long)M + row] : 0.f;
-    float xh[V][8], t[V][8];
+    if (!kAhead) request(row);
+    const float r = nr, mean = nm;
+    Eight<T> cx[V], cy[V];
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < V; ++c) {
       const int i = 8 * (lane + G * c);
-      load8(x + row * D, i, n, xh[c]);
-      load8(dy + row * D, i, n, t[c]);
+      cx[c] = nx[c];
+      cy[c] = ny[c];
+      if (!kKeep) load_w(c);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        xh[c][j] = i + j < n ? (xh[c][j] - mean) * r : 0.f;
-        sw[c][j] += t[c][j] * xh[c][j];
-        sb[c][j] += t[c][j];
-        t[c][j] *= w[c][j];
-        s[0] += t[c][j];
-        s[1] += t[c][j] * xh[c][j];
+        const float g = (float)cy[c].v[j], t = g * w[c][j];
+        const float xh = live && i + j < D ? ((float)cx[c].v[j] - mean) * r : 0.f;
+        sw[c][j] = fmaf(g, xh, sw[c][j]);
+        if (FULL) sb[c][j] += g;
+        if (FULL) s[0] += t;
+        s[1] = fmaf(t, xh, s[1]);
       }
     }
+    if (kAhead) request(row + step);
     team_sum<G, 2>(s, buf[phase]);
     phase ^= 1;
     if (!live) continue;
-    const float m0 = layer ? s[0] / (float)D : 0.f, m1 = s[1] / (float)D;
+    const float m0 = FULL && layer ? s[0] / (float)D : 0.f, m1 = s[1] / (float)D;
 #pragma unroll
     for (int c = 0; c < V; ++c) {
       const int i = 8 * (lane + G * c);
       if (i >= D) continue;
+      if (!kKeep) load_w(c);
+      float o[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t[c][j] = r * (t[c][j] - m0 - xh[c][j] * m1);
-      store8(dx + row * D, i, D, t[c]);
+      for (int j = 0; j < 8; ++j)
+        o[j] = r * fmaf(-((float)cx[c].v[j] - mean) * r, m1, (float)cy[c].v[j] * w[c][j] - m0);
+      store8(dx + row * D, i, D, o);
     }
   }
   for (int which = 0; which < 2; ++which) {
@@ -293,7 +336,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_long_kernel(T* __restrict__ dx,
     for (int j = 0; j < 8; ++j) {
       const float t = b[j] * w[j];
       s[0] += t;
-      s[1] += i + j < D ? t * ((a[j] - mean) * r) : 0.f;
+      if (i + j < D) s[1] = fmaf(t, (a[j] - mean) * r, s[1]);
     }
   }
   team_sum<1024, 2>(s, buf);
@@ -303,7 +346,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_long_kernel(T* __restrict__ dx,
     load8(dy + row * D, i, D, b);
     if (weight) load8(weight, i, D, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = r * (b[j] * w[j] - m0 - (a[j] - mean) * r * m1);
+    for (int j = 0; j < 8; ++j) a[j] = r * fmaf(-(a[j] - mean) * r, m1, b[j] * w[j] - m0);
     store8(dx + row * D, i, D, a);
   }
 }
@@ -319,35 +362,41 @@ __global__ __launch_bounds__(256) void norm_cols_long_kernel(float* __restrict__
   for (long long row = blockIdx.y; row < M; row += gridDim.y) {
     const float t = (float)dy[row * D + i];
     const float mean = layer ? stats[(long long)M + row] : 0.f;
-    sw += t * (((float)x[row * D + i] - mean) * stats[row]);
+    sw = fmaf(t, ((float)x[row * D + i] - mean) * stats[row], sw);
     sb += t;
   }
   partial[((long long)blockIdx.y * 2) * D + i] = sw;
   partial[((long long)blockIdx.y * 2 + 1) * D + i] = sb;
 }
 
-// The partial sums of `count` work-groups, added in order: 64 columns per work-group, each of its four
-// waves a quarter of the partials.
-__global__ __launch_bounds__(256) void norm_finish_kernel(float* __restrict__ dweight, float* __restrict__ dbias,
-                                                          const float* __restrict__ partial, int count, int D)
+// The partial sums of `count` work-groups, added in a fixed order: 64 columns per work-group, each of its
+// sixteen waves a run of the partials.
+__global__ __launch_bounds__(1024) void norm_finish_kernel(float* __restrict__ dweight, float* __restrict__ dbias,
+                                                           const float* __restrict__ partial, int count, int D)
 {
-  __shared__ float part[4][64];
-  const int which = blockIdx.y, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + (threadIdx.x & 63);
+  __shared__ float part[16][64];
+  const int which = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = blockIdx.x * 64 + lane;
   float* out = which ? dbias : dweight;
   if (!out) return;
   float s = 0.f;
   if (col < D) {
-    const int per = (count + 3) / 4, end = min(count, (wave + 1) * per);
-    for (int k = wave * per; k < end; ++k) s += partial[((long long)k * 2 + which) * D + col];
+    const int per = (count + 15) / 16, end = min(count, (wave + 1) * per);
+    const float* q = partial + (long long)which * D + col;
+#pragma unroll 8
+    for (int k = wave * per; k < end; ++k) s += q[(long long)k * 2 * D];
   }
-  part[wave][threadIdx.x & 63] = s;
+  part[wave][lane] = s;
   __syncthreads();
-  if (wave == 0 && col < D)
-    out[col] = ((part[0][threadIdx.x] + part[1][threadIdx.x]) + part[2][threadIdx.x]) + part[3][threadIdx.x];
+  if (wave == 0 && col < D) {
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += part[k][lane];
+    out[col] = s;
+  }
 }
 
 constexpr int kNormRegisterRow = 16384;  // longest row kept in registers
-constexpr int kNormBwdGroups = 256;      // work-groups (and partial sums) of the backward: one per CU
+constexpr int kNormBwdGroups = 512;      // most work-groups (and partial sums) of the backward: two per CU
 
 template <typename T, int NT, int G, int V>
 hipError_t norm_fwd(void* y, float* stats, const void* x, const float* w, const float* b, int M, int D, float eps,
@@ -365,7 +414,11 @@ hipError_t norm_fwd_any(void* y, float* stats, const void* x, const float* w, co
   if (D <= 128) return norm_fwd<T, 256, 16, 1>(y, stats, x, w, b, M, D, eps, layer, s);
   if (D <= 512) return norm_fwd<T, 256, 64, 1>(y, stats, x, w, b, M, D, eps, layer, s);
   if (D <= 2048) return norm_fwd<T, 256, 256, 1>(y, stats, x, w, b, M, D, eps, layer, s);
-  if (D <= 8192) return norm_fwd<T, 1024, 1024, 1>(y, stats, x, w, b, M, D, eps, layer, s);
+  // longer rows: one work-group per row of sixteen waves while there are few rows, fewer
+  // waves per row, which wait less for each other, where there are enough rows to fill the chip
+  if (M < 2 * 256 && D <= 8192) return norm_fwd<T, 1024, 1024, 1>(y, stats, x, w, b, M, D, eps, layer, s);
+  if (D <= 4096) return norm_fwd<T, 256, 256, 2>(y, stats, x, w, b, M, D, eps, layer, s);
+  if (D <= 8192) return norm_fwd<T, 512, 512, 2>(y, stats, x, w, b, M, D, eps, layer, s);
   if (D <= kNormRegisterRow) return norm_fwd<T, 1024, 1024, 2>(y, stats, x, w, b, M, D, eps, layer, s);
   hipLaunchKernelGGL((norm_fwd_long_kernel<T>), dim3((unsigned)M), dim3(1024), 0, s, (T*)y, stats, (const T*)x, w, b, M,
                      D, eps, layer);
@@ -377,9 +430,10 @@ hipError_t norm_bwd(void* dx, float* partial, int& groups, const void* dy, const
                     const float* stats, int M, int D, int layer, int want_w, int want_b, hipStream_t s)
 {
   constexpr int R = NT / G;
-  groups = std::min((M + R - 1) / R, kNormBwdGroups);
-  hipLaunchKernelGGL((norm_bwd_kernel<T, NT, G, V>), dim3((unsigned)groups), dim3(NT), 0, s, (T*)dx, partial,
-                     (const T*)dy, (const T*)x, w, stats, M, D, layer, want_w, want_b);
+  groups = std::min((M + R - 1) / R, NT == 1024 ? kNormBwdGroups / 2 : kNormBwdGroups);
+  const auto kernel = layer || want_b ? norm_bwd_kernel<T, NT, G, V, true> : norm_bwd_kernel<T, NT, G, V, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(NT), 0, s, (T*)dx, partial, (const T*)dy, (const T*)x, w,
+                     stats, M, D, layer, want_w, want_b);
   return hipGetLastError();
 }
 template <typename T>
@@ -391,11 +445,13 @@ hipError_t norm_bwd_any(void* dx, float* dweight, float* dbias, const void* dy, 
   hipError_t e = hipSuccess;
   if (M <= 0) {
   } else if (D <= 128) {
-    e = norm_bwd<T, 1024, 16, 1>(dx, partial, groups, dy, x, w, stats, M, D, layer, ww, wb, s);
+    e = norm_bwd<T, 512, 16, 1>(dx, partial, groups, dy, x, w, stats, M, D, layer, ww, wb, s);
   } else if (D <= 512) {
-    e = norm_bwd<T, 1024, 64, 1>(dx, partial, groups, dy, x, w, stats, M, D, layer, ww, wb, s);
+    e = norm_bwd<T, 512, 64, 1>(dx, partial, groups, dy, x, w, stats, M, D, layer, ww, wb, s);
   } else if (D <= 2048) {
-    e = norm_bwd<T, 1024, 256, 1>(dx, partial, groups, dy, x, w, stats, M, D, layer, ww, wb, s);
+    e = norm_bwd<T, 512, 256, 1>(dx, partial, groups, dy, x, w, stats, M, D, layer, ww, wb, s);
+  } else if (D <= 4096) {
+    e = norm_bwd<T, 512, 512, 1>(dx, partial, groups, dy, x, w, stats, M, D, layer, ww, wb, s);
   } else if (D <= 8192) {
     e = norm_bwd<T, 1024, 1024, 1>(dx, partial, groups, dy, x, w, stats, M, D, layer, ww, wb, s);
   } else if (D <= kNormRegisterRow) {
@@ -412,7 +468,7 @@ hipError_t norm_bwd_any(void* dx, float* dweight, float* dbias, const void* dy, 
     }
   }
   if (e != hipSuccess || !(ww || wb)) return e;
-  hipLaunchKernelGGL(norm_finish_kernel, dim3((unsigned)((D + 63) / 64), 2), dim3(256), 0, s, dweight, dbias, partial,
+  hipLaunchKernelGGL(norm_finish_kernel, dim3((unsigned)((D + 63) / 64), 2), dim3(1024), 0, s, dweight, dbias, partial,
                      groups, D);
   return hipGetLastError();
 }
