@@ -22,6 +22,11 @@ template <typename T>
 struct Elem;
 template <>
 struct Elem<__bf16> {
+  static MX_DEV f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c)
+  {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  }
   static MX_DEV f32x16 mfma(i32x4 a, i32x4 b, f32x16 c)
   {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
@@ -30,6 +35,11 @@ struct Elem<__bf16> {
 };
 template <>
 struct Elem<_Float16> {
+  static MX_DEV f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c)
+  {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+  }
   static MX_DEV f32x16 mfma(i32x4 a, i32x4 b, f32x16 c)
   {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
@@ -427,21 +437,24 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   });
 }
 
-// The runs' partial sums, added in order, and the epilogue: a thread per 8 columns of a row.
+// The runs' partial sums, added in order, and the epilogue: a thread per 8 columns of a row, one wave per
+// work-group, so that the few threads of few rows spread over the CUs.
 template <typename T, DenseEpi EPI>
-__global__ __launch_bounds__(256) void dense_finish_kernel(DenseArgs p)
+__global__ __launch_bounds__(64) void dense_finish_kernel(DenseArgs p)
 {
   const int per_row = p.N / 8;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long i = (long long)blockIdx.x * 64 + threadIdx.x;
   if (i >= (long long)p.M * per_row) return;
   const int row = (int)(i / per_row), col = (int)(i % per_row) * 8;
   float v[8] = {}, u[8] = {};
   constexpr int W = EPI == kDenseGlu ? 2 : 1;
   const long long stride = (long long)p.M * p.N * W;
   const float* q = p.partial + (long long)row * p.N * W + col;
-  for (int k = 0; k < p.splits; ++k, q += stride) {
-    add_sums(q, v);
-    if constexpr (EPI == kDenseGlu) add_sums(q + p.N, u);
+  // eight runs' loads in flight: with few rows the loop is its loads' latency and nothing else
+#pragma unroll 8
+  for (int k = 0; k < p.splits; ++k) {
+    add_sums(q + k * stride, v);
+    if constexpr (EPI == kDenseGlu) add_sums(q + k * stride + p.N, u);
   }
   if constexpr (EPI == kDenseGlu)
     epi_glu<T, 8>(p, row, col, v, u);
@@ -449,6 +462,93 @@ __global__ __launch_bounds__(256) void dense_finish_kernel(DenseArgs p)
     epi_dglu<T, 8>(p, row, col, v);
   else
     epi_store<T, 8>(p, row, col, v);
+}
+
+// ------------------------------------------------------------------ few rows
+// The forward products of up to 16 rows: bound by reading the weights once, so a work-group takes only 16
+// weight rows (kDenseGlu: 8 of gate and the same 8 of up), which gives every CU some, and its eight waves
+// cut K among them: each streams its run of the rows straight into the registers of
+// v_mfma_f32_16x16x32 (lane l: weight row l % 16, terms 8 (l / 16)..+7 of 32, the next steps' loads in
+// flight), and the eight sums meet in LDS in a fixed order. No partial sums in memory, no second launch.
+// Rows past the last (of x or of the weights) read the last one's bytes and are not stored.
+// One row, D = 7168, F = 2048: gate/up 12.9 us (58.7 MB, 4.5 TB/s), down 9.3; 64 x 128 tiles with eight and
+// eight runs of K and their joins 18.0 and 11.4. With 32 rows, each wave reading 2 x 16 rows of x beside
+// its weights, 25 and 14 us against 18 and 12: the tiles take those.
+constexpr int kFewRows = 16;
+
+template <typename T, DenseEpi EPI>
+__global__ __launch_bounds__(512) void dense_few_kernel(DenseArgs p)
+{
+  constexpr int NW = 8, U = 8;  // waves; steps of 32 terms in flight, twice
+  __shared__ __attribute__((aligned(16))) float sums[NW][kFewRows][16];
+  __shared__ __attribute__((aligned(16))) float total[kFewRows][16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, q = lane >> 4;
+  constexpr int kCols = EPI == kDenseGlu ? 8 : 16;
+  const int n0 = blockIdx.x * kCols;
+  const int wrow = min(n0 + (EPI == kDenseGlu ? i & 7 : i), p.N - 1);
+  const T* wp = static_cast<const T*>(EPI == kDenseGlu && i >= 8 ? p.b[1] : p.b[0]) + wrow * p.ldb + 8 * q;
+  const T* xp = static_cast<const T*>(p.a[0]) + min(i, p.M - 1) * p.lda + 8 * q;
+
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  // whole steps [s, end) of this wave; the partial step at the end of K is the last wave's extra one
+  const int whole = p.K / 32, per = (whole + NW - 1) / NW;
+  int s = min(wave * per, whole);
+  const int end = min(s + per, whole);
+  i32x4 w[2][U], x[2][U];
+  const auto request = [&](auto h, int first) {
+    static_for<U>([&](auto u) {
+      const int k = min(first + u, end - 1) * 32;  // past the run: its last step again, not used
+      w[h][u] = *reinterpret_cast<const i32x4*>(wp + k);
+      x[h][u] = *reinterpret_cast<const i32x4*>(xp + k);
+    });
+  };
+  const auto multiply = [&](auto h, int n) {
+    static_for<U>([&](auto u) {
+      if (u < n) acc = Elem<T>::mfma16(w[h][u], x[h][u], acc);
+    });
+  };
+  using Zero = std::integral_constant<int, 0>;
+  using One = std::integral_constant<int, 1>;
+  if (s < end) {
+    request(Zero{}, s);
+    for (; s < end; s += 2 * U) {
+      if (s + U < end) request(One{}, s + U);
+      multiply(Zero{}, end - s);
+      if (s + 2 * U < end) request(Zero{}, s + 2 * U);
+      if (s + U < end) multiply(One{}, end - s - U);
+    }
+  }
+  if (wave == NW - 1 && whole * 32 < p.K) {
+    const bool in = whole * 32 + 8 * q < p.K;
+    const int k = in ? whole * 32 : -8 * q;  // a lane past K: terms 0.., taken as zeros
+    const i32x4 zero = {0, 0, 0, 0};
+    const i32x4 wt = *reinterpret_cast<const i32x4*>(wp + k), xt = *reinterpret_cast<const i32x4*>(xp + k);
+    acc = Elem<T>::mfma16(in ? wt : zero, in ? xt : zero, acc);
+  }
+  *reinterpret_cast<f32x4*>(&sums[wave][i][4 * q]) = acc;
+  __syncthreads();
+  if (threadIdx.x < kFewRows * 16) {
+    float t = 0.f;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) t += (&sums[v][0][0])[threadIdx.x];
+    (&total[0][0])[threadIdx.x] = t;
+  }
+  __syncthreads();
+  constexpr int kGroups = EPI == kDenseGlu ? 1 : 2;  // of 8 columns
+  const int row = threadIdx.x / kGroups, c = threadIdx.x % kGroups * 8;
+  if (row >= p.M || n0 + c >= p.N) return;
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = total[row][c + j];
+  if constexpr (EPI == kDenseGlu) {
+    float u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = total[row][8 + j];
+    epi_glu<T, 8>(p, row, n0, v, u);
+  } else {
+    epi_store<T, 8>(p, row, n0 + c, v);
+  }
 }
 
 // The tiles there are (kDenseGlu: half the columns are columns of h), one work-group per CU each, and what
@@ -464,6 +564,8 @@ constexpr Tile kTiles[] = {{256, 256, 1.13f, 1.80f, 8.f}, {128, 256, 0.66f, 1.02
 constexpr int kNTiles = sizeof(kTiles) / sizeof(kTiles[0]);
 constexpr int kCUs = 256;
 constexpr int kMaxSplits = 16;
+
+constexpr int kFewTile = -1;  // dense_few_kernel
 
 struct Plan {
   int tile, splits, run;
@@ -481,6 +583,7 @@ Plan plan_dense(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg)
   const long long cols = epi == kDenseGlu ? 2LL * N : N;
   const int steps = (K + kDenseStep - 1) / kDenseStep * nseg;
   const float stream = ((float)cols + M) * K * nseg * 2.f / 4.5e6f;  // the operands once from HBM
+  if (shape == kDenseForward && M <= kFewRows) return {kFewTile, 1, steps, stream + 4.f};
   Plan best = {0, 1, steps, 1e30f};
   for (int t = 0; t < kNTiles; ++t) {
     const Tile& tile = kTiles[t];
@@ -492,7 +595,7 @@ Plan plan_dense(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg)
       float us = full * (run * tile.busy * slow + tile.ends);
       if (rest) us += run * (tile.step + (tile.busy - tile.step) * rest / kCUs) * slow + tile.ends;
       us = std::max(us, stream);
-      if (splits > 1) us += 4.f + (float)M * cols * splits * 1.5e-6f;
+      if (splits > 1) us += 3.f + 0.3f * splits + (float)M * cols * splits * 1.5e-6f;
       if (us < best.us) best = {t, splits, run, us};
       if (tiles * splits >= 4 * kCUs) break;
     }
@@ -509,7 +612,7 @@ void launch_tiles(const DenseArgs& a, int splits, hipStream_t s)
 
 // A product whose last tile row is nearly empty takes its whole tile rows first and the rows behind them by
 // themselves, where the two are expected to be quicker (4099 rows, gate/up: 4096 in one round of 256 x 256
-// tiles and 3 rows, 225 us; two rounds 340).
+// tiles and 3 rows, 220 us; two rounds 340).
 struct Cut {
   int rows;  // of the first part; M: one part
   Plan first, rest;
@@ -537,6 +640,12 @@ size_t plan_bytes(const Plan& p, DenseEpi epi, int M, int N)
 template <typename T, DenseShape SH, DenseEpi EPI>
 hipError_t launch_plan(const Plan& plan, DenseArgs a, float* partial, hipStream_t s)
 {
+  if constexpr (SH == kDenseForward)
+    if (plan.tile == kFewTile) {
+      const int cols = EPI == kDenseGlu ? 8 : 16;
+      hipLaunchKernelGGL((dense_few_kernel<T, EPI>), dim3((unsigned)((a.N + cols - 1) / cols)), dim3(512), 0, s, a);
+      return hipGetLastError();
+    }
   const Tile& tile = kTiles[plan.tile];
   const int cols = EPI == kDenseGlu ? tile.cols / 2 : tile.cols;
   a.tiles_m = (a.M + tile.rows - 1) / tile.rows;
@@ -551,8 +660,8 @@ hipError_t launch_plan(const Plan& plan, DenseArgs a, float* partial, hipStream_
     default: launch_tiles<T, 2, 2, 1, 2, 5, SH, EPI>(a, plan.splits, s); break;
   }
   if (plan.splits > 1)
-    hipLaunchKernelGGL((dense_finish_kernel<T, EPI>), dim3((unsigned)(((long long)a.M * (a.N / 8) + 255) / 256)),
-                       dim3(256), 0, s, a);
+    hipLaunchKernelGGL((dense_finish_kernel<T, EPI>), dim3((unsigned)(((long long)a.M * (a.N / 8) + 63) / 64)),
+                       dim3(64), 0, s, a);
   return hipGetLastError();
 }
 
