@@ -404,9 +404,8 @@ class MXFP4Kernel:
             raise ValueError(f"top_k must lie in [1, min(E, 64)] = [1, {min(E, 64)}], got {top_k}")
 
     # -- dense operators ---------------------------------------------------------------------
-    # Device tensors only (ValueError otherwise); lazylora_amd.dense wraps these in autograd. Small calls
-    # are bound by host work, so each public method checks its arguments and an inner one, which the
-    # backward passes call with what their forward checked, launches.
+    # Device tensors only (ValueError otherwise): the C entry points as they are, forward and backward by
+    # themselves; lazylora_amd.dense offers them differentiable.
     def ffn_forward(self, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
                     act="swiglu", gate_delta: Optional[torch.Tensor] = None,
                     up_delta: Optional[torch.Tensor] = None, save_for_backward: bool = False):
@@ -454,12 +453,6 @@ class MXFP4Kernel:
         grad_h = grad_h if grad_h is None else _arg(grad_h, "grad_h", (M, F), dt, dev)
         x = _arg(x, "x", (M, D), dt, dev) if need_w_in else None
         h = _arg(h, "h", (M, F), dt, dev) if need_w_down else None
-        return self._ffn_backward(grad_y, gu, w, code, kind, grad_h, x, h, need_x)
-
-    def _ffn_backward(self, grad_y, gu, w, code, kind, grad_h, x, h, need_x):
-        dt, dev = grad_y.dtype, grad_y.device
-        M, Do = grad_y.shape
-        F, D = w[0].shape
         dgu = torch.empty((M, 2 * F), dtype=dt, device=dev)
         dx = torch.empty((M, D), dtype=dt, device=dev) if need_x else None
         dwg = dwu = dwd = None
@@ -514,13 +507,7 @@ class MXFP4Kernel:
         stats = _arg(stats, "stats", (2, M), torch.float32, dev)
         if weight is not None:
             weight = _arg(weight, "weight", (D,), torch.float32, dev)
-        return self._norm_backward(grad_y, x.contiguous(), weight, stats, kind, need_weight, need_bias)
-
-    def _norm_backward(self, grad_y, x, weight, stats, kind, need_weight, need_bias):
-        M, D = x.shape
-        dev = x.device
-        if not grad_y.is_contiguous():
-            grad_y = grad_y.contiguous()
+        x, grad_y = x.contiguous(), grad_y.contiguous()
         dx = torch.empty_like(x)
         dw = torch.empty(D, dtype=torch.float32, device=dev) if need_weight else None
         db = torch.empty(D, dtype=torch.float32, device=dev) if need_bias else None
@@ -546,9 +533,6 @@ class MXFP4Kernel:
                 raise ValueError("a seed tensor must hold one int64 on x's device")
         elif not 0 <= seed < 2 ** 64:
             raise ValueError(f"seed must lie in [0, 2^64), got {seed}")
-        return self._dropout(x, p, seed, stream)
-
-    def _dropout(self, x, p, seed, stream):
         x = x.contiguous()
         y = torch.empty_like(x)
         number, where = (0, seed.data_ptr()) if isinstance(seed, torch.Tensor) else (seed, None)

@@ -83,3 +83,19 @@ def test_dropout_refusals(lib):
                {"p": float("nan")}, {"dtype": I32}):
         assert call(**kw) == -1, kw
     assert call(n=0, x=None, y=None) == 0
+
+
+def test_operators_raise_where_the_library_is_off(monkeypatch):
+    import torch
+    from lazylora_amd import dense
+    monkeypatch.setenv("LAZYLORA_NO_NATIVE", "1")
+    x = torch.zeros(4, 8)
+    for call in (lambda: dense.rms_norm(x), lambda: dense.layer_norm(x), lambda: dense.dropout(x, 0.5, 1),
+                 lambda: dense.gated_ffn(x, x, x, x.T)):
+        with pytest.raises(RuntimeError, match="unavailable"):
+            call()
+
+
+def test_autograd_module_is_built():
+    from lazylora_amd import _dense_autograd
+    assert all(hasattr(_dense_autograd, n) for n in ("norm", "dropout", "gated_ffn"))
