@@ -282,7 +282,8 @@ int mxfp4_ffn_backward(void *dx, void *dw_gate, void *dw_up, void *dw_down, void
  * lazy_lora/streaming/trunk_streamer.py:23-34, is the RMS form):
  *   m = mean(x) (0 for MXFP4_NORM_RMS), r = 1 / sqrt(mean((x - m)^2) + eps),
  *   y = (x - m) r * weight + bias.
- * x and y [M, D] of dtype MXFP4_F32, _BF16 or _F16; weight and bias [D] fp32, each may be NULL.
+ * x and y [M, D] of dtype MXFP4_F32, _BF16 or _F16, 1 <= D <= 2^20; weight and bias [D] fp32, each may
+ * be NULL.
  * stats: 2 M floats (r, then m for layer norm) for the backward, or NULL. */
 #define MXFP4_NORM_RMS 0
 #define MXFP4_NORM_LAYER 1
