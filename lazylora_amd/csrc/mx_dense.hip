@@ -465,47 +465,62 @@ __global__ __launch_bounds__(64) void dense_finish_kernel(DenseArgs p)
 }
 
 // ------------------------------------------------------------------ few rows
-// The forward products of up to 16 rows: bound by reading the weights once, so a work-group takes only 16
-// weight rows (kDenseGlu: 8 of gate and the same 8 of up), which gives every CU some, and its eight waves
-// cut K among them: each streams its run of the rows straight into the registers of
-// v_mfma_f32_16x16x32 (lane l: weight row l % 16, terms 8 (l / 16)..+7 of 32, the next steps' loads in
-// flight), and the eight sums meet in LDS in a fixed order. No partial sums in memory, no second launch.
-// Rows past the last (of x or of the weights) read the last one's bytes and are not stored.
-// One row, D = 7168, F = 2048: gate/up 12.9 us (58.7 MB, 4.5 TB/s), down 9.3; 64 x 128 tiles with eight and
-// eight runs of K and their joins 18.0 and 11.4. With 32 rows, each wave reading 2 x 16 rows of x beside
-// its weights, 25 and 14 us against 18 and 12: the tiles take those.
-constexpr int kFewRows = 16;
+// The forward products of up to 64 rows: bound by reading the weights once, so a work-group takes only
+// 16 WB weight rows (kDenseGlu: half of them gate, the same of up), which gives many CUs some, and its eight
+// waves cut K among them: each streams its run of the rows straight into the registers of
+// v_mfma_f32_16x16x32 (lane l: weight row l % 16, terms 8 (l / 16)..+7 of 32; MB blocks of 16 rows of x the
+// same way, from L2; the next steps' loads in flight), and the eight sums meet in LDS in a fixed order. No
+// partial sums in memory, no second launch. Rows past the last (of x or of the weights) read the last one's
+// bytes and are not stored. A CU takes about 36 bytes per ns this way, its work-group's weight rows and all
+// of x: two blocks of weight rows (x read half as often) pay where one would mean a second round.
+// One row, D = 7168, F = 2048: gate/up 13 us (58.7 MB, 4.5 TB/s), where 64 x 128 tiles with eight runs of K
+// and their join take 18. 37 rows, D = 3584, F = 1536, down: 8 us against 12; gate/up 16 against 14.
+constexpr int kFewRows = 64;
 
-template <typename T, DenseEpi EPI>
+template <typename T, int WB, int MB, DenseEpi EPI>
 __global__ __launch_bounds__(512) void dense_few_kernel(DenseArgs p)
 {
-  constexpr int NW = 8, U = 8;  // waves; steps of 32 terms in flight, twice
-  __shared__ __attribute__((aligned(16))) float sums[NW][kFewRows][16];
-  __shared__ __attribute__((aligned(16))) float total[kFewRows][16];
+  constexpr int NW = 8, U = WB + MB <= 3 ? 8 : 4;  // waves; steps of 32 terms in flight, twice
+  constexpr int kRows = 16 * MB, kWide = 16 * WB;
+  __shared__ __attribute__((aligned(16))) float sums[NW][kRows][kWide];
+  __shared__ __attribute__((aligned(16))) float total[kRows][kWide];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
-  constexpr int kCols = EPI == kDenseGlu ? 8 : 16;
+  constexpr int kCols = EPI == kDenseGlu ? kWide / 2 : kWide;
   const int n0 = blockIdx.x * kCols;
-  const int wrow = min(n0 + (EPI == kDenseGlu ? i & 7 : i), p.N - 1);
-  const T* wp = static_cast<const T*>(EPI == kDenseGlu && i >= 8 ? p.b[1] : p.b[0]) + wrow * p.ldb + 8 * q;
-  const T* xp = static_cast<const T*>(p.a[0]) + min(i, p.M - 1) * p.lda + 8 * q;
+  const T* wp[WB];
+  const T* xp[MB];
+#pragma unroll
+  for (int b = 0; b < WB; ++b) {
+    const int r = 16 * b + i, up = EPI == kDenseGlu && r >= kCols;
+    wp[b] = static_cast<const T*>(p.b[up]) + min(n0 + (up ? r - kCols : r), p.N - 1) * p.ldb + 8 * q;
+  }
+#pragma unroll
+  for (int b = 0; b < MB; ++b) xp[b] = static_cast<const T*>(p.a[0]) + min(16 * b + i, p.M - 1) * p.lda + 8 * q;
 
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[MB][WB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int b = 0; b < WB; ++b) acc[m][b] = f32x4{0.f, 0.f, 0.f, 0.f};
   // whole steps [s, end) of this wave; the partial step at the end of K is the last wave's extra one
   const int whole = p.K / 32, per = (whole + NW - 1) / NW;
   int s = min(wave * per, whole);
   const int end = min(s + per, whole);
-  i32x4 w[2][U], x[2][U];
+  i32x4 w[2][U][WB], x[2][U][MB];
   const auto request = [&](auto h, int first) {
     static_for<U>([&](auto u) {
       const int k = min(first + u, end - 1) * 32;  // past the run: its last step again, not used
-      w[h][u] = *reinterpret_cast<const i32x4*>(wp + k);
-      x[h][u] = *reinterpret_cast<const i32x4*>(xp + k);
+      static_for<WB>([&](auto b) { w[h][u][b] = *reinterpret_cast<const i32x4*>(wp[b] + k); });
+      static_for<MB>([&](auto b) { x[h][u][b] = *reinterpret_cast<const i32x4*>(xp[b] + k); });
     });
   };
   const auto multiply = [&](auto h, int n) {
     static_for<U>([&](auto u) {
-      if (u < n) acc = Elem<T>::mfma16(w[h][u], x[h][u], acc);
+      if (u < n)
+        static_for<MB>([&](auto m) {
+          static_for<WB>([&](auto b) { acc[m][b] = Elem<T>::mfma16(w[h][u][b], x[h][u][m], acc[m][b]); });
+        });
     });
   };
   using Zero = std::integral_constant<int, 0>;
@@ -523,19 +538,28 @@ __global__ __launch_bounds__(512) void dense_few_kernel(DenseArgs p)
     const bool in = whole * 32 + 8 * q < p.K;
     const int k = in ? whole * 32 : -8 * q;  // a lane past K: terms 0.., taken as zeros
     const i32x4 zero = {0, 0, 0, 0};
-    const i32x4 wt = *reinterpret_cast<const i32x4*>(wp + k), xt = *reinterpret_cast<const i32x4*>(xp + k);
-    acc = Elem<T>::mfma16(in ? wt : zero, in ? xt : zero, acc);
+    i32x4 wt[WB];
+    static_for<WB>([&](auto b) {
+      const i32x4 v = *reinterpret_cast<const i32x4*>(wp[b] + k);
+      wt[b] = in ? v : zero;
+    });
+    static_for<MB>([&](auto m) {
+      const i32x4 v = *reinterpret_cast<const i32x4*>(xp[m] + k);
+      static_for<WB>([&](auto b) { acc[m][b] = Elem<T>::mfma16(wt[b], in ? v : zero, acc[m][b]); });
+    });
   }
-  *reinterpret_cast<f32x4*>(&sums[wave][i][4 * q]) = acc;
+  static_for<MB>([&](auto m) {
+    static_for<WB>([&](auto b) { *reinterpret_cast<f32x4*>(&sums[wave][16 * m + i][16 * b + 4 * q]) = acc[m][b]; });
+  });
   __syncthreads();
-  if (threadIdx.x < kFewRows * 16) {
+  for (int e = threadIdx.x; e < kRows * kWide; e += 512) {
     float t = 0.f;
 #pragma unroll
-    for (int v = 0; v < NW; ++v) t += (&sums[v][0][0])[threadIdx.x];
-    (&total[0][0])[threadIdx.x] = t;
+    for (int v = 0; v < NW; ++v) t += (&sums[v][0][0])[e];
+    (&total[0][0])[e] = t;
   }
   __syncthreads();
-  constexpr int kGroups = EPI == kDenseGlu ? 1 : 2;  // of 8 columns
+  constexpr int kGroups = kCols / 8;  // of 8 columns
   const int row = threadIdx.x / kGroups, c = threadIdx.x % kGroups * 8;
   if (row >= p.M || n0 + c >= p.N) return;
   float v[8];
@@ -544,11 +568,27 @@ __global__ __launch_bounds__(512) void dense_few_kernel(DenseArgs p)
   if constexpr (EPI == kDenseGlu) {
     float u[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = total[row][8 + j];
-    epi_glu<T, 8>(p, row, n0, v, u);
+    for (int j = 0; j < 8; ++j) u[j] = total[row][kCols + c + j];
+    epi_glu<T, 8>(p, row, n0 + c, v, u);
   } else {
     epi_store<T, 8>(p, row, n0 + c, v);
   }
+}
+
+template <typename T, int WB, DenseEpi EPI>
+hipError_t launch_few(const DenseArgs& a, hipStream_t s)
+{
+  const int cols = 16 * WB / (EPI == kDenseGlu ? 2 : 1);
+  const dim3 grid((unsigned)((a.N + cols - 1) / cols)), block(512);
+  if (a.M <= 16)
+    hipLaunchKernelGGL((dense_few_kernel<T, WB, 1, EPI>), grid, block, 0, s, a);
+  else if (a.M <= 32)
+    hipLaunchKernelGGL((dense_few_kernel<T, WB, 2, EPI>), grid, block, 0, s, a);
+  else if (a.M <= 48)
+    hipLaunchKernelGGL((dense_few_kernel<T, WB, 3, EPI>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((dense_few_kernel<T, WB, 4, EPI>), grid, block, 0, s, a);
+  return hipGetLastError();
 }
 
 // The tiles there are (kDenseGlu: half the columns are columns of h), one work-group per CU each, and what
@@ -565,7 +605,7 @@ constexpr int kNTiles = sizeof(kTiles) / sizeof(kTiles[0]);
 constexpr int kCUs = 256;
 constexpr int kMaxSplits = 16;
 
-constexpr int kFewTile = -1;  // dense_few_kernel
+constexpr int kFewOne = -1, kFewTwo = -2;  // dense_few_kernel with one and two blocks of weight rows
 
 struct Plan {
   int tile, splits, run;
@@ -583,8 +623,14 @@ Plan plan_dense(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg)
   const long long cols = epi == kDenseGlu ? 2LL * N : N;
   const int steps = (K + kDenseStep - 1) / kDenseStep * nseg;
   const float stream = ((float)cols + M) * K * nseg * 2.f / 4.5e6f;  // the operands once from HBM
-  if (shape == kDenseForward && M <= kFewRows) return {kFewTile, 1, steps, stream + 4.f};
   Plan best = {0, 1, steps, 1e30f};
+  if (shape == kDenseForward && M <= kFewRows)
+    for (int blocks = 1; blocks <= 2; ++blocks) {
+      const long long groups = (cols + 16 * blocks - 1) / (16 * blocks);
+      const float cu = 3.f + (float)((groups + kCUs - 1) / kCUs) * (16 * blocks + M) * K / 18e3f;
+      const float us = std::max(stream + 2.f, cu) + 0.1f * cu;
+      if (us < best.us) best = {blocks == 1 ? kFewOne : kFewTwo, 1, steps, us};
+    }
   for (int t = 0; t < kNTiles; ++t) {
     const Tile& tile = kTiles[t];
     const long long tiles = ((M + tile.rows - 1LL) / tile.rows) * ((cols + tile.cols - 1) / tile.cols);
@@ -641,11 +687,8 @@ template <typename T, DenseShape SH, DenseEpi EPI>
 hipError_t launch_plan(const Plan& plan, DenseArgs a, float* partial, hipStream_t s)
 {
   if constexpr (SH == kDenseForward)
-    if (plan.tile == kFewTile) {
-      const int cols = EPI == kDenseGlu ? 8 : 16;
-      hipLaunchKernelGGL((dense_few_kernel<T, EPI>), dim3((unsigned)((a.N + cols - 1) / cols)), dim3(512), 0, s, a);
-      return hipGetLastError();
-    }
+    if (plan.tile < 0)
+      return plan.tile == kFewOne ? launch_few<T, 1, EPI>(a, s) : launch_few<T, 2, EPI>(a, s);
   const Tile& tile = kTiles[plan.tile];
   const int cols = EPI == kDenseGlu ? tile.cols / 2 : tile.cols;
   a.tiles_m = (a.M + tile.rows - 1) / tile.rows;
