@@ -108,6 +108,26 @@ def test_forward_and_backward(k, M, D, F, Do, act, dt):
         check(name, got, want[name])
 
 
+@pytest.mark.parametrize("M,D,F,Do", [(4099, 520, 2056, 4104), (2050, 328, 1544, 2312), (1100, 1032, 776, 3080),
+                                      (700, 2056, 392, 1544), (3330, 2568, 4104, 2056), (1000, 7176, 520, 1544),
+                                      (1000, 1032, 2056, 264), (4096, 264, 2056, 7176), (9, 264, 2056, 4104),
+                                      (25, 136, 2056, 4104), (40, 264, 2056, 4104), (60, 328, 2056, 4104)])
+@pytest.mark.parametrize("act,dt", [("situ", torch.bfloat16), ("swiglu", torch.float16)])
+def test_large_tiles(k, M, D, F, Do, act, dt):
+    """Sizes that the large tiles take, whole and cut, with ragged last rows, columns and steps, and wide
+    products of few rows."""
+    case("large", M, D, F, Do, act, dt)
+    t = inputs(M, M, D, F, Do, dt)
+    want = reference(t, act, True)
+    y, h, gu = k.ffn_forward(t["x"], t["wg"], t["wu"], t["wd"], act, t["gd"], t["ud"], save_for_backward=True)
+    check("y", y, want["y"])
+    check("h", h, want["h"])
+    dgu, dx, dwg, dwu, dwd = k.ffn_backward(t["dy"], gu, t["wg"], t["wu"], t["wd"], act, t["dh"], t["x"], h,
+                                            need_w_in=True, need_w_down=True)
+    for name, got in (("dg", dgu[:, :F]), ("du", dgu[:, F:]), ("dx", dx), ("dwg", dwg), ("dwu", dwu), ("dwd", dwd)):
+        check(name, got, want[name])
+
+
 @pytest.mark.parametrize("M", [1, 5, 16, 31, 48, 63, 65, 96, 127, 130, 191, 200, 255, 384])
 def test_every_row_count(k, M):
     """The row count decides which kernel runs; no deltas, no grad_h, frozen weights."""
