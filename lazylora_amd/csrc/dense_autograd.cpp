@@ -1,7 +1,8 @@
 // The dense operators as autograd functions (lazylora_amd/dense.py documents them): argument checks,
-// allocation, launches through the C ABI and the backward passes, all on the host in C++. In Python a
-// training step of a small norm spent 46 of its 93 us in the backward function, which autograd runs in a
-// thread of its own, where the interpreter is several times slower than in the caller's.
+// allocation, launches through the C ABI and the backward passes, all on the host in C++. Autograd runs
+// backward functions in a thread of its own, where Python is several times slower than in the caller's:
+// forward and backward of a small norm took 103 us with Python functions and take 62 with these, of which
+// autograd itself needs 45.
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
