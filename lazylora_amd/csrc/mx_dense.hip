@@ -71,15 +71,6 @@ MX_DEV void store_sums(float* p, const float (&v)[8])
   *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
   *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
 }
-MX_DEV void add_sums(const float* p, float (&v)[8])
-{
-  const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[j] += a[j];
-    v[4 + j] += b[j];
-  }
-}
 
 // The epilogues, on NV neighbouring columns n.. of row m.
 template <typename T, int NV>
@@ -450,11 +441,31 @@ __global__ __launch_bounds__(64) void dense_finish_kernel(DenseArgs p)
   constexpr int W = EPI == kDenseGlu ? 2 : 1;
   const long long stride = (long long)p.M * p.N * W;
   const float* q = p.partial + (long long)row * p.N * W + col;
-  // eight runs' loads in flight: with few rows the loop is its loads' latency and nothing else
-#pragma unroll 8
-  for (int k = 0; k < p.splits; ++k) {
-    add_sums(q + k * stride, v);
-    if constexpr (EPI == kDenseGlu) add_sums(q + k * stride + p.N, u);
+  // eight runs' loads in flight, whatever the count (the last run's again past it, not added): with few rows
+  // the loop is its loads' latency and nothing else
+  constexpr int kAhead = 8;
+  for (int k = 0; k < p.splits; k += kAhead) {
+    f32x4 in[kAhead][2 * W];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const float* r = q + min(k + j, p.splits - 1) * stride;
+#pragma unroll
+      for (int e = 0; e < 2 * W; ++e) in[j][e] = *reinterpret_cast<const f32x4*>(r + (e >> 1) * p.N + 4 * (e & 1));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const bool add = k + j < p.splits;  // no branch: the loads would sink into it, one behind the other
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] += add ? in[j][0][e] : 0.f;
+        v[4 + e] += add ? in[j][1][e] : 0.f;
+        if constexpr (EPI == kDenseGlu) {
+          u[e] += add ? in[j][2][e] : 0.f;
+          u[4 + e] += add ? in[j][3][e] : 0.f;
+        }
+      }
+    }
   }
   if constexpr (EPI == kDenseGlu)
     epi_glu<T, 8>(p, row, col, v, u);
