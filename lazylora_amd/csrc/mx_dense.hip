@@ -609,9 +609,10 @@ hipError_t launch_few(const DenseArgs& a, hipStream_t s)
 struct Tile {
   int rows, cols;
   float step, busy, ends;
+  float row_major;  // the same step with row-major operands: twice the LDS reads, and short runs of memory
 };
-constexpr Tile kTiles[] = {{256, 256, 1.13f, 1.80f, 8.f}, {128, 256, 0.66f, 1.02f, 7.f},
-                           {128, 128, 0.45f, 0.57f, 6.f}, {64, 128, 0.28f, 0.40f, 5.f}};
+constexpr Tile kTiles[] = {{256, 256, 1.13f, 1.80f, 8.f, 1.15f}, {128, 256, 0.66f, 1.02f, 7.f, 1.15f},
+                           {128, 128, 0.50f, 0.57f, 6.f, 1.3f}, {64, 128, 0.42f, 0.42f, 5.f, 1.5f}};
 constexpr int kNTiles = sizeof(kTiles) / sizeof(kTiles[0]);
 constexpr int kCUs = 256;
 constexpr int kMaxSplits = 16;
@@ -630,7 +631,6 @@ struct Plan {
 // in one run, 129 with 256 x 256 in one, 73 in four.
 Plan plan_dense(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg)
 {
-  const float slow = shape == kDenseForward ? 1.f : 1.15f;  // row-major operands: twice the LDS reads
   const long long cols = epi == kDenseGlu ? 2LL * N : N;
   const int steps = (K + kDenseStep - 1) / kDenseStep * nseg;
   const float stream = ((float)cols + M) * K * nseg * 2.f / 4.5e6f;  // the operands once from HBM
@@ -644,6 +644,7 @@ Plan plan_dense(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg)
     }
   for (int t = 0; t < kNTiles; ++t) {
     const Tile& tile = kTiles[t];
+    const float slow = shape == kDenseForward ? 1.f : tile.row_major;
     const long long tiles = ((M + tile.rows - 1LL) / tile.rows) * ((cols + tile.cols - 1) / tile.cols);
     for (int want = 1; want <= kMaxSplits && want <= std::max(steps, 1); ++want) {
       const int run = (steps + want - 1) / want, splits = run > 0 ? (steps + run - 1) / run : 1;
@@ -652,7 +653,7 @@ Plan plan_dense(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg)
       float us = full * (run * tile.busy * slow + tile.ends);
       if (rest) us += run * (tile.step + (tile.busy - tile.step) * rest / kCUs) * slow + tile.ends;
       us = std::max(us, stream);
-      if (splits > 1) us += 3.f + 0.3f * splits + (float)M * cols * splits * 1.5e-6f;
+      if (splits > 1) us += 4.f + (float)M * cols * splits * 1.5e-6f;
       if (us < best.us) best = {t, splits, run, us};
       if (tiles * splits >= 4 * kCUs) break;
     }
