@@ -58,6 +58,15 @@ bool records(at::ArrayRef<Tensor> ts)
     if (t.defined() && t.requires_grad()) return true;
   return false;
 }
+// A launch computes values and records nothing: it would drop a tensor's forward-mode tangent, which says that
+// the derivative along it is zero. Every call and every backward pass looks at its tensors first.
+void check_modes(at::ArrayRef<Tensor> ts)
+{
+  for (const Tensor& t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
+                                "the dense operators have no forward-mode derivative (an input or upstream gradient "
+                                "carries a tangent)");
+}
 // Gradients that autograd may use but not differentiate: where a graph of them is asked for, a second
 // derivative raises instead of coming out as zero.
 variable_list once(variable_list grads)
@@ -126,6 +135,7 @@ struct Norm : torch::autograd::Function<Norm> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads)
   {
+    check_modes(grads);
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
     const NormSizes n = norm_sizes(x);
@@ -150,6 +160,7 @@ struct Norm : torch::autograd::Function<Norm> {
 Tensor norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t kind)
 {
   const Tensor w = given(weight), b = given(bias);
+  check_modes({x, w, b});
   if (records({x, w, b})) return Norm::apply(x, weight, bias, eps, kind);
   const NormSizes n = norm_sizes(x);
   return norm_run(x.contiguous(), vector_arg(w, "weight", n, x), vector_arg(b, "bias", n, x), eps, kind, n, nullptr);
@@ -179,6 +190,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads)
   {
+    check_modes(grads);
     const Tensor seed_dev = ctx->get_saved_variables()[0];
     return once({dropout_run(grads[0], ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(),
                              seed_dev, (uint64_t)ctx->saved_data["stream"].toInt()),
@@ -188,6 +200,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
 Tensor dropout(const Tensor& x, double p, uint64_t seed, const OptTensor& seed_dev, uint64_t stream)
 {
+  check_modes({x});
   TORCH_CHECK_VALUE(x.is_cuda() && dtype_code(x) >= 0,
                     "x must be a float32, bfloat16 or float16 tensor on the HIP device");
   TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "p must lie in [0, 1], got ", p);
@@ -271,6 +284,7 @@ struct Ffn : torch::autograd::Function<Ffn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads)
   {
+    check_modes(grads);
     variable_list out(8);
     const Tensor gh = grads.size() > 1 && grads[1].defined() ? tidy(grads[1]) : Tensor();
     if (!grads[0].defined() && !gh.defined()) return out;
@@ -307,6 +321,7 @@ variable_list gated_ffn(const Tensor& x, const Tensor& wg, const Tensor& wu, con
                         const OptTensor& gate_delta, const OptTensor& up_delta, bool hidden)
 {
   const Tensor gd = given(gate_delta), ud = given(up_delta);
+  check_modes({x, wg, wu, wd, gd, ud});
   if (records({x, wg, wu, wd, gd, ud})) return Ffn::apply(x, wg, wu, wd, gate_delta, up_delta, act, hidden);
   Tensor y, h;
   ffn_run(ffn_args(x, wg, wu, wd, gd, ud), act, y, h, nullptr);
