@@ -3,8 +3,11 @@
 // backward functions in a thread of its own, where Python is several times slower than in the caller's:
 // forward and backward of a small norm took 103 us with Python functions and take 62 with these, of which
 // autograd itself needs 45.
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../include/lazylora_mxfp4.h"
@@ -59,9 +62,17 @@ bool records(at::ArrayRef<Tensor> ts)
   return false;
 }
 // A launch computes values and records nothing: it would drop a tensor's forward-mode tangent, which says that
-// the derivative along it is zero. Every call and every backward pass looks at its tensors first.
+// the derivative along it is zero, and a tracer would see the outputs allocated but not filled. Every call and
+// every backward pass looks for both first.
 void check_modes(at::ArrayRef<Tensor> ts)
 {
+  using c10::impl::TorchDispatchModeTLS;
+  const bool traced = torch::jit::tracer::isTracing() ||
+                      c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+                      (TorchDispatchModeTLS::any_modes_set() &&
+                       TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
+  TORCH_CHECK_NOT_IMPLEMENTED(!traced, "the dense operators cannot be traced (torch.jit.trace, make_fx, torch.export): "
+                                       "a trace would not hold their launches");
   for (const Tensor& t : ts)
     TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
                                 "the dense operators have no forward-mode derivative (an input or upstream gradient "

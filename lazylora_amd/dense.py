@@ -10,8 +10,9 @@ They run in hand-written kernels (csrc/mx_dense.hip, csrc/mx_rows.hip), as autog
 (csrc/dense_autograd.cpp), on the current stream of their tensors' device, and raise ValueError for
 tensors they do not take; nothing falls back to torch. Sums, statistics and activation functions are
 fp32 whatever the tensors' type, and each result is rounded once. Results do not depend on timing (no
-atomics). Without a gradient to record a call saves nothing; a second derivative raises. So does
-forward-mode differentiation (NotImplementedError): the launches would drop a tangent.
+atomics). Without a gradient to record a call saves nothing; a second derivative raises. So do
+forward-mode differentiation and tracing (torch.jit.trace, make_fx; NotImplementedError): a launch
+would drop a tangent and leave no trace. torch.compile breaks its graph at a call.
 """
 from typing import Optional, Tuple, Union
 

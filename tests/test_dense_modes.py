@@ -33,3 +33,32 @@ def test_tangents_are_refused(name, grad):
                 fn(*moved)
     with pytest.raises(ValueError, match="HIP device|bfloat16"):  # without a tangent: the ordinary checks
         fn(*args)
+
+
+@pytest.mark.parametrize("name", ["norm", "dropout", "gated_ffn"])
+def test_tracers_are_refused(name):
+    """torch.jit.trace and make_fx (before and after the dispatcher) would record the outputs' allocation and
+    nothing that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    fn, args = _calls()[name]
+    with pytest.raises(NotImplementedError, match="trace"):
+        torch.jit.trace(fn, tuple(args), check_trace=False)
+    for mode in ("real", "fake"):
+        for pre in (False, True):
+            with pytest.raises(NotImplementedError, match="trace"):
+                make_fx(fn, tracing_mode=mode, pre_dispatch=pre)(*args)
+    with pytest.raises(ValueError, match="HIP device|bfloat16"):  # outside again: the ordinary checks
+        fn(*args)
+
+
+def test_other_dispatch_modes_are_not_tracers():
+    """A mode that only watches (a flop counter, selective checkpointing) does not stop the call."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    fn, args = _calls()["norm"]
+    with Watch(), pytest.raises(ValueError, match="HIP device"):
+        fn(*args)

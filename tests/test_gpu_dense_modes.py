@@ -1,5 +1,5 @@
-"""The dense operators' backward passes under forward-mode differentiation, and the calls that remain as
-they were beside it."""
+"""The dense operators' backward passes under forward-mode differentiation and under tracers, and the calls
+that remain as they were beside them."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
@@ -52,3 +52,30 @@ def test_inputs_with_tangents_are_refused():
         with pytest.raises(NotImplementedError, match="forward-mode"):
             rms_norm(fwad.make_dual(x, torch.ones_like(x)))
         assert torch.equal(rms_norm(x), plain)
+
+
+@pytest.mark.parametrize("name", ["norm", "dropout", "gated_ffn"])
+def test_traced_backward_is_refused(name):
+    """A graph recorded before, differentiated while a tracer runs."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    case("traced backward", name)
+    y, leaves = graphs()[name]
+    dy = torch.randn_like(y)
+    for pre in (False, True):
+        with pytest.raises(NotImplementedError, match="trace"):
+            make_fx(lambda g: torch.autograd.grad(y, leaves, g, retain_graph=True), pre_dispatch=pre)(dy)
+    with pytest.raises(RuntimeError):  # torch itself refuses to trace over recorded tensors
+        torch.jit.trace(lambda g: torch.autograd.grad(y, leaves, g, retain_graph=True), (dy,), check_trace=False)
+    assert all(g.isfinite().all() for g in torch.autograd.grad(y, leaves, dy))
+
+
+def test_modes_that_watch():
+    """Under a flop counter and inside a compiled function (whose graph breaks at the call) results stay."""
+    from torch.utils.flop_counter import FlopCounterMode
+    from lazylora_amd.dense import rms_norm
+    case("watching modes")
+    x = torch.randn(4, 16, device="cuda")
+    plain = rms_norm(x)
+    with FlopCounterMode(display=False):
+        assert torch.equal(rms_norm(x), plain)
+    assert torch.equal(torch.compile(lambda t: rms_norm(t) + 1, backend="eager")(x), plain + 1)
