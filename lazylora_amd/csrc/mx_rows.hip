@@ -102,16 +102,32 @@ MX_DEV void team_sum(float (&s)[NS], float* buf)
   }
 }
 
+// HIP takes fewer than 2^32 threads per launch: work past 2^29 of them goes in launches of its own (milliseconds
+// each). launch(first, count) makes one of `count` work-groups from number `first` on.
+constexpr long long kLaunchThreads = 1LL << 29;
+template <typename F>
+hipError_t in_launches(long long groups, int threads, const F& launch)
+{
+  const long long most = kLaunchThreads / threads;
+  for (long long first = 0; first < groups; first += most) {
+    launch(first, (unsigned)std::min(most, groups - first));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 // One team of G lanes per row, the row in registers (V pieces of 8 elements per lane), so x is read once
 // also where the variance needs the mean first.
 template <typename T, int NT, int G, int V>
 __global__ __launch_bounds__(NT) void norm_fwd_kernel(T* __restrict__ y, float* __restrict__ stats,
                                                       const T* __restrict__ x, const float* __restrict__ weight,
-                                                      const float* __restrict__ bias, int M, int D, float eps, int layer)
+                                                      const float* __restrict__ bias, int M, int D, float eps, int layer,
+                                                      long long first)
 {
   __shared__ float buf[2][NT / 64 * 1];
   const int lane = threadIdx.x % G;
-  const long long row = (long long)blockIdx.x * (NT / G) + threadIdx.x / G;
+  const long long row = (first + blockIdx.x) * (NT / G) + threadIdx.x / G;
   const bool live = row < M;
   const int n = live ? D : 0;
   const T* xr = x + row * D;
@@ -166,10 +182,10 @@ template <typename T>
 __global__ __launch_bounds__(1024) void norm_fwd_long_kernel(T* __restrict__ y, float* __restrict__ stats,
                                                              const T* __restrict__ x, const float* __restrict__ weight,
                                                              const float* __restrict__ bias, int M, int D, float eps,
-                                                             int layer)
+                                                             int layer, long long first)
 {
   __shared__ float buf[2][16];
-  const long long row = blockIdx.x;
+  const long long row = first + blockIdx.x;
   const T* xr = x + row * D;
   float mean = 0.f, v[8];
   if (layer) {
@@ -320,10 +336,11 @@ template <typename T>
 __global__ __launch_bounds__(1024) void norm_bwd_long_kernel(T* __restrict__ dx, const T* __restrict__ dy,
                                                              const T* __restrict__ x,
                                                              const float* __restrict__ weight,
-                                                             const float* __restrict__ stats, int M, int D, int layer)
+                                                             const float* __restrict__ stats, int M, int D, int layer,
+                                                             long long first)
 {
   __shared__ float buf[32];
-  const long long row = blockIdx.x;
+  const long long row = first + blockIdx.x;
   const float r = stats[row], mean = layer ? stats[(long long)M + row] : 0.f;
   float s[2] = {0.f, 0.f}, a[8], b[8], w[8];
 #pragma unroll
@@ -403,9 +420,10 @@ hipError_t norm_fwd(void* y, float* stats, const void* x, const float* w, const 
                     int layer, hipStream_t s)
 {
   constexpr int R = NT / G;
-  hipLaunchKernelGGL((norm_fwd_kernel<T, NT, G, V>), dim3((unsigned)((M + R - 1) / R)), dim3(NT), 0, s, (T*)y, stats,
-                     (const T*)x, w, b, M, D, eps, layer);
-  return hipGetLastError();
+  return in_launches((M + R - 1LL) / R, NT, [&](long long first, unsigned count) {
+    hipLaunchKernelGGL((norm_fwd_kernel<T, NT, G, V>), dim3(count), dim3(NT), 0, s, (T*)y, stats, (const T*)x, w, b, M,
+                       D, eps, layer, first);
+  });
 }
 template <typename T>
 hipError_t norm_fwd_any(void* y, float* stats, const void* x, const float* w, const float* b, int M, int D, float eps,
@@ -420,9 +438,10 @@ hipError_t norm_fwd_any(void* y, float* stats, const void* x, const float* w, co
   if (D <= 4096) return norm_fwd<T, 256, 256, 2>(y, stats, x, w, b, M, D, eps, layer, s);
   if (D <= 8192) return norm_fwd<T, 512, 512, 2>(y, stats, x, w, b, M, D, eps, layer, s);
   if (D <= kNormRegisterRow) return norm_fwd<T, 1024, 1024, 2>(y, stats, x, w, b, M, D, eps, layer, s);
-  hipLaunchKernelGGL((norm_fwd_long_kernel<T>), dim3((unsigned)M), dim3(1024), 0, s, (T*)y, stats, (const T*)x, w, b, M,
-                     D, eps, layer);
-  return hipGetLastError();
+  return in_launches(M, 1024, [&](long long first, unsigned count) {
+    hipLaunchKernelGGL((norm_fwd_long_kernel<T>), dim3(count), dim3(1024), 0, s, (T*)y, stats, (const T*)x, w, b, M, D,
+                       eps, layer, first);
+  });
 }
 
 template <typename T, int NT, int G, int V>
@@ -430,7 +449,7 @@ hipError_t norm_bwd(void* dx, float* partial, int& groups, const void* dy, const
                     const float* stats, int M, int D, int layer, int want_w, int want_b, hipStream_t s)
 {
   constexpr int R = NT / G;
-  groups = std::min((M + R - 1) / R, NT == 1024 ? kNormBwdGroups / 2 : kNormBwdGroups);
+  groups = (int)std::min<long long>((M + R - 1LL) / R, NT == 1024 ? kNormBwdGroups / 2 : kNormBwdGroups);
   const auto kernel = layer || want_b ? norm_bwd_kernel<T, NT, G, V, true> : norm_bwd_kernel<T, NT, G, V, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(NT), 0, s, (T*)dx, partial, (const T*)dy, (const T*)x, w,
                      stats, M, D, layer, want_w, want_b);
@@ -457,9 +476,10 @@ hipError_t norm_bwd_any(void* dx, float* dweight, float* dbias, const void* dy, 
   } else if (D <= kNormRegisterRow) {
     e = norm_bwd<T, 1024, 1024, 2>(dx, partial, groups, dy, x, w, stats, M, D, layer, ww, wb, s);
   } else {
-    hipLaunchKernelGGL((norm_bwd_long_kernel<T>), dim3((unsigned)M), dim3(1024), 0, s, (T*)dx, (const T*)dy,
-                       (const T*)x, w, stats, M, D, layer);
-    e = hipGetLastError();
+    e = in_launches(M, 1024, [&](long long first, unsigned count) {
+      hipLaunchKernelGGL((norm_bwd_long_kernel<T>), dim3(count), dim3(1024), 0, s, (T*)dx, (const T*)dy, (const T*)x, w,
+                         stats, M, D, layer, first);
+    });
     if (e == hipSuccess && (ww || wb)) {
       groups = std::min(M, kNormBwdGroups);
       hipLaunchKernelGGL((norm_cols_long_kernel<T>), dim3((unsigned)((D + 255) / 256), (unsigned)groups), dim3(256), 0,
@@ -495,10 +515,11 @@ MX_DEV void philox7(uint32_t (&c)[4], uint32_t k0, uint32_t k1)
 // word is below floor(p 2^32); a dropped element is 0 even where x is NaN or infinite.
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_kernel(T* y, const T* x, long long n, uint64_t threshold, float scale,
-                                                      uint64_t seed, const uint64_t* seed_dev, uint64_t stream)
+                                                      uint64_t seed, const uint64_t* seed_dev, uint64_t stream,
+                                                      long long first)
 {
   if (seed_dev) seed = *seed_dev;
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
+  const long long i = ((first + blockIdx.x) * 256 + threadIdx.x) * 8;
   if (i >= n) return;
   const int left = n - i < 8 ? (int)(n - i) : 8;
   float v[8];
@@ -542,17 +563,15 @@ hipError_t launch_dropout(void* y, const void* x, long long n, uint64_t threshol
                           const uint64_t* seed_dev, uint64_t stream_id, int dtype, hipStream_t s)
 {
   if (n <= 0) return hipSuccess;
-  const dim3 grid((unsigned)((n + 2047) / 2048)), block(256);
-  if (dtype == MXFP4_F32)
-    hipLaunchKernelGGL(dropout_kernel<float>, grid, block, 0, s, (float*)y, (const float*)x, n, threshold, scale, seed,
-                       seed_dev, stream_id);
-  else if (dtype == MXFP4_BF16)
-    hipLaunchKernelGGL(dropout_kernel<__bf16>, grid, block, 0, s, (__bf16*)y, (const __bf16*)x, n, threshold, scale,
-                       seed, seed_dev, stream_id);
-  else
-    hipLaunchKernelGGL(dropout_kernel<_Float16>, grid, block, 0, s, (_Float16*)y, (const _Float16*)x, n, threshold,
-                       scale, seed, seed_dev, stream_id);
-  return hipGetLastError();
+  const auto typed = [&](auto zero) {
+    using T = decltype(zero);
+    return in_launches((n + 2047) / 2048, 256, [&](long long first, unsigned count) {
+      hipLaunchKernelGGL(dropout_kernel<T>, dim3(count), dim3(256), 0, s, (T*)y, (const T*)x, n, threshold, scale, seed,
+                         seed_dev, stream_id, first);
+    });
+  };
+  if (dtype == MXFP4_F32) return typed(0.f);
+  return dtype == MXFP4_BF16 ? typed((__bf16)0.f) : typed((_Float16)0.f);
 }
 
 }  // namespace mx
