@@ -414,8 +414,8 @@ class MXFP4Kernel:
         y = h Wd^T with w_gate, w_up [F, D] and w_down [Do, F] (mxfp4_ffn_forward). gu is the fp32
         gate | up [M, 2F] that ffn_backward takes, or None without save_for_backward."""
         dt, dev = x.dtype, x.device
-        code, kind, (D, F, Do) = _ffn_sizes(dt, dev, w_gate, w_down, act)
         M = x.shape[0] if x.dim() == 2 else -1
+        code, kind, (D, F, Do) = _ffn_sizes(dt, dev, M, w_gate, w_down, act)
         x = _arg(x, "x", (M, D), dt, dev)
         w_gate, w_up = _arg(w_gate, "w_gate", (F, D), dt, dev), _arg(w_up, "w_up", (F, D), dt, dev)
         w_down = _arg(w_down, "w_down", (Do, F), dt, dev)
@@ -444,8 +444,8 @@ class MXFP4Kernel:
         if need_w_down and h is None:
             raise ValueError("need_w_down=True takes the forward's h")
         dt, dev = grad_y.dtype, grad_y.device
-        code, kind, (D, F, Do) = _ffn_sizes(dt, dev, w_gate, w_down, act)
         M = grad_y.shape[0] if grad_y.dim() == 2 else -1
+        code, kind, (D, F, Do) = _ffn_sizes(dt, dev, M, w_gate, w_down, act)
         grad_y = _arg(grad_y, "grad_y", (M, Do), dt, dev)
         w = (_arg(w_gate, "w_gate", (F, D), dt, dev), _arg(w_up, "w_up", (F, D), dt, dev),
              _arg(w_down, "w_down", (Do, F), dt, dev))
@@ -476,6 +476,7 @@ class MXFP4Kernel:
         """(y, stats) of the RMS or layer norm of x [M, D] (float32, bfloat16 or float16) over its last
         axis, weight and bias [D] float32 or None (mxfp4_norm_forward); stats [2, M] float32 is what
         norm_backward takes, or None without save_for_backward."""
+        _check_norm_sizes(x)
         dev, code = x.device, _FLOATS.get(x.dtype)
         if x.dim() != 2 or x.shape[1] == 0 or dev.type != "cuda" or code is None:
             raise ValueError("x must be a float32, bfloat16 or float16 tensor [M, D], D > 0, on the HIP device, got "
@@ -498,6 +499,7 @@ class MXFP4Kernel:
                       need_bias: bool = False):
         """(dx, dweight, dbias) for dL/dy (mxfp4_norm_backward); the column gradients are float32, None
         unless asked for."""
+        _check_norm_sizes(x)
         dt, dev = x.dtype, x.device
         if x.dim() != 2 or x.shape[1] == 0 or dev.type != "cuda" or dt not in _FLOATS:
             raise ValueError("x must be the forward's")
@@ -600,20 +602,29 @@ def _arg(t: torch.Tensor, name: str, shape, dt: torch.dtype, dev: torch.device) 
     return _aligned(t.contiguous())
 
 
-def _ffn_sizes(dt, dev, w_gate, w_down, act):
-    """(dtype code, activation code, (D, F, Do)) of a call of the gated feed-forward block."""
+def _check_norm_sizes(x: torch.Tensor) -> None:
+    """What the C entry points' 32-bit sizes hold (ctypes would wrap larger ones without a word)."""
+    if x.dim() == 2 and (x.shape[0] >= 2 ** 31 or x.shape[1] > 2 ** 20):
+        raise ValueError(f"x has too many rows or columns for the norm: {tuple(x.shape)}")
+
+
+def _ffn_sizes(dt, dev, M, w_gate, w_down, act):
+    """(dtype code, activation code, (D, F, Do)) of a call of the gated feed-forward block on M rows."""
     if dt != torch.bfloat16 and dt != torch.float16:
         raise ValueError(f"the feed-forward block takes bfloat16 or float16, got {dt}")
-    if dev.type != "cuda":
-        raise ValueError(f"the feed-forward block takes tensors on the HIP device, got {dev}")
     if act not in _ACTS:
         raise ValueError(f"unknown activation {act!r}")
     if w_gate.dim() != 2 or w_down.dim() != 2:
         raise ValueError("the weights must be 2-D")
     F, D = w_gate.shape
     Do = w_down.shape[0]
+    if M > 2 ** 24 or max(D, F, Do) > 2 ** 20:
+        raise ValueError("the feed-forward block takes at most 2^24 rows and widths of 2^20, got "
+                         f"{M} rows, D = {D}, F = {F}, Do = {Do}")
     if D % 8 or F % 8 or Do % 8 or not (D and F and Do):
         raise ValueError(f"D = {D}, F = {F} and Do = {Do} must be positive multiples of 8")
+    if dev.type != "cuda":
+        raise ValueError(f"the feed-forward block takes tensors on the HIP device, got {dev}")
     return _FLOATS[dt], _ACTS[act], (D, F, Do)
 
 

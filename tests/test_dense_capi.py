@@ -99,3 +99,26 @@ def test_operators_raise_where_the_library_is_off(monkeypatch):
 def test_autograd_module_is_built():
     from lazylora_amd import _dense_autograd
     assert all(hasattr(_dense_autograd, n) for n in ("norm", "dropout", "gated_ffn"))
+
+
+def test_sizes_past_the_c_types_are_refused(lib):
+    """Sizes that 32 bits would wrap to small ones (the call would compute those rows and leave the rest
+    unwritten); expanded tensors, nothing is allocated. The size is looked at before the device."""
+    import torch
+    from lazylora_amd.native import MXFP4Kernel
+    k = MXFP4Kernel(lib)
+    z = lambda *s: torch.zeros((1,) * len(s), dtype=torch.bfloat16).expand(*s)
+    f32 = lambda *s: torch.zeros((1,) * len(s)).expand(*s)
+    for M, D in ((2 ** 32 + 5, 1), (2 ** 31, 1), (1, 2 ** 32 + 8), (1, 2 ** 20 + 1)):
+        with pytest.raises(ValueError, match="too many rows or columns"):
+            k.norm_forward(z(M, D))
+        with pytest.raises(ValueError, match="too many rows or columns"):
+            k.norm_backward(z(M, D), z(M, D), None, f32(2, M))
+    big = 2 ** 32 + 8
+    for M, D, F, Do in ((2 ** 32 + 4, 8, 8, 8), (2 ** 24 + 1, 8, 8, 8), (2, big, 8, 8), (2, 8, big, 8), (2, 8, 8, big),
+                        (2, 8, 2 ** 20 + 8, 8)):
+        w = (z(F, D), z(F, D), z(Do, F))
+        with pytest.raises(ValueError, match=r"2\^24 rows"):
+            k.ffn_forward(z(M, D), *w)
+        with pytest.raises(ValueError, match=r"2\^24 rows"):
+            k.ffn_backward(z(M, Do), f32(M, 2 * F), *w)
