@@ -37,7 +37,10 @@ FLAGS = [
 
 
 def _run(cmd):
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        res = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as exc:  # no such compiler
+        return 127, str(exc)
     err = "\n".join(l for l in res.stderr.splitlines() if "packed-fp32-ops" not in l and l.strip())
     return res.returncode, err
 
@@ -66,7 +69,9 @@ def _autograd_commands(objdir):
 
 def build(verbose: bool = False) -> str:
     """Compile every source into LIB, and the autograd module over it (always recompiles; the
-    translation units in parallel, objects under _build/). Returns the library path."""
+    translation units in parallel, objects under _build/). Returns the library path. LIB needs hipcc
+    alone and is linked whatever becomes of the module, which needs torch's and Python's headers and a
+    host compiler; RuntimeError, afterwards, if the module could not be built."""
     from concurrent.futures import ThreadPoolExecutor
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
@@ -76,30 +81,40 @@ def build(verbose: bool = False) -> str:
         obj = os.path.join(objdir, os.path.splitext(src)[0] + ".o")
         jobs.append(([HIPCC] + compile_flags + FILE_FLAGS.get(src, []) + ["-c", os.path.join(CSRC, src), "-o", obj],
                      obj))
-    auto_cmd, auto_obj, auto_out, auto_libs = _autograd_commands(objdir)
-    jobs.append((auto_cmd, auto_obj))
+    module, trouble = None, ""
+    try:
+        module = _autograd_commands(objdir)
+    except ImportError as exc:
+        trouble = str(exc)
+    commands = [cmd for cmd, _ in jobs] + ([module[0]] if module else [])
     if verbose:
-        for cmd, _ in jobs:
+        for cmd in commands:
             print(" ".join(cmd), flush=True)
-    with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 1, 16)) as ex:
-        results = list(ex.map(lambda j: _run(j[0]), jobs))
+    with ThreadPoolExecutor(max_workers=min(len(commands), os.cpu_count() or 1, 16)) as ex:
+        results = list(ex.map(_run, commands))
     for (cmd, _), (rc, err) in zip(jobs, results):
         if rc != 0:
-            raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({rc}) on {cmd[-3]}:\n{err}")
+            raise RuntimeError(f"hipcc failed ({rc}) on {cmd[-3]}:\n{err}")
         if verbose and err:
             print(err, file=sys.stderr)
-    tmp = LIB + ".tmp"
-    rc, err = _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC"] + [o for _, o in jobs if o != auto_obj]
-                   + ["-Wl,-soname," + os.path.basename(LIB), "-o", tmp])
+    _link([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC"] + [o for _, o in jobs]
+          + ["-Wl,-soname," + os.path.basename(LIB)], LIB)
+    if module:
+        (cmd, obj, out, libs), (rc, trouble) = module, results[-1]
+        if rc == 0:
+            _link([cmd[0], "-shared", "-fPIC", obj] + libs, out)
+            return LIB
+    raise RuntimeError(f"{os.path.basename(LIB)} is built, but not the autograd module over it ({AUTOGRAD}, the "
+                       f"dense operators' Python entry points):\n{trouble}")
+
+
+def _link(cmd, out):
+    """Link into a file beside `out` and move it there, so that a running process keeps what it has loaded."""
+    tmp = out + ".tmp"
+    rc, err = _run(cmd + ["-o", tmp])
     if rc != 0:
-        raise RuntimeError(f"link failed ({rc}):\n{err}")
-    os.replace(tmp, LIB)
-    tmp = auto_out + ".tmp"
-    rc, err = _run([auto_cmd[0], "-shared", "-fPIC", auto_obj] + auto_libs + ["-o", tmp])
-    if rc != 0:
-        raise RuntimeError(f"link failed ({rc}):\n{err}")
-    os.replace(tmp, auto_out)
-    return LIB
+        raise RuntimeError(f"link of {os.path.basename(out)} failed ({rc}):\n{err}")
+    os.replace(tmp, out)
 
 
 if __name__ == "__main__":
