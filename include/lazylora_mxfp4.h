@@ -269,9 +269,10 @@ int mxfp4_ffn_forward(void *y, void *h, float *gu, const void *x, const void *w_
                       hipStream_t stream);
 
 /* Its backward: with dh = dy Wd (+ grad_h, the gradient that reaches h from elsewhere, [M, F] or NULL),
- * dgu [M, 2F] = dL/dgate | dL/dup of each row (always written; also the gradients of the deltas), and,
- * each unless its pointer is NULL, dx [M, D], dw_gate and dw_up [F, D] (both or neither) and
- * dw_down [Do, F]. h and gu are the forward's. With M = 0 the weight gradients are zero. */
+ * dgu [M, 2F] = dL/dgate | dL/dup of each row (also the gradients of the deltas; NULL only where
+ * neither dx nor dw_gate is asked for), and, each unless its pointer is NULL, dx [M, D], dw_gate and
+ * dw_up [F, D] (both or neither) and dw_down [Do, F]. h and gu are the forward's; what only a product
+ * that is not asked for reads may be NULL. With M = 0 the weight gradients are zero. */
 int mxfp4_ffn_backward(void *dx, void *dw_gate, void *dw_up, void *dw_down, void *dgu, const void *dy,
                        const void *grad_h, const void *x, const void *h, const float *gu,
                        const void *w_gate, const void *w_up, const void *w_down, int dtype, int M, int D,

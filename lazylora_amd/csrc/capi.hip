@@ -1125,14 +1125,16 @@ int mxfp4_ffn_backward(void* dx, void* dw_gate, void* dw_up, void* dw_down, void
   if (workspace_bytes < mxfp4_ffn_workspace_size(M, D, F, Do))
     return fail(MXFP4_EWORKSPACE, "ffn_backward: workspace too small%s");
   if (!dw_gate != !dw_up) return fail(MXFP4_EINVAL, "ffn_backward: dw_gate and dw_up go together%s");
-  if (M > 0 && (!dgu || !dy || !gu || !w_gate || !w_up || !w_down || (dw_gate && !x) || (dw_down && !h)))
+  const bool through = dgu || dx || dw_gate;  // something reads the gradient of gate | up
+  if (M > 0 && (!dy || (dw_gate && !x) || (dw_down && !h) ||
+                (through && (!dgu || !gu || !w_gate || !w_up || !w_down))))
     return fail(MXFP4_EINVAL, "ffn_backward: null pointer%s");
   if (!all_aligned16({dx, dw_gate, dw_up, dw_down, dgu, dy, grad_h, x, h, gu, w_gate, w_up, w_down, workspace}))
     return fail(MXFP4_EINVAL, "ffn_backward: pointers must be 16-byte aligned%s");
   const char* dg = static_cast<const char*>(dgu);
   float* part = static_cast<float*>(workspace);
   mx::DenseArgs a = {};
-  if (M > 0) {
+  if (through && M > 0) {
     a.a[0] = a.a[1] = dy; a.lda = Do;
     a.b[0] = a.b[1] = w_down; a.ldb = F;
     a.M = M; a.N = F; a.K = Do; a.nseg = 1;

@@ -307,23 +307,26 @@ struct Ffn : torch::autograd::Function<Ffn> {
     auto shape = ctx->saved_data["lead"].toIntVector();
     Tensor dx;
     if (ctx->needs_input_grad(0)) dx = at::empty(shape, wg.options());
-    const bool need_in = x.defined();
+    const bool has_gd = ctx->saved_data["gate_delta"].toBool(), has_ud = ctx->saved_data["up_delta"].toBool();
+    const bool need_gd = has_gd && ctx->needs_input_grad(4), need_ud = has_ud && ctx->needs_input_grad(has_gd ? 5 : 4);
+    // this backward's own needs: it may be for some of the leaves that the forward saw
+    const bool need_in = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     const Tensor dwg = need_in ? at::empty_like(wg) : Tensor(), dwu = need_in ? at::empty_like(wu) : Tensor();
-    const Tensor dwd = h.defined() ? at::empty_like(wd) : Tensor();
+    const Tensor dwd = ctx->needs_input_grad(3) ? at::empty_like(wd) : Tensor();
+    Tensor dgu;
     shape.back() = 2LL * F;
-    const Tensor dgu = at::empty(shape, wg.options());
+    if (dx.defined() || need_in || need_gd || need_ud) dgu = at::empty(shape, wg.options());
     size_t n;
     const Tensor ws = ffn_workspace(M, D, F, Do, wg, n);
-    check(mxfp4_ffn_backward(ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), dgu.data_ptr(), gy.data_ptr(), ptr(gh), ptr(x), ptr(h),
+    check(mxfp4_ffn_backward(ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), ptr(dgu), gy.data_ptr(), ptr(gh), ptr(x), ptr(h),
                              fptr(gu), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), dtype_code(wg), M, D, F, Do,
                              (int)ctx->saved_data["act"].toInt(), ptr(ws), n, stream_of(wg)));
     out[0] = dx;
     if (ctx->needs_input_grad(1)) out[1] = dwg;
     if (ctx->needs_input_grad(2)) out[2] = dwu;
     out[3] = dwd;
-    const bool has_gd = ctx->saved_data["gate_delta"].toBool(), has_ud = ctx->saved_data["up_delta"].toBool();
-    if (has_gd && ctx->needs_input_grad(4)) out[4] = dgu.narrow(-1, 0, F);
-    if (has_ud && ctx->needs_input_grad(has_gd ? 5 : 4)) out[5] = dgu.narrow(-1, F, F);
+    if (need_gd) out[4] = dgu.narrow(-1, 0, F);
+    if (need_ud) out[5] = dgu.narrow(-1, F, F);
     return once(std::move(out));
   }
 };

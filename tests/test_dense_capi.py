@@ -122,3 +122,15 @@ def test_sizes_past_the_c_types_are_refused(lib):
             k.ffn_forward(z(M, D), *w)
         with pytest.raises(ValueError, match=r"2\^24 rows"):
             k.ffn_backward(z(M, Do), f32(M, 2 * F), *w)
+
+
+def test_ffn_backward_without_the_gate_and_up_gradient(lib):
+    """dgu may be NULL only where neither dx nor dw_gate is asked for; then what its product reads may be too."""
+    unread = dict.fromkeys(("dx", "dwg", "dwu", "dgu", "gu", "wg", "wu", "wd", "x"))
+    for name in ("dy", "h"):
+        assert ffn_bwd(lib, {**unread, name: None}) == -1
+        assert b"null" in lib.mxfp4_last_error()
+    assert ffn_bwd(lib, {**unread, "dx": P}) == -1
+    assert ffn_bwd(lib, {**unread, "dwg": P, "dwu": P, "x": P}) == -1
+    assert ffn_bwd(lib, {**unread, "dgu": P}) == -1
+    assert ffn_bwd(lib, {**unread, "dwd": None}) == 0  # nothing asked for: nothing to do

@@ -152,3 +152,35 @@ def test_offsets_past_32_bits(k):
     want = reference(last, "situ", True)
     for name, got in (("y", y), ("h", h), ("dg", dgu[:, :1024]), ("du", dgu[:, 1024:]), ("dx", dx)):
         check(name, got[-300:], want[name])
+
+
+def test_gradients_not_asked_for_are_not_made(k):
+    """A backward for some of the leaves allocates no gradient of the others: dx of a trainable block no weight
+    gradients, a down weight alone no gradient of gate | up. What is asked for is what the whole backward gives."""
+    from lazylora_amd.dense import gated_ffn
+    case("gradients asked for")
+
+    def peak(t, names):
+        y = gated_ffn(t["x"], t["wg"], t["wu"], t["wd"])
+        whole = torch.autograd.grad(y, [t[n] for n in ("x", "wg", "wu", "wd")], t["dy"], retain_graph=True)
+        whole = dict(zip(("x", "wg", "wu", "wd"), whole))
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = torch.autograd.grad(y, [t[n] for n in names], t["dy"])
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, whole[n]) for g, n in zip(got, names)), names
+        return torch.cuda.max_memory_allocated() - before
+
+    def leaves(*sizes):
+        t = inputs(12, *sizes, torch.bfloat16, deltas=False)
+        for n in ("x", "wg", "wu", "wd"):
+            t[n].requires_grad_(True)
+        return t
+
+    # 8 rows: dx and the split sums are small, a weight gradient 16 MiB
+    t = leaves(8, 2048, 4096, 2048)
+    assert peak(t, ["x"]) < 2 ** 24
+    assert 2 ** 24 <= peak(t, ["x", "wd"]) < 2 ** 25
+    # 4096 rows: gate | up's gradient is 32 MiB, the down weight's 1/4 MiB
+    assert peak(leaves(4096, 64, 2048, 64), ["wd"]) < 2 ** 25
