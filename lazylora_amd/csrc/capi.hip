@@ -589,6 +589,44 @@ int scratch_on_current_device(uint8_t** out)
   return MXFP4_OK;
 }
 
+// Argument checks of the dense operators. Not inside extern "C": there even an unnamed namespace's functions
+// get C names, and the library exports them.
+constexpr int kDenseMaxWidth = 1 << 20, kDenseMaxRows = 1 << 24;
+
+int check_ffn(const char* who, int dtype, int M, int D, int F, int Do, int act_kind)
+{
+  static thread_local char msg[160];
+  const auto bad = [&](const char* what) {
+    snprintf(msg, sizeof(msg), "%s: %s", who, what);
+    return fail(MXFP4_EINVAL, "%s", msg);
+  };
+  if (dtype != MXFP4_BF16 && dtype != MXFP4_F16) return bad("dtype must be MXFP4_BF16 or MXFP4_F16");
+  if (act_kind != MXFP4_ACT_SWIGLU && act_kind != MXFP4_ACT_SITU) return bad("unknown activation");
+  if (M < 0 || M > kDenseMaxRows) return bad("M must lie in [0, 2^24]");
+  for (int v : {D, F, Do})
+    if (v <= 0 || v > kDenseMaxWidth || v % 8) return bad("D, F and Do must be multiples of 8 in [8, 2^20]");
+  return MXFP4_OK;
+}
+bool all_aligned16(std::initializer_list<const void*> ps)
+{
+  for (const void* p : ps)
+    if (!aligned16(p)) return false;
+  return true;
+}
+
+int check_rows(const char* who, int M, int D, int kind, int dtype)
+{
+  static thread_local char msg[160];
+  const auto bad = [&](const char* what) {
+    snprintf(msg, sizeof(msg), "%s: %s", who, what);
+    return fail(MXFP4_EINVAL, "%s", msg);
+  };
+  if (dtype != MXFP4_F32 && dtype != MXFP4_BF16 && dtype != MXFP4_F16) return bad("dtype must be F32, BF16 or F16");
+  if (kind != MXFP4_NORM_RMS && kind != MXFP4_NORM_LAYER) return bad("unknown norm");
+  if (M < 0 || D < 1 || D > kDenseMaxWidth) return bad("need M >= 0 and D in [1, 2^20]");
+  return MXFP4_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1047,33 +1085,6 @@ int mxfp4_router_topk_backward(float* grad_logits, const int64_t* topk_idx, cons
 }
 
 // ---------------------------------------------------------------- dense operators
-namespace {
-
-constexpr int kDenseMaxWidth = 1 << 20, kDenseMaxRows = 1 << 24;
-
-int check_ffn(const char* who, int dtype, int M, int D, int F, int Do, int act_kind)
-{
-  static thread_local char msg[160];
-  const auto bad = [&](const char* what) {
-    snprintf(msg, sizeof(msg), "%s: %s", who, what);
-    return fail(MXFP4_EINVAL, "%s", msg);
-  };
-  if (dtype != MXFP4_BF16 && dtype != MXFP4_F16) return bad("dtype must be MXFP4_BF16 or MXFP4_F16");
-  if (act_kind != MXFP4_ACT_SWIGLU && act_kind != MXFP4_ACT_SITU) return bad("unknown activation");
-  if (M < 0 || M > kDenseMaxRows) return bad("M must lie in [0, 2^24]");
-  for (int v : {D, F, Do})
-    if (v <= 0 || v > kDenseMaxWidth || v % 8) return bad("D, F and Do must be multiples of 8 in [8, 2^20]");
-  return MXFP4_OK;
-}
-bool all_aligned16(std::initializer_list<const void*> ps)
-{
-  for (const void* p : ps)
-    if (!aligned16(p)) return false;
-  return true;
-}
-
-}  // namespace
-
 size_t mxfp4_ffn_workspace_size(int M, int D, int F, int Do)
 {
   if (M <= 0 || D <= 0 || F <= 0 || Do <= 0) return 0;
@@ -1166,19 +1177,6 @@ int mxfp4_ffn_backward(void* dx, void* dw_gate, void* dw_up, void* dw_down, void
     a.out = dw_down; a.ldo = F; a.split_m = Do;
     MX_TRY(mx::launch_dense(mx::kDenseWgrad, mx::kDenseStore, a, dtype, part, stream), "ffn_backward: down weight");
   }
-  return MXFP4_OK;
-}
-
-static int check_rows(const char* who, int M, int D, int kind, int dtype)
-{
-  static thread_local char msg[160];
-  const auto bad = [&](const char* what) {
-    snprintf(msg, sizeof(msg), "%s: %s", who, what);
-    return fail(MXFP4_EINVAL, "%s", msg);
-  };
-  if (dtype != MXFP4_F32 && dtype != MXFP4_BF16 && dtype != MXFP4_F16) return bad("dtype must be F32, BF16 or F16");
-  if (kind != MXFP4_NORM_RMS && kind != MXFP4_NORM_LAYER) return bad("unknown norm");
-  if (M < 0 || D < 1 || D > kDenseMaxWidth) return bad("need M >= 0 and D in [1, 2^20]");
   return MXFP4_OK;
 }
 

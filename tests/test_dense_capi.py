@@ -134,3 +134,14 @@ def test_ffn_backward_without_the_gate_and_up_gradient(lib):
     assert ffn_bwd(lib, {**unread, "dwg": P, "dwu": P, "x": P}) == -1
     assert ffn_bwd(lib, {**unread, "dgu": P}) == -1
     assert ffn_bwd(lib, {**unread, "dwd": None}) == 0  # nothing asked for: nothing to do
+
+
+def test_only_the_entry_points_have_c_names(lib):
+    """Any other C name that the library exports could meet a host program's function of that name."""
+    import re
+    import subprocess
+    from lazylora_amd import native
+    out = subprocess.run(["nm", "-D", "--defined-only", native.LIB_PATH], capture_output=True, text=True, check=True)
+    names = [l.split()[-1] for l in out.stdout.splitlines() if " T " in l]
+    assert "mxfp4_gemm" in names
+    assert [n for n in names if not n.startswith(("mxfp4_", "_Z", "_init", "_fini"))] == []
