@@ -268,6 +268,13 @@ int mxfp4_ffn_forward(void *y, void *h, float *gu, const void *x, const void *w_
                       int D, int F, int Do, int act_kind, void *workspace, size_t workspace_bytes,
                       hipStream_t stream);
 
+/* Which kernels a call of these sizes runs, for diagnosis and tests. product: 0 gate/up, 1 down, 2 gradient
+ * of gate/up, 3 dx, 4 gate/up weight gradients, 5 down weight gradient. plan[0..2]: rows of the result, tile
+ * and runs of K of its first launch, plan[3..5] the same of the rows behind them (0 rows: there are none).
+ * tile: 0 256 x 256, 1 128 x 256, 2 128 x 128, 3 64 x 128 (gate/up: half as many columns of h), -1 and -2
+ * the few-row kernel with 16 and 32 weight rows. */
+int mxfp4_ffn_plan(int product, int M, int D, int F, int Do, int *plan);
+
 /* Its backward: with dh = dy Wd (+ grad_h, the gradient that reaches h from elsewhere, [M, F] or NULL),
  * dgu [M, 2F] = dL/dgate | dL/dup of each row (also the gradients of the deltas; NULL only where
  * neither dx nor dw_gate is asked for), and, each unless its pointer is NULL, dx [M, D], dw_gate and

@@ -4,6 +4,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <array>
 #include <mutex>
 #include <type_traits>
 
@@ -607,6 +608,21 @@ int check_ffn(const char* who, int dtype, int M, int D, int F, int Do, int act_k
     if (v <= 0 || v > kDenseMaxWidth || v % 8) return bad("D, F and Do must be multiples of 8 in [8, 2^20]");
   return MXFP4_OK;
 }
+// The six products of the block, in the order in which a step runs them.
+struct FfnProduct {
+  mx::DenseShape shape;
+  mx::DenseEpi epi;
+  int M, N, K, nseg;
+};
+std::array<FfnProduct, 6> ffn_products(int M, int D, int F, int Do)
+{
+  return {{{mx::kDenseForward, mx::kDenseGlu, M, F, D, 1},
+           {mx::kDenseForward, mx::kDenseStore, M, Do, F, 1},
+           {mx::kDenseDgrad, mx::kDenseDGlu, M, F, Do, 1},
+           {mx::kDenseDgrad, mx::kDenseStore, M, D, F, 2},
+           {mx::kDenseWgrad, mx::kDenseStore, 2 * F, D, M, 1},
+           {mx::kDenseWgrad, mx::kDenseStore, Do, F, M, 1}}};
+}
 bool all_aligned16(std::initializer_list<const void*> ps)
 {
   for (const void* p : ps)
@@ -1088,13 +1104,20 @@ int mxfp4_router_topk_backward(float* grad_logits, const int64_t* topk_idx, cons
 size_t mxfp4_ffn_workspace_size(int M, int D, int F, int Do)
 {
   if (M <= 0 || D <= 0 || F <= 0 || Do <= 0) return 0;
-  // the products of a call run one after another and share the bytes
-  return std::max({mx::dense_partial_bytes(mx::kDenseForward, mx::kDenseGlu, M, F, D, 1),
-                   mx::dense_partial_bytes(mx::kDenseForward, mx::kDenseStore, M, Do, F, 1),
-                   mx::dense_partial_bytes(mx::kDenseDgrad, mx::kDenseDGlu, M, F, Do, 1),
-                   mx::dense_partial_bytes(mx::kDenseDgrad, mx::kDenseStore, M, D, F, 2),
-                   mx::dense_partial_bytes(mx::kDenseWgrad, mx::kDenseStore, 2 * F, D, M, 1),
-                   mx::dense_partial_bytes(mx::kDenseWgrad, mx::kDenseStore, Do, F, M, 1)});
+  size_t bytes = 0;  // the products of a call run one after another and share them
+  for (const FfnProduct& p : ffn_products(M, D, F, Do))
+    bytes = std::max(bytes, mx::dense_partial_bytes(p.shape, p.epi, p.M, p.N, p.K, p.nseg));
+  return bytes;
+}
+
+int mxfp4_ffn_plan(int product, int M, int D, int F, int Do, int* plan)
+{
+  const int rc = check_ffn("ffn_plan", MXFP4_BF16, M, D, F, Do, MXFP4_ACT_SWIGLU);
+  if (rc != MXFP4_OK) return rc;
+  if (product < 0 || product > 5 || !plan) return fail(MXFP4_EINVAL, "ffn_plan: product must lie in [0, 5]%s");
+  const FfnProduct p = ffn_products(M, D, F, Do)[product];
+  mx::dense_choice(p.shape, p.epi, p.M, p.N, p.K, p.nseg, plan);
+  return MXFP4_OK;
 }
 
 int mxfp4_ffn_forward(void* y, void* h, float* gu, const void* x, const void* w_gate, const void* w_up,

@@ -45,6 +45,9 @@ enum DenseShape : int { kDenseForward = 0, kDenseDgrad = 1, kDenseWgrad = 2 };
 // Bytes of partial sums that launch_dense may use for a product of these sizes, and the product
 // (dtype MXFP4_BF16 or MXFP4_F16; partial: that many bytes).
 size_t dense_partial_bytes(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg);
+// What launch_dense chooses for a product: rows, tile and runs of K of its first part and of its second (0 rows:
+// one part). tile: 0 .. 3 from the largest to the smallest, -1 and -2 the few-row kernel (mx_dense.hip).
+void dense_choice(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg, int* choice);
 hipError_t launch_dense(DenseShape shape, DenseEpi epi, const DenseArgs& a, int dtype, float* partial, hipStream_t s);
 
 // Layer / RMS norm over rows of D elements (dtype MXFP4_F32, _BF16 or _F16), fp32 statistics

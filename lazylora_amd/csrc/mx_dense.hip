@@ -763,6 +763,23 @@ size_t dense_partial_bytes(DenseShape shape, DenseEpi epi, int M, int N, int K, 
   return std::max(plan_bytes(cut.first, epi, cut.rows, N), plan_bytes(cut.rest, epi, M - cut.rows, N));
 }
 
+void dense_choice(DenseShape shape, DenseEpi epi, int M, int N, int K, int nseg, int* choice)
+{
+  std::fill_n(choice, 6, 0);
+  if (M <= 0 || N <= 0) return;
+  const Cut cut = cut_dense(shape, epi, M, N, K, nseg);
+  const Plan* part = &cut.first;
+  for (int rows : {cut.rows, M - cut.rows}) {
+    if (rows > 0) {
+      choice[0] = rows;
+      choice[1] = part->tile;
+      choice[2] = part->splits;
+    }
+    choice += 3;
+    part = &cut.rest;
+  }
+}
+
 hipError_t launch_dense(DenseShape shape, DenseEpi epi, const DenseArgs& a, int dtype, float* partial, hipStream_t s)
 {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;

@@ -110,6 +110,8 @@ def _load_library() -> ctypes.CDLL:
     cll, cu64 = ctypes.c_longlong, ctypes.c_uint64
     lib.mxfp4_ffn_workspace_size.restype = sz
     lib.mxfp4_ffn_workspace_size.argtypes = [ci, ci, ci, ci]
+    lib.mxfp4_ffn_plan.restype = ci
+    lib.mxfp4_ffn_plan.argtypes = [ci] * 5 + [ctypes.POINTER(ci)]
     lib.mxfp4_ffn_forward.restype = ci
     lib.mxfp4_ffn_forward.argtypes = [vp] * 9 + [ci] * 6 + [vp, sz, vp]
     lib.mxfp4_ffn_backward.restype = ci
