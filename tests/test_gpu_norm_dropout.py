@@ -287,3 +287,34 @@ def test_norm_and_dropout_on_a_side_stream_and_captured(k):
         torch.cuda.synchronize()
         want = step()
         assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+# rows enough that every work-group of the backward takes several, a last pass of fewer rows than teams among
+# them: more than 16384 rows up to width 128, 4096 up to 512, 1024 up to 2048, 512 up to 4096, 256 above
+MANY_ROWS = [(16400, 64), (33000, 127), (4101, 300), (8200, 512), (1030, 2048), (3001, 1000), (1000, 3584), (1600, 2049),
+             (600, 4100), (700, 8192), (260, 8200), (515, 16384), (520, 16400), (1100, 16385)]
+
+
+@pytest.mark.parametrize("M,D", MANY_ROWS)
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("layer", [0, 1])
+def test_norm_many_rows(k, M, D, dt, layer):
+    case("norm, many rows", M, D, dt, "layer" if layer else "rms")
+    g = torch.Generator(device="cuda").manual_seed(M + D)
+    x = (torch.randn(M, D, device="cuda", generator=g) * 2 + 0.5).to(dt)
+    w = 1 + 0.2 * torch.randn(D, device="cuda", generator=g)
+    b = 0.3 * torch.randn(D, device="cuda", generator=g) if layer else None
+    dy = torch.randn(M, D, device="cuda", generator=g).to(dt)
+    (y, ey), (dx, edx), (dw, edw), (db, edb) = norm_reference(x, w, b, dy, layer, 1e-5)
+    got, stats = k.norm_forward(x, w, b, 1e-5, layer, save_for_backward=True)
+    check("y", got, y, ey)
+    gx, gw, gb = k.norm_backward(dy, x, w, stats, layer, need_weight=True, need_bias=True)
+    check("dx", gx, dx, edx)
+    check("dw", gw, dw, edw)
+    check("db", gb, db, edb)
+    gx2, gw2, none = k.norm_backward(dy, x, w, stats, layer, need_weight=True)
+    assert none is None and torch.equal(gx, gx2) and torch.equal(gw, gw2)
+    plain, none, _ = k.norm_backward(dy, x, None, stats, layer)  # no weight, no column sums
+    (_, _), (dx1, edx1), _, _ = norm_reference(x, None, b, dy, layer, 1e-5)
+    check("dx without a weight", plain, dx1, edx1)
+    assert none is None
