@@ -38,10 +38,13 @@ void check(int rc)
 
 hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
-// t, contiguous and 16-byte aligned (a copy where it is not).
+// t with its values as they lie in memory: contiguous, and no view that stands for its negative (the imaginary part
+// of a conjugate; one of a single element is contiguous).
+Tensor laid_out(const Tensor& t) { return t.resolve_neg().contiguous(); }
+// The same and 16-byte aligned (a copy where it is not).
 Tensor tidy(const Tensor& t)
 {
-  Tensor c = t.contiguous();
+  Tensor c = laid_out(t);
   return reinterpret_cast<uintptr_t>(c.data_ptr()) & 15 ? c.clone() : c;
 }
 Tensor arg(const Tensor& t, const char* name, at::IntArrayRef shape, const Tensor& like, at::ScalarType dtype)
@@ -115,7 +118,7 @@ Tensor vector_arg(const Tensor& t, const char* name, const NormSizes& n, const T
   TORCH_CHECK_VALUE(t.is_floating_point() && t.dim() == 1 && t.size(0) == n.D && t.device() == x.device(), name,
                     " must be a floating tensor [", n.D, "] on ", x.device(), ", got ", t.scalar_type(), " ", t.sizes(),
                     " on ", t.device());
-  return t.to(at::kFloat).contiguous();
+  return laid_out(t.to(at::kFloat));
 }
 Tensor norm_run(const Tensor& x, const Tensor& w, const Tensor& b, double eps, int64_t kind, const NormSizes& n,
                 Tensor* stats)
@@ -135,7 +138,7 @@ struct Norm : torch::autograd::Function<Norm> {
   {
     const NormSizes n = norm_sizes(x);
     const Tensor w = vector_arg(given(weight), "weight", n, x), b = vector_arg(given(bias), "bias", n, x);
-    const Tensor xc = x.contiguous();
+    const Tensor xc = laid_out(x);
     Tensor stats;
     const Tensor y = norm_run(xc, w, b, eps, kind, n, &stats);
     ctx->save_for_backward({xc, w, stats});
@@ -154,7 +157,7 @@ struct Norm : torch::autograd::Function<Norm> {
     const int64_t wtype = ctx->saved_data["wtype"].toInt(), btype = ctx->saved_data["btype"].toInt();
     const bool has_w = wtype >= 0, has_b = btype >= 0;  // the inputs are numbered without the absent ones
     const bool need_w = has_w && ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(has_w ? 2 : 1);
-    const Tensor gy = grads[0].contiguous();
+    const Tensor gy = laid_out(grads[0]);
     Tensor dx = at::empty_like(x), dw, db, ws;
     if (need_w) dw = at::empty({n.D}, stats.options());
     if (need_b) db = at::empty({n.D}, stats.options());
@@ -174,14 +177,14 @@ Tensor norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, dou
   check_modes({x, w, b});
   if (records({x, w, b})) return Norm::apply(x, weight, bias, eps, kind);
   const NormSizes n = norm_sizes(x);
-  return norm_run(x.contiguous(), vector_arg(w, "weight", n, x), vector_arg(b, "bias", n, x), eps, kind, n, nullptr);
+  return norm_run(laid_out(x), vector_arg(w, "weight", n, x), vector_arg(b, "bias", n, x), eps, kind, n, nullptr);
 }
 
 // ---------------------------------------------------------------- dropout
 Tensor dropout_run(const Tensor& t, double p, uint64_t seed, const Tensor& seed_dev, uint64_t stream)
 {
   const c10::DeviceGuard guard(t.device());
-  const Tensor x = t.contiguous();
+  const Tensor x = laid_out(t);
   Tensor y = at::empty_like(x);
   if (x.numel())
     check(mxfp4_dropout(y.data_ptr(), x.data_ptr(), x.numel(), p, seed, static_cast<const uint64_t*>(ptr(seed_dev)),

@@ -488,7 +488,7 @@ class MXFP4Kernel:
             weight = _arg(weight, "weight", (D,), torch.float32, dev)
         if bias is not None:
             bias = _arg(bias, "bias", (D,), torch.float32, dev)
-        x = x.contiguous()
+        x = x.resolve_neg().contiguous()
         y = torch.empty_like(x)
         stats = torch.empty((2, M), dtype=torch.float32, device=dev) if save_for_backward else None
         if M:
@@ -511,7 +511,7 @@ class MXFP4Kernel:
         stats = _arg(stats, "stats", (2, M), torch.float32, dev)
         if weight is not None:
             weight = _arg(weight, "weight", (D,), torch.float32, dev)
-        x, grad_y = x.contiguous(), grad_y.contiguous()
+        x, grad_y = x.resolve_neg().contiguous(), grad_y.resolve_neg().contiguous()
         dx = torch.empty_like(x)
         dw = torch.empty(D, dtype=torch.float32, device=dev) if need_weight else None
         db = torch.empty(D, dtype=torch.float32, device=dev) if need_bias else None
@@ -537,7 +537,7 @@ class MXFP4Kernel:
                 raise ValueError("a seed tensor must hold one int64 on x's device")
         elif not 0 <= seed < 2 ** 64:
             raise ValueError(f"seed must lie in [0, 2^64), got {seed}")
-        x = x.contiguous()
+        x = x.resolve_neg().contiguous()
         y = torch.empty_like(x)
         number, where = (0, seed.data_ptr()) if isinstance(seed, torch.Tensor) else (seed, None)
         self._launch(x.device, self.lib.mxfp4_dropout, y.data_ptr(), x.data_ptr(), x.numel(), p, number, where, stream,
@@ -601,7 +601,7 @@ def _arg(t: torch.Tensor, name: str, shape, dt: torch.dtype, dev: torch.device) 
     """t, contiguous and 16-byte aligned (a copy where it is not), of this shape and type on dev."""
     if t.shape != shape or t.dtype != dt or t.device != dev:
         raise ValueError(f"{name} must be {dt} {list(shape)} on {dev}, got {t.dtype} {list(t.shape)} on {t.device}")
-    return _aligned(t.contiguous())
+    return _aligned(t.resolve_neg().contiguous())
 
 
 def _check_norm_sizes(x: torch.Tensor) -> None:

@@ -184,3 +184,51 @@ def test_gradients_not_asked_for_are_not_made(k):
     assert 2 ** 24 <= peak(t, ["x", "wd"]) < 2 ** 25
     # 4096 rows: gate | up's gradient is 32 MiB, the down weight's 1/4 MiB
     assert peak(leaves(4096, 64, 2048, 64), ["wd"]) < 2 ** 25
+
+
+def test_one_optional_input_alone(k):
+    """A bias without a weight, an up delta without a gate delta: each gradient goes to its own input."""
+    from lazylora_amd.dense import gated_ffn, layer_norm
+    case("optional inputs")
+    x, dy = torch.randn(6, 40, device="cuda"), torch.randn(6, 40, device="cuda")
+    bias = torch.randn(40, device="cuda", requires_grad=True)
+    for lead in (x, x.clone().requires_grad_(True)):
+        y = layer_norm(lead, None, bias)
+        (gb,) = torch.autograd.grad(y, (bias,), dy, retain_graph=True)
+        assert ((gb.double() - dy.double().sum(0)).abs() <= 8 * 2.0 ** -24 * dy.double().abs().sum(0)).all()
+        assert torch.equal(y.detach(), layer_norm(x, torch.ones(40, device="cuda"), bias.detach()))
+    t = inputs(13, 20, 72, 40, 48, torch.bfloat16)
+    t["ud"].requires_grad_(True)
+    want = reference({**{n: v.detach() for n, v in t.items()}, "gd": None}, "situ", False)
+    y = gated_ffn(t["x"], t["wg"], t["wu"], t["wd"], "situ", None, t["ud"])
+    check("y", y.detach(), want["y"])
+    (gu,) = torch.autograd.grad(y, (t["ud"],), t["dy"])
+    check("du", gu, want["du"])
+
+
+def test_negative_views(k):
+    """The imaginary part of a conjugate is a view that stands for its negative: read with its sign, of inputs,
+    weights and upstream gradients (of one element such a view is contiguous and is not copied first)."""
+    from lazylora_amd.dense import dropout, layer_norm, rms_norm
+    case("negative views")
+    z = lambda *s: torch.randn(*s, dtype=torch.cfloat, device="cuda").conj().imag
+    for shape in ((1, 1), (1,), (3, 8)):
+        x, plain = z(*shape), None
+        plain = x.resolve_neg().clone()
+        assert x.is_neg() and not plain.is_neg()
+        w = z(shape[-1])
+        wp = w.resolve_neg().clone()
+        assert torch.equal(dropout(x, 0.0, 1), plain)
+        assert torch.equal(k.dropout(x, 0.0, 1), plain)
+        assert torch.equal(rms_norm(x, w), rms_norm(plain, wp))
+        assert torch.equal(layer_norm(x, w, w), layer_norm(plain, wp, wp))
+        leaf = torch.randn(*shape, device="cuda", requires_grad=True)
+        for fn in (lambda v: dropout(v, 0.0, 1), lambda v: rms_norm(v, w, 0.1)):
+            (got,) = torch.autograd.grad(fn(leaf), (leaf,), x)
+            (want,) = torch.autograd.grad(fn(leaf), (leaf,), plain)
+            assert torch.equal(got, want)
+        if len(shape) == 2:
+            y, st = k.norm_forward(x, w.resolve_neg(), None, 0.1, 0, True)
+            assert torch.equal(y, rms_norm(plain, wp, 0.1))
+            assert torch.equal(k.norm_backward(x, plain, wp, st)[0], k.norm_backward(plain, plain, wp, st)[0])
+            assert torch.equal(k.norm_backward(plain, x, w, st)[0], k.norm_backward(plain, plain, wp, st)[0])
