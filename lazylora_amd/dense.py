@@ -61,7 +61,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis, var the mean square distance
-    from the mean. x float32, bfloat16 or float16; weight and bias [D] of any floating type, or None.
+    from the mean. x float32, bfloat16 or float16; weight and bias [D] of any floating type (float64 too is
+    taken as float32), or None.
     Differentiable in all three."""
     return _module().norm(x, weight, bias, eps, NORM_LAYER)
 
