@@ -314,6 +314,59 @@ int mxfp4_norm_backward(void *dx, float *dweight, float *dbias, const void *dy, 
 int mxfp4_dropout(void *y, const void *x, long long n, double p, uint64_t seed,
                   const uint64_t *seed_device, uint64_t stream_id, int dtype, hipStream_t stream);
 
+/* ---- expert selection with groups -----------------------------------------------------------
+ * mxfp4_router_topk's step for routers of other forms:
+ *   s = sigmoid(logits) or softmax(logits) over the E experts; c = s + bias (bias may be NULL);
+ *   of num_groups equal runs of experts the topk_groups with the largest group score stay (1 <= topk_groups <=
+ *   num_groups; MXFP4_GROUP_TOP2: the sum of the group's two largest c, or its one c; MXFP4_GROUP_MAX: its
+ *   largest); topk_idx[t, :] = the top_k largest c of those, descending; topk_w[t, j] = s[t, topk_idx[t, j]],
+ *   divided by (their sum + 1e-20) when renormalize != 0 and top_k > 1, then times routed_scaling_factor.
+ * The order is that of exact arithmetic on the given logits and bias (without a bias that of the logits), not
+ * that of rounded scores; equal values and equal groups go to the lower number, NaN comes before every
+ * number. A softmax row of nothing but -inf has scores 0; one with +inf has scores NaN.
+ * logits [N, E] of MXFP4_F32, _BF16 or _F16, bias [E] fp32. E <= 4096, num_groups <= 64 and a divisor of E,
+ * top_k <= min(64, topk_groups E / num_groups); where num_groups is no power of two, E / num_groups at most
+ * 64 times 64 / (the next power of two). */
+#define MXFP4_SCORE_SIGMOID 0
+#define MXFP4_SCORE_SOFTMAX 1
+#define MXFP4_GROUP_TOP2 0
+#define MXFP4_GROUP_MAX 1
+int mxfp4_select_topk(int64_t *topk_idx, float *topk_w, const void *logits, int dtype, const float *bias,
+                      int N, int E, int top_k, int scoring, int num_groups, int topk_groups,
+                      int group_score, float routed_scaling_factor, int renormalize, hipStream_t stream);
+/* The gradient of its weights with respect to the logits: grad_logits [N, E] of the logits' dtype, fully
+ * written. topk_idx as the forward wrote it (distinct experts per token; ids outside [0, E) are left out),
+ * grad_w [N, top_k] fp32. The choice itself has no gradient and neither has the bias. */
+int mxfp4_select_topk_backward(void *grad_logits, const int64_t *topk_idx, const float *grad_w,
+                               const void *logits, int dtype, int N, int E, int top_k, int scoring,
+                               float routed_scaling_factor, int renormalize, hipStream_t stream);
+
+/* ---- 4-bit integer weights with group scales ------------------------------------------------
+ * W [R, K]: packed [R, K / 2] bytes (low nibble = even element), scales [R, K / group] of the activations'
+ * dtype (MXFP4_BF16 or _F16), zeros [R, K / group] bytes or NULL (8 everywhere);
+ *   W[r, k] = scales[r, k / group] * (code[r, k] - zeros[r, k / group]).
+ * group 32, 64 or 128, K a multiple of it; K and R at most 2^20. packed, x and y 16-byte aligned. Codes enter
+ * the products exactly, sums are fp32 and every result is rounded once (an infinity in a row of x gives NaN).
+ * No atomics on values: results do not depend on timing.
+ *
+ * y [M, R] = x [M, K] . W^T, M at most 2^24. */
+int mxfp4_int4_gemm(void *y, const void *x, const uint8_t *packed, const void *scales,
+                    const uint8_t *zeros, int dtype, int M, int K, int R, int group, hipStream_t stream);
+
+/* The routed expert layer over such weights:
+ *   out[t] = sum over slots of topk_w[t, j] W2_e . GLU(W1_e . h[t], W3_e . h[t]), e = topk_idx[t, j],
+ * h and out [N, D] of dtype, the GLU's results rounded to dtype in between. codes, scales and zeros: host
+ * arrays of 3 device pointers, W1 and W3 [E, F, D] and W2 [E, D, F] stacked expert-major (zeros may be NULL or
+ * hold NULLs). topk_idx [N, k] MXFP4_I32 or _I64, ids outside [0, E) contribute nothing; topk_w [N, k] fp32.
+ * D and F multiples of group, E at most 4096, N k at most 2^24, N D at most 2^32. The 256-byte aligned
+ * workspace holds the routing and the rows between the products while the call runs. */
+size_t mxfp4_int4_moe_workspace_size(int N, int k, int E, int D, int F);
+int mxfp4_int4_moe_forward(void *out, const void *h, int dtype, const void *topk_idx, int idx_dtype,
+                           const float *topk_w, int N, int k, const uint8_t *const *codes,
+                           const void *const *scales, const uint8_t *const *zeros, int E, int D, int F,
+                           int group, int act_kind, void *workspace, size_t workspace_bytes,
+                           hipStream_t stream);
+
 /* Phase timing of the routed-layer calls made on the calling thread, the counterpart of the
  * reference's LAZYLORA_PROFILE timings (lazy_lora/trainer/lazy_trainer.py:192-194). While
  * enabled, every mxfp4_moe_forward/backward call records HIP events on its stream around

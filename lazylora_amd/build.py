@@ -12,9 +12,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblazylora_mxfp4.so")
-AUTOGRAD = "_dense_autograd"  # the dense operators' autograd functions: a Python module over LIB
+AUTOGRAD = "_dense_autograd"  # the operators' autograd functions: a Python module over LIB
+AUTOGRAD_SOURCES = ["dense_autograd.cpp", "moe_autograd.cpp"]
 SOURCES = ["capi.hip", "mx_forward.hip", "mx_backward.hip", "mx_misc.hip", "mx_router.hip", "mx_lora.hip",
-           "mx_dense.hip", "mx_rows.hip"]
+           "mx_dense.hip", "mx_rows.hip", "mx_select.hip", "mx_int4.hip"]
 
 # per-file flags: the transposed products keep their accumulators in VGPRs (the MFMA's VGPR
 # form); with the default heuristics the compiler splits them over AGPRs and VGPRs and shuffles
@@ -46,25 +47,25 @@ def _run(cmd):
 
 
 def _autograd_commands(objdir):
-    """(compile command, object, module path, link options) of the autograd module: host C++ against the
+    """(compile commands, objects, module path, link options) of the autograd module: host C++ against the
     installed torch, linked to LIB beside it."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
     root = os.path.dirname(torch.__file__)
-    obj = os.path.join(objdir, AUTOGRAD + ".o")
+    objs = [os.path.join(objdir, os.path.splitext(src)[0] + ".o") for src in AUTOGRAD_SOURCES]
     includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                 os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include"), sysconfig.get_paths()["include"]]
     cmd = ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1",
             "-DUSE_ROCM=1", f"-DTORCH_EXTENSION_NAME={AUTOGRAD}",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-           + [f"-isystem{d}" for d in includes]
-           + ["-c", os.path.join(CSRC, "dense_autograd.cpp"), "-o", obj])
+           + [f"-isystem{d}" for d in includes])
+    cmds = [cmd + ["-c", os.path.join(CSRC, src), "-o", obj] for src, obj in zip(AUTOGRAD_SOURCES, objs)]
     out = os.path.join(HERE, AUTOGRAD + sysconfig.get_config_var("EXT_SUFFIX"))
     libs = [f"-L{d}" for d in cpp_extension.library_paths()] + [
         "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_hip", LIB, "-Wl,-rpath,$ORIGIN"]
-    return cmd, obj, out, libs
+    return cmds, objs, out, libs
 
 
 def build(verbose: bool = False) -> str:
@@ -86,7 +87,7 @@ def build(verbose: bool = False) -> str:
         module = _autograd_commands(objdir)
     except ImportError as exc:
         trouble = str(exc)
-    commands = [cmd for cmd, _ in jobs] + ([module[0]] if module else [])
+    commands = [cmd for cmd, _ in jobs] + (module[0] if module else [])
     if verbose:
         for cmd in commands:
             print(" ".join(cmd), flush=True)
@@ -100,9 +101,10 @@ def build(verbose: bool = False) -> str:
     _link([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC"] + [o for _, o in jobs]
           + ["-Wl,-soname," + os.path.basename(LIB)], LIB)
     if module:
-        (cmd, obj, out, libs), (rc, trouble) = module, results[-1]
-        if rc == 0:
-            _link([cmd[0], "-shared", "-fPIC", obj] + libs, out)
+        cmds, objs, out, libs = module
+        trouble = "\n".join(err for rc, err in results[len(jobs):] if rc != 0)
+        if all(rc == 0 for rc, _ in results[len(jobs):]):
+            _link([cmds[0][0], "-shared", "-fPIC"] + objs + libs, out)
             return LIB
     raise RuntimeError(f"{os.path.basename(LIB)} is built, but not the autograd module over it ({AUTOGRAD}, the "
                        f"dense operators' Python entry points):\n{trouble}")

@@ -11,7 +11,9 @@
 #include "../../include/lazylora_mxfp4.h"
 #include "mx_dense.h"
 #include "mx_device.h"
+#include "mx_int4.h"
 #include "mx_kernels.h"
+#include "mx_select.h"
 
 // Device scratch of mxfp4_gemm_noalloc (see scratch_on_current_device below).
 constexpr size_t kScratchBytes = size_t(16) << 20;
@@ -643,6 +645,53 @@ int check_rows(const char* who, int M, int D, int kind, int dtype)
   return MXFP4_OK;
 }
 
+int check_select(const char* who, int dtype, int N, int E, int top_k, int scoring)
+{
+  static thread_local char msg[160];
+  const auto bad = [&](const char* what) {
+    snprintf(msg, sizeof(msg), "%s: %s", who, what);
+    return fail(MXFP4_EINVAL, "%s", msg);
+  };
+  if (dtype != MXFP4_F32 && dtype != MXFP4_BF16 && dtype != MXFP4_F16) return bad("dtype must be F32, BF16 or F16");
+  if (scoring != MXFP4_SCORE_SIGMOID && scoring != MXFP4_SCORE_SOFTMAX) return bad("unknown scoring");
+  if (N < 0 || E < 1 || E > 4096) return bad("need N >= 0 and E in [1, 4096]");
+  if (top_k < 1 || top_k > E || top_k > 64) return bad("need 1 <= top_k <= min(E, 64)");
+  return MXFP4_OK;
+}
+
+// A matrix of group-scaled 4-bit codes [R, K].
+int check_int4(const char* who, int dtype, int group, int K, int R)
+{
+  static thread_local char msg[160];
+  const auto bad = [&](const char* what) {
+    snprintf(msg, sizeof(msg), "%s: %s", who, what);
+    return fail(MXFP4_EINVAL, "%s", msg);
+  };
+  if (dtype != MXFP4_BF16 && dtype != MXFP4_F16) return bad("dtype must be BF16 or F16");
+  if (group != 32 && group != 64 && group != 128) return bad("group must be 32, 64 or 128");
+  if (K < 1 || K % group || K > kDenseMaxWidth || R < 1 || R > kDenseMaxWidth)
+    return bad("the widths must lie in [1, 2^20], the contracted one a multiple of group");
+  return MXFP4_OK;
+}
+
+// Workspace of a routed call over 4-bit weights: the tile count, the tiles, the pairs in their order, the
+// hidden rows (16 bits) and the down product's (fp32).
+constexpr long long kInt4MaxPairs = 1 << 24;
+struct Int4Workspace {
+  size_t tiles, order, hidden, rows, bytes;
+};
+Int4Workspace int4_workspace(int P, int E, int D, int F)
+{
+  const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  Int4Workspace w;
+  w.tiles = 256;
+  w.order = w.tiles + up(sizeof(int4) * mx::int4_max_tiles(P, E));
+  w.hidden = w.order + up(sizeof(int) * (size_t)P);
+  w.rows = w.hidden + up((size_t)2 * P * F);
+  w.bytes = w.rows + up(sizeof(float) * (size_t)P * D);
+  return w;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1248,6 +1297,146 @@ int mxfp4_dropout(void* y, const void* x, long long n, double p, uint64_t seed, 
   const float scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f;
   MX_TRY(mx::launch_dropout(y, x, n, (uint64_t)(p * 4294967296.0), scale, seed, seed_device, stream_id, dtype, stream),
          "dropout");
+  return MXFP4_OK;
+}
+
+// ---------------------------------------------------------------- expert selection with groups
+int mxfp4_select_topk(int64_t* topk_idx, float* topk_w, const void* logits, int dtype, const float* bias, int N, int E,
+                      int top_k, int scoring, int num_groups, int topk_groups, int group_score,
+                      float routed_scaling_factor, int renormalize, hipStream_t stream)
+{
+  const int rc = check_select("select_topk", dtype, N, E, top_k, scoring);
+  if (rc != MXFP4_OK) return rc;
+  if (group_score != MXFP4_GROUP_TOP2 && group_score != MXFP4_GROUP_MAX)
+    return fail(MXFP4_EINVAL, "select_topk: group_score must be MXFP4_GROUP_TOP2 or _MAX%s");
+  if (num_groups < 1 || num_groups > mx::kSelectLanes || E % num_groups || topk_groups < 1 || topk_groups > num_groups)
+    return fail(MXFP4_EINVAL, "select_topk: need 1 <= topk_groups <= num_groups <= 64, num_groups a divisor of E%s");
+  if (top_k > topk_groups * (E / num_groups))
+    return fail(MXFP4_EINVAL, "select_topk: the kept groups hold fewer than top_k experts%s");
+  if (mx::select_per_lane(E, num_groups) > mx::kSelectMaxPer)
+    return fail(MXFP4_EINVAL, "select_topk: the groups are too large for their number%s");
+  if (N == 0) return MXFP4_OK;
+  if (!topk_idx || !topk_w || !logits) return fail(MXFP4_EINVAL, "select_topk: null pointer%s");
+  mx::SelectArgs a = {};
+  a.topk_idx = reinterpret_cast<long long*>(topk_idx);
+  a.topk_w = topk_w;
+  a.logits = logits;
+  a.bias = bias;
+  a.N = N; a.E = E; a.top_k = top_k;
+  a.softmax = scoring == MXFP4_SCORE_SOFTMAX;
+  a.top2 = group_score == MXFP4_GROUP_TOP2;
+  a.num_groups = num_groups; a.topk_groups = topk_groups;
+  a.scale = routed_scaling_factor;
+  a.renormalize = renormalize && top_k > 1;
+  MX_TRY(mx::launch_select(a, dtype, stream), "select_topk");
+  return MXFP4_OK;
+}
+
+int mxfp4_select_topk_backward(void* grad_logits, const int64_t* topk_idx, const float* grad_w, const void* logits,
+                               int dtype, int N, int E, int top_k, int scoring, float routed_scaling_factor,
+                               int renormalize, hipStream_t stream)
+{
+  const int rc = check_select("select_topk_backward", dtype, N, E, top_k, scoring);
+  if (rc != MXFP4_OK) return rc;
+  if (N == 0) return MXFP4_OK;
+  if (!grad_logits || !topk_idx || !grad_w || !logits)
+    return fail(MXFP4_EINVAL, "select_topk_backward: null pointer%s");
+  mx::SelectBwdArgs a = {};
+  a.grad_logits = grad_logits;
+  a.topk_idx = reinterpret_cast<const long long*>(topk_idx);
+  a.grad_w = grad_w;
+  a.logits = logits;
+  a.N = N; a.E = E; a.top_k = top_k;
+  a.softmax = scoring == MXFP4_SCORE_SOFTMAX;
+  a.scale = routed_scaling_factor;
+  a.renormalize = renormalize && top_k > 1;
+  MX_TRY(mx::launch_select_bwd(a, dtype, stream), "select_topk_backward");
+  return MXFP4_OK;
+}
+
+// ---------------------------------------------------------------- 4-bit integer weights
+int mxfp4_int4_gemm(void* y, const void* x, const uint8_t* packed, const void* scales, const uint8_t* zeros, int dtype,
+                    int M, int K, int R, int group, hipStream_t stream)
+{
+  const int rc = check_int4("int4_gemm", dtype, group, K, R);
+  if (rc != MXFP4_OK) return rc;
+  if (M < 0 || M > (1 << 24)) return fail(MXFP4_EINVAL, "int4_gemm: M must lie in [0, 2^24]%s");
+  if (M == 0) return MXFP4_OK;
+  if (!y || !x || !packed || !scales) return fail(MXFP4_EINVAL, "int4_gemm: null pointer%s");
+  if (!all_aligned16({y, x, packed}))
+    return fail(MXFP4_EINVAL, "int4_gemm: y, x and packed must be 16-byte aligned%s");
+  if (reinterpret_cast<uintptr_t>(scales) & 1) return fail(MXFP4_EINVAL, "int4_gemm: scales must be 2-byte aligned%s");
+  mx::Int4Args a = {};
+  a.w[0] = {packed, scales, zeros};
+  a.x = x;
+  a.y = y;
+  a.M = M; a.K = K; a.R = R;
+  MX_TRY(mx::launch_int4_gemm(a, group, dtype, stream), "int4_gemm");
+  return MXFP4_OK;
+}
+
+size_t mxfp4_int4_moe_workspace_size(int N, int k, int E, int D, int F)
+{
+  if (N <= 0 || k <= 0 || E <= 0 || D <= 0 || F <= 0 || (long long)N * k > kInt4MaxPairs) return 0;
+  return int4_workspace(N * k, E, D, F).bytes;
+}
+
+int mxfp4_int4_moe_forward(void* out, const void* h, int dtype, const void* topk_idx, int idx_dtype,
+                           const float* topk_w, int N, int k, const uint8_t* const* codes, const void* const* scales,
+                           const uint8_t* const* zeros, int E, int D, int F, int group, int act_kind, void* workspace,
+                           size_t workspace_bytes, hipStream_t stream)
+{
+  int rc = check_int4("int4_moe_forward", dtype, group, D, F);
+  if (rc == MXFP4_OK) rc = check_int4("int4_moe_forward", dtype, group, F, D);
+  if (rc != MXFP4_OK) return rc;
+  if (idx_dtype != MXFP4_I32 && idx_dtype != MXFP4_I64)
+    return fail(MXFP4_EINVAL, "int4_moe_forward: idx_dtype must be I32 or I64%s");
+  if (act_kind != MXFP4_ACT_SWIGLU && act_kind != MXFP4_ACT_SITU)
+    return fail(MXFP4_EINVAL, "int4_moe_forward: unknown activation%s");
+  if (N < 0 || k < 1 || E < 1 || E > 4096 || (long long)N * k > kInt4MaxPairs || (long long)N * D > (1LL << 32))
+    return fail(MXFP4_EINVAL, "int4_moe_forward: need N >= 0, k >= 1, 1 <= E <= 4096, N k <= 2^24, N D <= 2^32%s");
+  if (N == 0) return MXFP4_OK;
+  if (!out || !h || !topk_idx || !topk_w || !codes || !scales || !workspace)
+    return fail(MXFP4_EINVAL, "int4_moe_forward: null pointer%s");
+  for (int m = 0; m < 3; ++m) {
+    if (!codes[m] || !scales[m]) return fail(MXFP4_EINVAL, "int4_moe_forward: null weight pointer%s");
+    if (!aligned16(codes[m]) || (reinterpret_cast<uintptr_t>(scales[m]) & 1))
+      return fail(MXFP4_EINVAL, "int4_moe_forward: codes must be 16-byte and scales 2-byte aligned%s");
+  }
+  if (!all_aligned16({out, h}) || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return fail(MXFP4_EINVAL, "int4_moe_forward: out and h must be 16-byte, the workspace 256-byte aligned%s");
+  const Int4Workspace ws = int4_workspace(N * k, E, D, F);
+  if (workspace_bytes < ws.bytes) return fail(MXFP4_EWORKSPACE, "int4_moe_forward: workspace too small%s");
+  char* base = static_cast<char*>(workspace);
+  const auto matrix = [&](int m) { return mx::Int4Matrix{codes[m], scales[m], zeros ? zeros[m] : nullptr}; };
+  mx::Int4Args a = {};
+  a.pairs = {topk_idx, idx_dtype == MXFP4_I64, N * k, k, E};
+  a.act = act_kind;
+  if (a.pairs.P > mx::kInt4ScanPairs) {
+    int* n_tiles = reinterpret_cast<int*>(base);
+    int4* tiles = reinterpret_cast<int4*>(base + ws.tiles);
+    int* order = reinterpret_cast<int*>(base + ws.order);
+    MX_TRY(mx::launch_int4_route(a.pairs, tiles, n_tiles, order, stream), "int4_moe_forward: routing");
+    a.tiles = tiles;
+    a.n_tiles = n_tiles;
+    a.order = order;
+  }
+  a.w[0] = matrix(0);
+  a.w[1] = matrix(1);
+  a.x = h;
+  a.x_div = k;
+  a.y = base + ws.hidden;
+  a.K = D; a.R = F;
+  MX_TRY(mx::launch_int4_glu(a, group, dtype, stream), "int4_moe_forward: gate/up");
+  a.w[0] = matrix(2);
+  a.x = base + ws.hidden;
+  a.x_div = 1;
+  a.y = base + ws.rows;
+  a.K = F; a.R = D;
+  MX_TRY(mx::launch_int4_pairs(a, group, dtype, stream), "int4_moe_forward: down");
+  MX_TRY(mx::launch_int4_combine(out, reinterpret_cast<const float*>(base + ws.rows), topk_w, a.pairs, D, dtype,
+                                 stream),
+         "int4_moe_forward: combine");
   return MXFP4_OK;
 }
 

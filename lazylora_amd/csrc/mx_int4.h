@@ -1,0 +1,56 @@
+// Kernel arguments and launch helpers of the products with group-scaled 4-bit weights (mx_int4.hip).
+// Host-visible; no torch types.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace mx {
+
+// One matrix [R, K], or E of them stacked: codes [R, K / 2] (low nibble = even element), scales [R, K / group]
+// of the activations' type, zero points [R, K / group] bytes or null (8 everywhere).
+struct Int4Matrix {
+  const uint8_t* q;
+  const void* s;
+  const uint8_t* z;
+};
+
+// The (token, slot) pairs of a routed call; pair p is slot p % k of token p / k.
+struct Int4Pairs {
+  const void* idx;  // [P] expert ids of 32 or 64 bits; outside [0, E): the pair has no expert
+  int idx64;
+  int P, k, E;
+};
+
+struct Int4Args {
+  Int4Matrix w[2];  // the second of a gate/up product
+  const void* x;    // rows of K elements
+  void* y;
+  int M, K, R;
+  // routed: x row of pair p is p / x_div, y row p
+  Int4Pairs pairs;
+  int x_div;
+  const int4* tiles;   // {expert, first, rows, 0} into order, n_tiles of them; null: found from the ids (P <= 64)
+  const int* n_tiles;
+  const int* order;
+  int act;
+  // set by the launcher: row groups of 16 weight rows, the first row tile of this launch
+  int row_groups, tile0;
+};
+
+// y [M, R] = x [M, K] W^T (dtype MXFP4_BF16 or _F16).
+hipError_t launch_int4_gemm(const Int4Args& a, int group, int dtype, hipStream_t s);
+
+// Rows of a routed tile for P pairs over E experts, and how many tiles there can be.
+int int4_tile_rows(int P, int E);
+inline int int4_max_tiles(int P, int E) { return P / int4_tile_rows(P, E) + (P < E ? P : E); }
+constexpr int kInt4ScanPairs = 64;  // up to so many pairs the products find their rows themselves
+hipError_t launch_int4_route(const Int4Pairs& p, int4* tiles, int* n_tiles, int* order, hipStream_t s);
+// h [P, R] = GLU(x W1^T, x W3^T) of each pair's expert.
+hipError_t launch_int4_glu(const Int4Args& a, int group, int dtype, hipStream_t s);
+// y [P, R] fp32 = x W^T of each pair's expert.
+hipError_t launch_int4_pairs(const Int4Args& a, int group, int dtype, hipStream_t s);
+// out [N, D] = sum over slots, in slot order, of topk_w y of the pairs that have an expert.
+hipError_t launch_int4_combine(void* out, const float* y, const float* topk_w, const Int4Pairs& p, int D, int dtype,
+                               hipStream_t s);
+
+}  // namespace mx

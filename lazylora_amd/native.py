@@ -35,6 +35,8 @@ _ACTS = {"swiglu": ACT_SWIGLU, "situ": ACT_SITU, "situ_glu": ACT_SITU, ACT_SWIGL
 
 F32, BF16, I32, I64, F16 = 0, 1, 2, 3, 4
 NORM_RMS, NORM_LAYER = 0, 1
+SCORINGS = {"sigmoid": 0, "softmax": 1}
+GROUP_SCORES = {"top2": 0, "max": 1}
 _FLOATS = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 MOE_SAVE = 1
 MOE_REUSE_FORWARD = 2
@@ -124,6 +126,16 @@ def _load_library() -> ctypes.CDLL:
     lib.mxfp4_norm_backward.argtypes = [vp] * 7 + [ci] * 4 + [vp, sz, vp]
     lib.mxfp4_dropout.restype = ci
     lib.mxfp4_dropout.argtypes = [vp, vp, cll, ctypes.c_double, cu64, vp, cu64, ci, vp]
+    lib.mxfp4_select_topk.restype = ci
+    lib.mxfp4_select_topk.argtypes = [vp, vp, vp, ci, vp] + [ci] * 7 + [ctypes.c_float, ci, vp]
+    lib.mxfp4_select_topk_backward.restype = ci
+    lib.mxfp4_select_topk_backward.argtypes = [vp] * 4 + [ci] * 5 + [ctypes.c_float, ci, vp]
+    lib.mxfp4_int4_gemm.restype = ci
+    lib.mxfp4_int4_gemm.argtypes = [vp] * 5 + [ci] * 5 + [vp]
+    lib.mxfp4_int4_moe_workspace_size.restype = sz
+    lib.mxfp4_int4_moe_workspace_size.argtypes = [ci] * 5
+    lib.mxfp4_int4_moe_forward.restype = ci
+    lib.mxfp4_int4_moe_forward.argtypes = [vp, vp, ci, vp, ci, vp, ci, ci, vp, vp, vp] + [ci] * 5 + [vp, sz, vp]
     lib.mxfp4_moe_timing.restype = ci
     lib.mxfp4_moe_timing.argtypes = [ci]
     lib.mxfp4_moe_timed_calls.restype = ci

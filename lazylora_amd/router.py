@@ -10,6 +10,10 @@ routed-expert layer without a host round trip. Gradients flow from topk_weights 
 the logits into x (and the gate weight, if it requires grad), as torch autograd does through the
 reference's torch branch; the trainer relies on that (lazy_lora/trainer/lazy_trainer.py:842-844).
 
+`select_experts` is the same step for routers of other forms, from logits of any floating type: softmax or
+sigmoid scores, a choice limited to the best groups of experts, with its gradient; `route`,
+KimiK3MoERouter and LatentMoEBlock take its options.
+
 Differences from the reference, all deliberate:
   * equal biased scores go to the lower expert id first (torch.topk leaves their order
     unspecified; the NumPy branch's argsort is not stable either);
@@ -24,7 +28,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from lazylora_amd.native import kernel
+from lazylora_amd.dense import _module
+from lazylora_amd.native import GROUP_SCORES, SCORINGS, kernel
 
 
 def _native():
@@ -55,12 +60,40 @@ class _Select(torch.autograd.Function):
         return grad_logits, None, None, None, None
 
 
+def select_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor] = None, scoring: str = "sigmoid",
+                   num_groups: int = 1, topk_groups: Optional[int] = None, group_score: str = "top2",
+                   renormalize: bool = True, routed_scaling_factor: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(topk_indices [..., top_k] int64, topk_weights [..., top_k] fp32) from router logits [..., E] (float32,
+    bfloat16 or float16, on the HIP device), differentiable in the logits.
+
+    Scores are sigmoid(logits) or softmax(logits) (`scoring`); the choice goes by score + bias (bias [E] of any
+    floating type, for the choice only: no gradient), the weights are the chosen scores, divided by their sum +
+    1e-20 with `renormalize` (and top_k > 1), times routed_scaling_factor. With num_groups > 1 the experts form
+    that many equal runs and only the topk_groups best of them (None: all) can be chosen from, by the sum of
+    each group's two largest values of score + bias (group_score "top2") or by its largest ("max").
+
+    Indices are in descending order of score + bias, as exact arithmetic on the given numbers has it (without a
+    bias: of the logits); equal values go to the lower id, equal groups to the lower number, NaN comes first. A
+    softmax row of -inf alone has weights 0. E <= 4096 (where num_groups is no power of two, 64 * 64 experts
+    for the next power of two of groups), num_groups <= 64, top_k <= min(64, experts of the kept groups).
+    Second derivatives, forward-mode differentiation and tracing raise, as in lazylora_amd.dense."""
+    if scoring not in SCORINGS:
+        raise ValueError(f"unknown scoring {scoring!r}")
+    if group_score not in GROUP_SCORES:
+        raise ValueError(f"unknown group score {group_score!r}")
+    return _module().select_experts(logits, bias, top_k, SCORINGS[scoring], num_groups,
+                            num_groups if topk_groups is None else topk_groups, GROUP_SCORES[group_score],
+                            routed_scaling_factor, renormalize)
+
+
 def route(x: Union[torch.Tensor, np.ndarray], weight: Union[torch.Tensor, np.ndarray],
           bias: Optional[Union[torch.Tensor, np.ndarray]] = None, top_k: int = 16,
-          routed_scaling_factor: float = 1.0, renormalize: bool = True):
+          routed_scaling_factor: float = 1.0, renormalize: bool = True, scoring: str = "sigmoid",
+          num_groups: int = 1, topk_groups: Optional[int] = None, group_score: str = "top2"):
     """(topk_indices [N, k] int64, topk_weights [N, k] fp32) for tokens x [..., hidden] and gate
     weight [E, hidden] (moe_router.py:81-99). NumPy in, NumPy out; torch tensors come back on
-    x's device."""
+    x's device. scoring, num_groups, topk_groups and group_score as in select_experts, which makes the
+    selection unless they are the reference's (sigmoid, one group)."""
     as_numpy = isinstance(x, np.ndarray)
     xt = torch.from_numpy(np.asarray(x, np.float32)) if as_numpy else x
     if xt.is_cuda:
@@ -77,7 +110,11 @@ def route(x: Union[torch.Tensor, np.ndarray], weight: Union[torch.Tensor, np.nda
         raise ValueError(f"x has width {xt.shape[-1]} but the gate takes {hidden}")
     b = None if bias is None else torch.as_tensor(bias).to(dev, torch.float32)
     logits = F.linear(xt.reshape(-1, hidden).to(dev, torch.float32), w)   # [N, E] fp32
-    idx, tw = _Select.apply(logits, b, int(top_k), float(routed_scaling_factor), bool(renormalize))
+    if scoring == "sigmoid" and num_groups == 1 and topk_groups in (None, 1):
+        idx, tw = _Select.apply(logits, b, int(top_k), float(routed_scaling_factor), bool(renormalize))
+    else:
+        idx, tw = select_experts(logits, int(top_k), b, scoring, num_groups, topk_groups, group_score,
+                                 bool(renormalize), float(routed_scaling_factor))
     if as_numpy:
         return idx.cpu().numpy(), tw.detach().cpu().numpy()
     if not xt.is_cuda:
@@ -86,11 +123,13 @@ def route(x: Union[torch.Tensor, np.ndarray], weight: Union[torch.Tensor, np.nda
 
 
 class KimiK3MoERouter(nn.Module):
-    """KimiK3MoERouter (lazy_lora/core/moe_router.py:23-135) with the selection on MI355X."""
+    """KimiK3MoERouter (lazy_lora/core/moe_router.py:23-135) with the selection on MI355X; scoring and the
+    group arguments as in select_experts."""
 
     def __init__(self, hidden_size: int = 7168, num_experts: int = 896, top_k: int = 16,
                  routed_scaling_factor: float = 1.0, renormalize: bool = True, use_bias: bool = True,
-                 device: Optional[Union[str, torch.device]] = None):
+                 device: Optional[Union[str, torch.device]] = None, scoring: str = "sigmoid", num_groups: int = 1,
+                 topk_groups: Optional[int] = None, group_score: str = "top2"):
         super().__init__()
         self.weight = nn.Parameter(torch.empty(num_experts, hidden_size, device=device))
         self.bias = nn.Parameter(torch.zeros(num_experts, device=device)) if use_bias else None
@@ -101,6 +140,7 @@ class KimiK3MoERouter(nn.Module):
         self.routed_scaling_factor = routed_scaling_factor
         self.renormalize = renormalize
         self.use_bias = use_bias
+        self.scoring, self.num_groups, self.topk_groups, self.group_score = scoring, num_groups, topk_groups, group_score
 
     def forward(self, x, weight=None, bias=None) -> Tuple[torch.Tensor, torch.Tensor]:
         """(topk_indices [N, top_k] int64, topk_weights [N, top_k] fp32). `weight`/`bias`
@@ -109,7 +149,8 @@ class KimiK3MoERouter(nn.Module):
             weight = self.weight
         if bias is None:
             bias = self.bias
-        return route(x, weight, bias, self.top_k, self.routed_scaling_factor, self.renormalize)
+        return route(x, weight, bias, self.top_k, self.routed_scaling_factor, self.renormalize, self.scoring,
+                     self.num_groups, self.topk_groups, self.group_score)
 
     @staticmethod
     def get_active_expert_set(topk_indices) -> List[int]:
