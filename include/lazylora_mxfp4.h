@@ -356,8 +356,8 @@ int mxfp4_int4_gemm(void *y, const void *x, const uint8_t *packed, const void *s
 /* The routed expert layer over such weights:
  *   out[t] = sum over slots of topk_w[t, j] W2_e . GLU(W1_e . h[t], W3_e . h[t]), e = topk_idx[t, j],
  * h and out [N, D] of dtype, the GLU's results rounded to dtype in between. codes, scales and zeros: host
- * arrays of 3 device pointers, W1 and W3 [E, F, D] and W2 [E, D, F] stacked expert-major (zeros may be NULL or
- * hold NULLs). topk_idx [N, k] MXFP4_I32 or _I64, ids outside [0, E) contribute nothing; topk_w [N, k] fp32.
+ * arrays of 3 device pointers, W1 and W3 [E, F, D] and W2 [E, D, F] stacked expert-major (zeros may be NULL, or
+ * hold three NULLs). topk_idx [N, k] MXFP4_I32 or _I64, ids outside [0, E) contribute nothing; topk_w [N, k] fp32.
  * D and F multiples of group, E at most 4096, N k at most 2^24, N D at most 2^32. The 256-byte aligned
  * workspace holds the routing and the rows between the products while the call runs. */
 size_t mxfp4_int4_moe_workspace_size(int N, int k, int E, int D, int F);

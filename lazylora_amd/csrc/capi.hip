@@ -1400,6 +1400,7 @@ int mxfp4_int4_moe_forward(void* out, const void* h, int dtype, const void* topk
     return fail(MXFP4_EINVAL, "int4_moe_forward: null pointer%s");
   for (int m = 0; m < 3; ++m) {
     if (!codes[m] || !scales[m]) return fail(MXFP4_EINVAL, "int4_moe_forward: null weight pointer%s");
+    if (zeros && !zeros[m] != !zeros[0]) return fail(MXFP4_EINVAL, "int4_moe_forward: zeros of all matrices or none%s");
     if (!aligned16(codes[m]) || (reinterpret_cast<uintptr_t>(scales[m]) & 1))
       return fail(MXFP4_EINVAL, "int4_moe_forward: codes must be 16-byte and scales 2-byte aligned%s");
   }
@@ -1412,7 +1413,8 @@ int mxfp4_int4_moe_forward(void* out, const void* h, int dtype, const void* topk
   mx::Int4Args a = {};
   a.pairs = {topk_idx, idx_dtype == MXFP4_I64, N * k, k, E};
   a.act = act_kind;
-  if (a.pairs.P > mx::kInt4ScanPairs) {
+  a.by_token = mx::int4_by_token(N, D, F);
+  if (!a.by_token && a.pairs.P > mx::kInt4ScanPairs) {
     int* n_tiles = reinterpret_cast<int*>(base);
     int4* tiles = reinterpret_cast<int4*>(base + ws.tiles);
     int* order = reinterpret_cast<int*>(base + ws.order);
@@ -1431,8 +1433,14 @@ int mxfp4_int4_moe_forward(void* out, const void* h, int dtype, const void* topk
   a.w[0] = matrix(2);
   a.x = base + ws.hidden;
   a.x_div = 1;
-  a.y = base + ws.rows;
   a.K = F; a.R = D;
+  if (a.by_token) {
+    a.y = out;
+    a.row_w = topk_w;
+    MX_TRY(mx::launch_int4_token(a, group, dtype, stream), "int4_moe_forward: down");
+    return MXFP4_OK;
+  }
+  a.y = base + ws.rows;
   MX_TRY(mx::launch_int4_pairs(a, group, dtype, stream), "int4_moe_forward: down");
   MX_TRY(mx::launch_int4_combine(out, reinterpret_cast<const float*>(base + ws.rows), topk_w, a.pairs, D, dtype,
                                  stream),

@@ -7,12 +7,19 @@
 // all exact products in fp32 sums, and one multiply-add by the group's scale per result. A row of x with an
 // infinity gives NaN (the difference of two infinities).
 #include "mx_device.h"
+#include <stdlib.h>
 #include "mx_int4.h"
 
 namespace mx {
 
 namespace {
 
+constexpr int kVecRows = 8;     // weight rows of a batch of the few-row form
+constexpr int kVecBatches = 16;  // batches of a work-group at most
+constexpr int kVecMost = 4;      // its rows of x at most
+constexpr int kVecMinK = 1024;  // and the shortest rows it takes
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 template <typename T>
@@ -26,6 +33,10 @@ struct Num<__bf16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                    0, 0);
   }
+  static MX_DEV float dot2(uint32_t a, uint32_t b, float c)
+  {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a), __builtin_bit_cast(bf16x2, b), c, false);
+  }
   static MX_DEV float widen(uint16_t v) { return bits_f((uint32_t)v << 16); }
   static MX_DEV uint16_t narrow(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 };
@@ -38,20 +49,37 @@ struct Num<_Float16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                   0);
   }
+  static MX_DEV float dot2(uint32_t a, uint32_t b, float c)
+  {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, a), __builtin_bit_cast(f16x2, b), c, false);
+  }
   static MX_DEV float widen(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
   static MX_DEV uint16_t narrow(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 };
 
+// The decoder's constants in registers: and-or of three operands is one instruction then, which takes one
+// scalar register and no literals.
+struct Decoder {
+  uint32_t mask, base;
+};
+template <typename T>
+MX_DEV Decoder decoder()
+{
+  Decoder d;
+  asm("s_mov_b32 %0, %1" : "=s"(d.mask) : "i"(Num<T>::kMask));
+  asm("v_mov_b32 %0, %1" : "=v"(d.base) : "i"(Num<T>::kBase));
+  return d;
+}
 // The 8 codes of a dword as 16-bit numbers 16 + q, in pairs of codes (p, p + 4), p = 0..3.
 template <typename T>
-MX_DEV i32x4 decode8(uint32_t w)
+MX_DEV i32x4 decode8(uint32_t w, Decoder k)
 {
   using N = Num<T>;
   i32x4 r;
   static_for<4>([&](auto pc) {
     constexpr int p = decltype(pc)::value, sh = 4 * p - N::kShift;
     const uint32_t v = sh < 0 ? w << (sh < 0 ? -sh : 0) : w >> (sh < 0 ? 0 : sh);
-    r[p] = (int)((v & N::kMask) | N::kBase);
+    r[p] = (int)((v & k.mask) | k.base);
   });
   return r;
 }
@@ -101,15 +129,244 @@ MX_DEV int pair_expert(const Int4Pairs& p, int i)
   return e >= 0 && e < p.E ? (int)e : -1;
 }
 
+// Sum over the 16 lanes of a row, in every lane.
+MX_DEV float row_sum(float v)
+{
+  v += dpp_lane<kDppXor1>(v);
+  v += dpp_lane<kDppXor2>(v);
+  v += dpp_lane<kDppHalfMirror>(v);
+  return v + dpp_lane<kDppMirror>(v);
+}
+
 enum Int4Epi : int {
   kInt4Store = 0,  // y[m] = the product's row, dense
   kInt4Glu = 1,    // y[p] = GLU of the gate and the up product of pair p
   kInt4Pair = 2,   // y[p] = the product of pair p, fp32
+  kInt4Token = 3,  // y[t] = the weighted sum of the products of token t's pairs
 };
 
+// Result o of a product (a gate and an up product).
+template <typename T, Int4Epi EPI>
+MX_DEV void store(const Int4Args& p, long long o, float a, float b)
+{
+  if (EPI == kInt4Pair)
+    static_cast<float*>(p.y)[o] = a;
+  else
+    static_cast<uint16_t*>(p.y)[o] = Num<T>::narrow(EPI == kInt4Glu ? glu_fwd(a, b, p.act) : a);
+}
+
+// The rows of a work-group's tile (up to ROWS of them): their numbers into rows[] (the places behind the last
+// repeat it), the expert and the count. False: there is nothing to do. The work-group synchronises after it.
+template <int ROWS, Int4Epi EPI>
+MX_DEV bool find_rows(const Int4Args& p, int tile, int* rows, int& e, int& nrows)
+{
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (EPI == kInt4Store) {
+    e = 0;
+    nrows = min(ROWS, p.M - tile * ROWS);
+    if (tid < ROWS) rows[tid] = tile * ROWS + min(tid, nrows - 1);
+  } else if (p.tiles) {
+    if (tile >= *p.n_tiles) return false;
+    const int4 t = p.tiles[tile];
+    e = __builtin_amdgcn_readfirstlane(t.x);  // the same on every lane: addresses from it are scalar
+    nrows = __builtin_amdgcn_readfirstlane(t.z);
+    if (tid < ROWS) rows[tid] = p.order[t.y + min(tid, nrows - 1)];
+  } else {
+    // the pairs of this one's expert from this one on, which must be the first of their tile
+    const int mine = lane < p.pairs.P ? pair_expert(p.pairs, lane) : -1;
+    e = __builtin_amdgcn_readlane(mine, tile);
+    if (e < 0) return false;
+    const uint64_t same = __builtin_amdgcn_ballot_w64(mine == e);
+    const int first = __popcll(same & ((1ull << tile) - 1));
+    if (first % ROWS) return false;
+    nrows = min(ROWS, __popcll(same) - first);
+    const int at = __popcll(same & ((1ull << lane) - 1)) - first;
+    if (tid < 64 && mine == e && at >= 0 && at < nrows) {
+      rows[at] = lane;
+      if (at == nrows - 1)
+        for (int i = nrows; i < ROWS; ++i) rows[i] = lane;
+    }
+  }
+  return true;
+}
+
+// A tile's rows of one matrix as buffers: codes, scales and zero points from row `first` on. A load adds a lane's
+// offset (past the buffer, kOob, it gives zeros and reads nothing) and one that the wave shares.
+constexpr uint32_t kOob = 0x80000000u;
+struct Rows {
+  __amdgpu_buffer_rsrc_t q, s, z;
+};
+MX_DEV __amdgpu_buffer_rsrc_t buffer(const void* base, uint32_t bytes)
+{
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+MX_DEV Rows weight_rows(const Int4Matrix& w, long long first, int count, int K, int groups)
+{
+  return {buffer(w.q + first * (K / 2), (uint32_t)count * (K / 2)),
+          buffer(static_cast<const uint16_t*>(w.s) + first * groups, 2u * count * groups),
+          buffer(w.z + first * groups, (uint32_t)count * groups)};
+}
+MX_DEV i32x4 load_codes(const Rows& w, uint32_t lane, uint32_t shared)
+{
+  return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(w.q, (int)lane, (int)shared, 0));
+}
+MX_DEV uint16_t load_scale(const Rows& w, uint32_t lane, uint32_t shared)
+{
+  return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(w.s, (int)(2 * lane), (int)(2 * shared), 0);
+}
+MX_DEV uint8_t load_zero(const Rows& w, uint32_t lane, uint32_t shared)
+{
+  return (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(w.z, (int)lane, (int)shared, 0);
+}
+
+// ------------------------------------------------------------------ few rows of x
+// Lane i keeps the elements 32 i .. 32 i + 31 of up to MR rows of x in registers and walks the weight rows,
+// kVecRows of them loaded while those before are summed. A wave's load is 1 KiB of one row, x is loaded once
+// for all rows of a work-group (the MFMA form below loads as many bytes of x as of codes for every 16 x 128
+// block), and a product is two instructions for two codes and one dot of two for each row of x. The lanes'
+// sums meet in exchanges of half-waves and quarter-waves, each of which halves how many there are, the waves'
+// in LDS.
+template <typename T, int G, bool ZP, int MR, Int4Epi EPI>
+__global__ __launch_bounds__(512) void int4_vec_kernel(Int4Args p)
+{
+  using N = Num<T>;
+  constexpr int NMAT = EPI == kInt4Glu ? 2 : 1, RB = kVecRows / NMAT, NV = kVecRows * MR;
+  extern __shared__ float red[];  // [waves][batches][NV]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int item = blockIdx.x / p.row_groups + p.tile0, r0 = (blockIdx.x % p.row_groups) * (p.batches * RB);
+  const int batches = min(p.batches, (p.R - r0 + RB - 1) / RB), groups = p.K / G;
+  const int team = EPI == kInt4Token ? wave / p.team : 0;  // waves that share a row of K
+  const int first_k = 32 * (EPI == kInt4Token ? (int)threadIdx.x - team * p.team * 64 : (int)threadIdx.x);
+  const int stride_k = 32 * 64 * (EPI == kInt4Token ? p.team : waves);
+  const Decoder dec = decoder<T>();
+  float* mine = red + wave * p.batches * NV;
+  // a lane's place of value i of a batch, i < NV / 4, after the exchanges
+  const int place = (lane >> 4 & 1) * (NV / 4) + (lane >> 5) * (NV / 2);
+  for (int i = lane; i < batches * NV; i += 64) mine[i] = 0.f;
+  wave_lds_fence();
+
+  // one expert's rows (of a token: one slot after another of this team's)
+  const auto rows_of_expert = [&](int e, long long x_row, float weight) {
+    Rows w[NMAT];
+#pragma unroll
+    for (int m = 0; m < NMAT; ++m)
+      w[m] = weight_rows(p.w[m], (long long)e * p.R + r0, min(p.batches * RB, p.R - r0), p.K, groups);
+    struct Batch {
+      i32x4 q[kVecRows];
+      uint16_t s[kVecRows];
+      uint8_t z[kVecRows];
+    };
+    for (int k = first_k; k - first_k < p.K; k += stride_k) {  // the same rounds on every lane
+      const bool in = k < p.K;
+      const uint32_t at_q = in ? (uint32_t)k / 2 : kOob, at_s = in ? (uint32_t)k / G : kOob / 2;
+      // A batch behind the last is loaded all the same, from past the buffers, so that what is in flight where the
+      // one before it is summed is the same on every path: at a branch around these loads the compiler waits for all.
+      const auto load = [&](int b, Batch& c) {
+        const uint32_t lane_q = b < batches ? at_q : kOob, lane_s = b < batches ? at_s : kOob / 2;
+#pragma unroll
+        for (int r = 0; r < kVecRows; ++r) {
+          const uint32_t row = min(b * RB + r % RB, p.R - 1 - r0);
+          c.q[r] = load_codes(w[r / RB], lane_q, row * (p.K / 2));
+          c.s[r] = load_scale(w[r / RB], lane_s, row * groups);
+          c.z[r] = ZP ? load_zero(w[r / RB], lane_s, row * groups) : (uint8_t)8;
+        }
+      };
+      Batch c0, c1;
+      load(0, c0);
+      uint32_t x[MR][16];
+      float sum[MR];
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        const long long row = EPI == kInt4Store ? min(m, p.M - 1) : x_row;
+        const i32x4* src = reinterpret_cast<const i32x4*>(static_cast<const uint16_t*>(p.x) + row * p.K + (in ? k : 0));
+        sum[m] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const i32x4 t = pair_up(src[j]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[m][4 * j + i] = in ? (uint32_t)t[i] : 0u;
+            sum[m] = N::dot2(x[m][4 * j + i], N::kOnes, sum[m]);
+          }
+        }
+      }
+      const auto multiply = [&](int b, const Batch& c) {
+        float v[NV];
+#pragma unroll
+        for (int r = 0; r < kVecRows; ++r) {
+          float t[MR];
+#pragma unroll
+          for (int m = 0; m < MR; ++m) t[m] = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const i32x4 d = decode8<T>((uint32_t)c.q[r][j], dec);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int m = 0; m < MR; ++m) t[m] = N::dot2(x[m][4 * j + i], (uint32_t)d[i], t[m]);
+          }
+          const float scale = N::widen(c.s[r]) * weight, zero = -16.0f - (float)c.z[r];
+#pragma unroll
+          for (int m = 0; m < MR; ++m) v[r * MR + m] = scale * fmaf(zero, sum[m], t[m]);
+        }
+        // of two values a lane keeps one, with the other lane's share
+#pragma unroll
+        for (int i = 0; i < NV / 2; ++i) {
+          const auto r = __builtin_amdgcn_permlane32_swap(f_bits(v[i]), f_bits(v[i + NV / 2]), false, false);
+          v[i] = bits_f(r[0]) + bits_f(r[1]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV / 4; ++i) {
+          const auto r = __builtin_amdgcn_permlane16_swap(f_bits(v[i]), f_bits(v[i + NV / 4]), false, false);
+          v[i] = row_sum(bits_f(r[0]) + bits_f(r[1]));
+        }
+        if ((lane & 15) == 0) {
+#pragma unroll
+          for (int i = 0; i < NV / 4; ++i) mine[b * NV + place + i] += v[i];
+        }
+      };
+      for (int b = 0; b < batches; b += 2) {
+        load(b + 1, c1);
+        __builtin_amdgcn_sched_barrier(0);  // the loads first, not where their registers are free at last
+        multiply(b, c0);
+        if (b + 1 >= batches) break;
+        load(b + 2, c0);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(b + 1, c1);
+      }
+    }
+  };
+  if (EPI == kInt4Token) {
+    const int teams = waves / p.team;
+    for (int j = team; j < p.pairs.k; j += teams) {
+      const int q = item * p.pairs.k + j;
+      const int e = __builtin_amdgcn_readfirstlane(pair_expert(p.pairs, q));
+      if (e >= 0) rows_of_expert(e, q, p.row_w[q]);
+    }
+  } else if (EPI == kInt4Glu) {
+    const int e = __builtin_amdgcn_readfirstlane(pair_expert(p.pairs, item));
+    if (e < 0) return;  // the whole work-group
+    rows_of_expert(e, item / p.x_div, 1.f);
+  } else {
+    rows_of_expert(0, 0, 1.f);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < batches * RB * MR; i += blockDim.x) {
+    const int b = i / (RB * MR), j = i % (RB * MR), m = j % MR, row = r0 + b * RB + j / MR;
+    float u = 0.f, v = 0.f;
+    for (int w = 0; w < waves; ++w) {
+      u += red[(w * p.batches + b) * NV + j];
+      if (NMAT == 2) v += red[(w * p.batches + b) * NV + RB * MR + j];
+    }
+    const long long o = EPI == kInt4Store ? m : item;
+    if ((EPI != kInt4Store || m < p.M) && row < p.R) store<T, EPI>(p, o * p.R + row, u, v);
+  }
+}
+
+// ------------------------------------------------------------------ tiles of rows of x
 // A work-group makes 16 weight rows x up to 16 MT rows of x; its waves share K, block pair by block pair (so
 // that a wave reads whole 128-byte lines), and their sums meet in LDS in the waves' order.
-template <typename T, int G, int MT, Int4Epi EPI, int MAXW>
+template <typename T, int G, bool ZP, int MT, Int4Epi EPI, int MAXW>
 __global__ __launch_bounds__(64 * MAXW) void int4_rows_kernel(Int4Args p)
 {
   using N = Num<T>;
@@ -120,45 +377,20 @@ __global__ __launch_bounds__(64 * MAXW) void int4_rows_kernel(Int4Args p)
   const int n = lane & 15, c = lane >> 4;
   const int tile = blockIdx.x / p.row_groups + p.tile0, r0 = (blockIdx.x % p.row_groups) * 16;
 
-  int e = 0, nrows;
-  if (EPI == kInt4Store) {
-    nrows = min(16 * MT, p.M - tile * (16 * MT));
-    if ((int)threadIdx.x < 16 * MT) rows[threadIdx.x] = tile * (16 * MT) + min((int)threadIdx.x, nrows - 1);
-  } else if (p.tiles) {
-    if (tile >= *p.n_tiles) return;
-    const int4 t = p.tiles[tile];
-    e = t.x;
-    nrows = t.z;
-    if ((int)threadIdx.x < 16 * MT) rows[threadIdx.x] = p.order[t.y + min((int)threadIdx.x, nrows - 1)];
-  } else {
-    // the pairs of this one's expert from this one on, which must be the first of their tile
-    const int mine = lane < p.pairs.P ? pair_expert(p.pairs, lane) : -1;
-    e = __builtin_amdgcn_readlane(mine, tile);
-    if (e < 0) return;
-    const uint64_t same = __builtin_amdgcn_ballot_w64(mine == e);
-    const int first = __popcll(same & ((1ull << tile) - 1));
-    if (first % (16 * MT)) return;
-    nrows = min(16 * MT, __popcll(same) - first);
-    const int at = __popcll(same & ((1ull << lane) - 1)) - first;
-    if (wave == 0 && mine == e && at >= 0 && at < nrows) rows[at] = lane;
-  }
+  int e, nrows;
+  if (!find_rows<16 * MT, EPI>(p, tile, rows, e, nrows)) return;
   __syncthreads();
 
-  const int wr = min(r0 + n, p.R - 1), groups = p.K / G;
-  const uint8_t* wq[NMAT];
-  const uint16_t* ws[NMAT];
-  const uint8_t* wz[NMAT];
+  const int wr = min(n, p.R - 1 - r0), groups = p.K / G;
+  const Decoder dec = decoder<T>();
+  Rows w[NMAT];
 #pragma unroll
-  for (int m = 0; m < NMAT; ++m) {
-    const long long r = (long long)e * p.R + wr;
-    wq[m] = p.w[m].q + r * (p.K / 2);
-    ws[m] = static_cast<const uint16_t*>(p.w[m].s) + r * groups;
-    wz[m] = p.w[m].z ? p.w[m].z + r * groups : nullptr;
-  }
+  for (int m = 0; m < NMAT; ++m)
+    w[m] = weight_rows(p.w[m], (long long)e * p.R + r0, min(16, p.R - r0), p.K, groups);
   const uint16_t* xr[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
-    const int i = rows[min(16 * t + n, nrows - 1)];
+    const int i = rows[16 * t + n];
     xr[t] = static_cast<const uint16_t*>(p.x) + (long long)(EPI == kInt4Store ? i : i / p.x_div) * p.K;
   }
 
@@ -175,17 +407,17 @@ __global__ __launch_bounds__(64 * MAXW) void int4_rows_kernel(Int4Args p)
     uint16_t s[NMAT][NG];
     uint8_t z[NMAT][NG];
   };
-  // past K the codes are some other of the row's and x is 0
+  // past K codes and x are 0
   const auto load = [&](int b, Block& k) {
-    const int kc = G == 128 ? b * 128 + 32 * c : min(b * 128 + 32 * c, p.K - 32);
+    const bool in = G == 128 || b * 128 + 32 * c < p.K;
 #pragma unroll
     for (int m = 0; m < NMAT; ++m) {
-      k.q[m] = *reinterpret_cast<const i32x4*>(wq[m] + kc / 2);
+      k.q[m] = load_codes(w[m], in ? (uint32_t)wr * (p.K / 2) + 16 * c : kOob, b * 64);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const int gi = G == 128 ? b : min(b * NG + g, groups - 1);
-        k.s[m][g] = ws[m][gi];
-        k.z[m][g] = wz[m] ? wz[m][gi] : (uint8_t)8;
+        k.s[m][g] = load_scale(w[m], (uint32_t)wr * groups, gi);
+        k.z[m][g] = ZP ? load_zero(w[m], (uint32_t)wr * groups, gi) : (uint8_t)8;
       }
     }
 #pragma unroll
@@ -211,15 +443,15 @@ __global__ __launch_bounds__(64 * MAXW) void int4_rows_kernel(Int4Args p)
       f32x4 sum[MT], dot[NMAT][MT];
 #pragma unroll
       for (int j = g * JG; j < (g + 1) * JG; ++j) {
-        i32x4 w[NMAT];
+        i32x4 b[NMAT];
 #pragma unroll
-        for (int m = 0; m < NMAT; ++m) w[m] = decode8<T>(d[m][j]);
+        for (int m = 0; m < NMAT; ++m) b[m] = decode8<T>(d[m][j], dec);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           const i32x4 x = pair_up(k.x[t][j]);
           sum[t] = N::mfma(x, ones, j == g * JG ? zero : sum[t]);
 #pragma unroll
-          for (int m = 0; m < NMAT; ++m) dot[m][t] = N::mfma(x, w[m], j == g * JG ? zero : dot[m][t]);
+          for (int m = 0; m < NMAT; ++m) dot[m][t] = N::mfma(x, b[m], j == g * JG ? zero : dot[m][t]);
         }
       }
 #pragma unroll
@@ -256,11 +488,7 @@ __global__ __launch_bounds__(64 * MAXW) void int4_rows_kernel(Int4Args p)
       for (int w = 0; w < waves; ++w) v[m] += sums[(w * NMAT + m) * MT * 256 + at];
     }
     if (row >= nrows || r0 + col >= p.R) continue;
-    const long long o = (long long)rows[row] * p.R + r0 + col;
-    if (EPI == kInt4Pair)
-      static_cast<float*>(p.y)[o] = v[0];
-    else
-      static_cast<uint16_t*>(p.y)[o] = N::narrow(EPI == kInt4Glu ? glu_fwd(v[0], v[NMAT - 1], p.act) : v[0]);
+    store<T, EPI>(p, (long long)rows[row] * p.R + r0 + col, v[0], v[NMAT - 1]);
   }
 }
 
@@ -341,7 +569,7 @@ __global__ __launch_bounds__(256) void int4_combine_kernel(uint16_t* out, const 
   *reinterpret_cast<u32x2*>(out + i) = r;
 }
 
-template <typename T, int G, int MT, Int4Epi EPI>
+template <typename T, int G, bool ZP, int MT, Int4Epi EPI>
 hipError_t launch_rows(Int4Args a, int tiles, hipStream_t s)
 {
   constexpr int NMAT = EPI == kInt4Glu ? 2 : 1, MAXW = MT == 1 ? 16 : 8;
@@ -356,7 +584,7 @@ hipError_t launch_rows(Int4Args a, int tiles, hipStream_t s)
   const int most = max(1, (int)(((1u << 31) / (64 * MAXW)) / a.row_groups));
   for (a.tile0 = 0; a.tile0 < tiles; a.tile0 += most) {
     const int now = min(most, tiles - a.tile0);
-    int4_rows_kernel<T, G, MT, EPI, MAXW>
+    int4_rows_kernel<T, G, ZP, MT, EPI, MAXW>
         <<<dim3((unsigned)now * a.row_groups), dim3(64 * waves), sizeof(f32x4) * waves * NMAT * MT * 64, s>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -364,18 +592,67 @@ hipError_t launch_rows(Int4Args a, int tiles, hipStream_t s)
   return hipSuccess;
 }
 
-template <typename T, Int4Epi EPI>
+// items: pairs (kInt4Glu) or tokens (kInt4Token)
+template <typename T, int G, bool ZP, int MR, Int4Epi EPI>
+hipError_t launch_vec(Int4Args a, int items, hipStream_t s)
+{
+  constexpr int RB = EPI == kInt4Glu ? kVecRows / 2 : kVecRows;
+  int waves = min(8, (a.K + 2047) / 2048);
+  if (EPI == kInt4Token) {
+    a.team = waves;
+    waves *= max(1, min(8 / waves, a.pairs.k));
+  }
+  // batches of a work-group: as many as leave the chip full once (16 waves a CU)
+  const int all = (a.R + RB - 1) / RB;
+  const long long full = 256 * (getenv("MXF") ? atoi(getenv("MXF")) : 16) / waves;
+  a.batches = (int)min((long long)kVecBatches, max(1LL, ((long long)all * items + full - 1) / full));
+  a.row_groups = (all + a.batches - 1) / a.batches;
+  const int most = max(1, (int)((1u << 22) / a.row_groups));  // a launch's threads are counted in 32 bits
+  for (a.tile0 = 0; a.tile0 < items; a.tile0 += most) {
+    int4_vec_kernel<T, G, ZP, MR, EPI><<<dim3((unsigned)min(most, items - a.tile0) * a.row_groups), 64 * waves,
+                                         sizeof(float) * waves * a.batches * kVecRows * MR, s>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+// rows: of a tile, 16, 32 or 64; or the few-row form's, 1, 2 or 4
+template <typename T, int G, bool ZP, Int4Epi EPI>
+hipError_t launch_tiles(const Int4Args& a, int rows, int tiles, hipStream_t s)
+{
+  if constexpr (EPI == kInt4Store) {
+    if (rows == 2) return launch_vec<T, G, ZP, 2, EPI>(a, tiles, s);
+    if (rows == 4) return launch_vec<T, G, ZP, 4, EPI>(a, tiles, s);
+  }
+  if constexpr (EPI != kInt4Pair) {
+    if (rows == 1) return launch_vec<T, G, ZP, 1, EPI>(a, tiles, s);
+  }
+  if constexpr (EPI != kInt4Token) {
+    if (rows == 16) return launch_rows<T, G, ZP, 1, EPI>(a, tiles, s);
+    if (rows == 32) return launch_rows<T, G, ZP, 2, EPI>(a, tiles, s);
+    return launch_rows<T, G, ZP, 4, EPI>(a, tiles, s);
+  }
+  return hipErrorInvalidValue;
+}
+template <typename T, bool ZP, Int4Epi EPI>
 hipError_t launch_group(const Int4Args& a, int group, int rows, int tiles, hipStream_t s)
 {
-#define MX_INT4_ROWS(G)                                                 \
-  (rows == 16 ? launch_rows<T, G, 1, EPI>(a, tiles, s)                  \
-              : rows == 32 ? launch_rows<T, G, 2, EPI>(a, tiles, s) : launch_rows<T, G, 4, EPI>(a, tiles, s))
   switch (group) {
-    case 32: return MX_INT4_ROWS(32);
-    case 64: return MX_INT4_ROWS(64);
-    default: return MX_INT4_ROWS(128);
+    case 32: return launch_tiles<T, 32, ZP, EPI>(a, rows, tiles, s);
+    case 64: return launch_tiles<T, 64, ZP, EPI>(a, rows, tiles, s);
+    default: return launch_tiles<T, 128, ZP, EPI>(a, rows, tiles, s);
   }
-#undef MX_INT4_ROWS
+}
+template <Int4Epi EPI>
+hipError_t launch_typed(const Int4Args& a, int group, int dtype, int rows, int tiles, hipStream_t s)
+{
+  const bool zp = a.w[0].z != nullptr;
+  if (dtype == 1)
+    return zp ? launch_group<__bf16, true, EPI>(a, group, rows, tiles, s)
+              : launch_group<__bf16, false, EPI>(a, group, rows, tiles, s);
+  return zp ? launch_group<_Float16, true, EPI>(a, group, rows, tiles, s)
+            : launch_group<_Float16, false, EPI>(a, group, rows, tiles, s);
 }
 
 int rows_of(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
@@ -384,18 +661,16 @@ template <Int4Epi EPI>
 hipError_t launch_routed(const Int4Args& a, int group, int dtype, hipStream_t s)
 {
   const int rows = int4_tile_rows(a.pairs.P, a.pairs.E);
-  const int tiles = a.tiles ? int4_max_tiles(a.pairs.P, a.pairs.E) : a.pairs.P;
-  return dtype == 1 ? launch_group<__bf16, EPI>(a, group, rows, tiles, s)
-                    : launch_group<_Float16, EPI>(a, group, rows, tiles, s);
+  return launch_typed<EPI>(a, group, dtype, rows, a.tiles ? int4_max_tiles(a.pairs.P, a.pairs.E) : a.pairs.P, s);
 }
 
 }  // namespace
 
 hipError_t launch_int4_gemm(const Int4Args& a, int group, int dtype, hipStream_t s)
 {
-  const int rows = rows_of(a.M), tiles = (int)(((long long)a.M + rows - 1) / rows);
-  return dtype == 1 ? launch_group<__bf16, kInt4Store>(a, group, rows, tiles, s)
-                    : launch_group<_Float16, kInt4Store>(a, group, rows, tiles, s);
+  const int rows = a.M <= kVecMost && a.K >= kVecMinK ? (a.M <= 2 ? a.M : 4) : rows_of(a.M);
+  const int tiles = (int)(((long long)a.M + rows - 1) / rows);
+  return launch_typed<kInt4Store>(a, group, dtype, rows, tiles, s);
 }
 
 int int4_tile_rows(int P, int E) { return rows_of(P / E); }
@@ -406,13 +681,19 @@ hipError_t launch_int4_route(const Int4Pairs& p, int4* tiles, int* n_tiles, int*
   return hipGetLastError();
 }
 
+bool int4_by_token(int N, int D, int F) { return N == 1 && min(D, F) >= kVecMinK; }
 hipError_t launch_int4_glu(const Int4Args& a, int group, int dtype, hipStream_t s)
 {
+  if (a.by_token) return launch_typed<kInt4Glu>(a, group, dtype, 1, a.pairs.P, s);
   return launch_routed<kInt4Glu>(a, group, dtype, s);
 }
 hipError_t launch_int4_pairs(const Int4Args& a, int group, int dtype, hipStream_t s)
 {
   return launch_routed<kInt4Pair>(a, group, dtype, s);
+}
+hipError_t launch_int4_token(const Int4Args& a, int group, int dtype, hipStream_t s)
+{
+  return launch_typed<kInt4Token>(a, group, dtype, 1, a.pairs.P / a.pairs.k, s);
 }
 
 hipError_t launch_int4_combine(void* out, const float* y, const float* topk_w, const Int4Pairs& p, int D, int dtype,

@@ -65,6 +65,8 @@ class Int4Experts:
             raise ValueError(f"w1 and w3 must be [E, F, D] and w2 [E, D, F], got {w1.shape}, {w3.shape} and {w2.shape}")
         if not w1.group == w3.group == w2.group:
             raise ValueError(f"the matrices must have one group size, got {w1.group}, {w3.group} and {w2.group}")
+        if any((w.zeros is None) != (w1.zeros is None) for w in (w3, w2)):
+            raise ValueError("zero points must be given for all three matrices or for none")
         if any(w.scales.dtype != w1.scales.dtype or w.packed.device != w1.packed.device for w in (w3, w2)):
             raise ValueError("the matrices must have scales of one type and lie on one device")
         self.w1, self.w3, self.w2 = w1, w3, w2

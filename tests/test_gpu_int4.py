@@ -72,6 +72,35 @@ def test_gemm(M, K, R, group, dtype):
             assert (err <= bound(xs, w, want, dt)).all(), (k, zeros, err.max())
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("K,R", [(1024, 8), (1152, 1), (2048, 13), (2176, 40), (7168, 100), (16384, 9), (20480, 19), (3584, 4100)])
+def test_gemm_long_rows(M, K, R):
+    """The lengths that one wave, a whole work-group and several rounds of one cover; rows past a batch."""
+    from lazylora_amd.int4 import int4_gemm
+    for dt, group, zeros in ((torch.bfloat16, 128, True), (torch.float16, 32, False), (torch.bfloat16, 64, True)):
+        gen = gen_of(M, K, R, group)
+        x = torch.randn(M, K, device="cuda", generator=gen).to(dt)
+        w = weight(gen, (), R, K, group, zeros, dt)
+        y = int4_gemm(x, w)
+        xs = x.double().cpu().numpy()
+        want = xs @ dense64(w).T
+        assert (np.abs(y.double().cpu().numpy() - want) <= bound(xs, w, want, dt)).all()
+
+
+def test_small_numbers_are_kept():
+    """Rows of x in the type's subnormal range, in every form of the product."""
+    from lazylora_amd.int4 import int4_gemm
+    for dt, tiny in ((torch.float16, 2.0 ** -24), (torch.float16, 2.0 ** -20), (torch.bfloat16, 2.0 ** -120)):
+        for M in (1, 3, 6, 20):
+            gen = gen_of(M)
+            x = (torch.randint(-3, 4, (M, 1024), device="cuda", generator=gen) * tiny).to(dt)
+            w = weight(gen, (), 24, 1024, 32, True, dt)
+            w.scales.copy_(torch.full_like(w.scales, 64.0))  # results in the normal range
+            want = x.double().cpu().numpy() @ dense64(w).T
+            err = np.abs(int4_gemm(x, w).double().cpu().numpy() - want)
+            assert (err <= torch.finfo(dt).eps * np.abs(want) + 1e-3 * np.abs(want).max()).all()
+
+
 def test_codes_are_exact():
     """Every code and zero point in every place of a group: one-hot rows give the weights themselves."""
     from lazylora_amd.int4 import Int4Weight, int4_gemm
@@ -112,7 +141,9 @@ ROUTED = [  # N, k, E, D, F, group, zeros, dtype, act
     (9, 8, 8, 128, 256, 64, False, "bf16", "situ"), (64, 1, 2, 96, 160, 32, True, "bf16", "swiglu"),
     (65, 1, 2, 96, 160, 32, False, "f16", "swiglu"), (100, 4, 5, 192, 64, 64, True, "bf16", "situ"),
     (300, 3, 70, 128, 128, 64, False, "f16", "swiglu"), (200, 2, 1200, 64, 64, 32, True, "bf16", "swiglu"),
-    (150, 2, 2, 128, 128, 128, False, "bf16", "swiglu"),
+    (150, 2, 2, 128, 128, 128, False, "bf16", "swiglu"), (1, 8, 12, 1024, 1152, 64, True, "bf16", "swiglu"),
+    (1, 3, 4, 2176, 1024, 128, False, "f16", "situ"), (1, 11, 16, 1024, 1024, 32, False, "bf16", "situ"),
+    (2, 8, 12, 1024, 1152, 64, True, "bf16", "swiglu"),
 ]
 
 
@@ -161,9 +192,12 @@ def test_same_expert_many_times():
     from lazylora_amd.int4 import int4_routed
     dt = torch.bfloat16
     gen = gen_of(9)
-    ex = layer(gen, 4, 128, 128, 64, True, dt)
     for N, k in ((1, 3), (20, 3), (33, 2), (90, 4)):
-        h = torch.randn(N, 128, device="cuda", generator=gen).to(dt)
+        if N == 1:
+            ex = layer(gen, 4, 1024, 1024, 64, True, dt)
+        else:
+            ex = layer(gen, 4, 128, 128, 64, True, dt)
+        h = torch.randn(N, ex.D, device="cuda", generator=gen).to(dt)
         idx = torch.full((N, k), 2, device="cuda")
         w = torch.rand(N, k, device="cuda", generator=gen)
         out = int4_routed(h, idx, w, ex)
@@ -259,6 +293,8 @@ def test_refusals():
         Int4Experts(ex.w1, ex.w3, weight(gen, (3,), 128, 64, 64, False, torch.bfloat16))
     with pytest.raises(ValueError):
         Int4Experts(w, w, w)
+    with pytest.raises(ValueError):
+        Int4Experts(ex.w1, ex.w3, weight(gen, (3,), 128, 64, 32, True, torch.bfloat16))
 
 
 def test_captured_and_replayed():
