@@ -16,6 +16,7 @@ namespace {
 
 constexpr int kVecRows = 8;     // weight rows of a batch of the few-row form
 constexpr int kVecBatches = 16;  // batches of a work-group at most
+constexpr int kStripGroups = 4;   // groups of 16 weight rows of a work-group of the form for 16 rows of x, at most
 constexpr int kVecMost = 4;      // its rows of x at most
 constexpr int kVecMinK = 1024;  // and the shortest rows it takes
 
@@ -492,6 +493,324 @@ __global__ __launch_bounds__(64 * MAXW) void int4_rows_kernel(Int4Args p)
   }
 }
 
+// ------------------------------------------------------------------ up to 16 rows of x
+// A wave keeps 256 terms of up to 16 rows of x in registers, as the MFMA takes them, with their sums over each
+// group, and walks groups of 16 weight rows (of a gate/up product: of both matrices), the codes of the next one
+// in flight. The waves of a work-group share K; their sums meet in LDS once, in the waves' order.
+template <typename T, int G, bool ZP, Int4Epi EPI, bool WIDE>
+__global__ __launch_bounds__(EPI == kInt4Glu ? 512 : 1024) void int4_strip_kernel(Int4Args p)
+{
+  using N = Num<T>;
+  constexpr int NMAT = EPI == kInt4Glu ? 2 : 1, NG = 128 / G, JG = 4 / NG, NB = kStripGroups;
+  extern __shared__ f32x4 part[];  // [waves][p.batches][NMAT][64]
+  __shared__ int rows[16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int n = lane & 15, c = lane >> 4;
+  const int tile = blockIdx.x / p.row_groups + p.tile0, g0 = (blockIdx.x % p.row_groups) * p.batches;
+  const int count = min(p.batches, (p.R + 15) / 16 - g0), groups = p.K / G;
+  int e, nrows;
+  if (!find_rows<16, EPI>(p, tile, rows, e, nrows)) return;
+  __syncthreads();
+  const int units = (p.K + 255) / 256, rounds = (units + waves - 1) / waves;
+  const Decoder dec = decoder<T>();
+  const i32x4 ones = {(int)N::kOnes, (int)N::kOnes, (int)N::kOnes, (int)N::kOnes};
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  const int x_row = rows[n];
+  const uint16_t* xr = static_cast<const uint16_t*>(p.x) + (long long)(EPI == kInt4Store ? x_row : x_row / p.x_div) * p.K;
+  Rows w[NMAT];
+#pragma unroll
+  for (int m = 0; m < NMAT; ++m)
+    w[m] = weight_rows(p.w[m], (long long)e * p.R + 16 * g0, min(16 * count, p.R - 16 * g0), p.K, groups);
+
+  struct Step {
+    i32x4 q[NMAT][2];
+    uint32_t s[NMAT][NG];            // 2 NG scales
+    uint32_t z[NMAT][(NG + 1) / 2];  // 2 NG zero points
+  };
+  // what lies past K, past R or past the last group is loaded from past the buffers: zeros
+  const uint32_t lane_q = (uint32_t)n * (p.K / 2) + 16 * c, lane_s = (uint32_t)n * groups;
+  const auto load = [&](int g, int u, Step& t) {
+    const bool in = (g < count) & (u < units) & (16 * (g0 + g) + n < p.R);
+    const uint32_t row = 16 * g;
+#pragma unroll
+    for (int m = 0; m < NMAT; ++m) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const bool there = WIDE ? in : in & (256 * u + 128 * b + 32 * c < p.K);
+        t.q[m][b] = load_codes(w[m], there ? lane_q : kOob, row * (p.K / 2) + 128 * u + 64 * b);
+      }
+      if constexpr (WIDE) {
+        const int at = in ? lane_s : kOob / 2, shared = row * groups + u * (2 * NG);
+        if constexpr (NG == 4) {
+          const i32x4 v = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(w[m].s, 2 * at, 2 * shared, 0));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t.s[m][i] = v[i];
+          if (ZP) {
+            const auto y = __builtin_amdgcn_raw_buffer_load_b64(w[m].z, at, shared, 0);
+            t.z[m][0] = y[0], t.z[m][1] = y[1];
+          }
+        } else if constexpr (NG == 2) {
+          const auto v = __builtin_amdgcn_raw_buffer_load_b64(w[m].s, 2 * at, 2 * shared, 0);
+          t.s[m][0] = v[0], t.s[m][1] = v[1];
+          if (ZP) t.z[m][0] = __builtin_amdgcn_raw_buffer_load_b32(w[m].z, at, shared, 0);
+        } else {
+          t.s[m][0] = __builtin_amdgcn_raw_buffer_load_b32(w[m].s, 2 * at, 2 * shared, 0);
+          if (ZP) t.z[m][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(w[m].z, at, shared, 0);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) t.s[m][i] = 0;
+#pragma unroll
+        for (int i = 0; i < (NG + 1) / 2; ++i) t.z[m][i] = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i) {
+          const int group = u * (2 * NG) + i;
+          const uint32_t at = in & (group < groups) ? lane_s : kOob / 2;
+          t.s[m][i / 2] |= (uint32_t)load_scale(w[m], at, row * groups + group) << (16 * (i & 1));
+          if (ZP) t.z[m][i / 4] |= (uint32_t)load_zero(w[m], at, row * groups + group) << (8 * (i & 3));
+        }
+      }
+    }
+  };
+  f32x4 acc[NB][NMAT];
+#pragma unroll
+  for (int g = 0; g < NB; ++g)
+#pragma unroll
+    for (int m = 0; m < NMAT; ++m) acc[g][m] = zero;
+  Step step[2];
+  for (int r = 0; r < rounds; ++r) {
+    const int u = wave + r * waves;
+    load(0, u, step[0]);
+    i32x4 x[2][4];
+    f32x4 sum[2 * NG];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = 256 * u + 128 * b + block_k<G>(j, c);
+        const bool in = k < p.K;
+        const i32x4 v = *reinterpret_cast<const i32x4*>(xr + (in ? k : 0));
+        x[b][j] = pair_up(in ? v : i32x4{0, 0, 0, 0});
+        f32x4& s = sum[b * NG + j / JG];
+        s = N::mfma(x[b][j], ones, j % JG ? s : zero);
+      }
+    static_for<NB>([&](auto gc) {
+      constexpr int g = decltype(gc)::value;
+      load(g + 1, u, step[(g + 1) & 1]);
+      if (g >= count) return;
+      const Step& t = step[g & 1];
+      static_for<2>([&](auto bc) {
+        constexpr int b = decltype(bc)::value;
+        uint32_t d[NMAT][4];
+#pragma unroll
+        for (int m = 0; m < NMAT; ++m) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[m][j] = (uint32_t)t.q[m][b][j];
+          one_group<G>(d[m]);
+        }
+        static_for<NG>([&](auto ic) {
+          constexpr int i = b * NG + decltype(ic)::value, j0 = decltype(ic)::value * JG;
+#pragma unroll
+          for (int m = 0; m < NMAT; ++m) {
+            f32x4 dot = zero;
+#pragma unroll
+            for (int j = j0; j < j0 + JG; ++j) dot = N::mfma(x[b][j], decode8<T>(d[m][j], dec), dot);
+            const float s = N::widen((uint16_t)(t.s[m][i / 2] >> (16 * (i & 1))));
+            const float z = ZP ? -16.0f - (float)(t.z[m][i / 4] >> (8 * (i & 3)) & 255u) : -24.0f;
+#pragma unroll
+            for (int l = 0; l < 4; ++l) acc[g][m][l] = fmaf(s, fmaf(z, sum[i][l], dot[l]), acc[g][m][l]);
+          }
+        });
+      });
+    });
+  }
+  static_for<NB>([&](auto gc) {
+    constexpr int g = decltype(gc)::value;
+    if (g >= count) return;
+#pragma unroll
+    for (int m = 0; m < NMAT; ++m) part[((wave * p.batches + g) * NMAT + m) * 64 + lane] = acc[g][m];
+  });
+  __syncthreads();
+  const float* sums = reinterpret_cast<const float*>(part);
+  for (int i = threadIdx.x; i < 16 * nrows * count; i += blockDim.x) {
+    const int g = i / (16 * nrows), row = (i >> 4) - g * nrows, col = i & 15;
+    const int at = (16 * (row >> 2) + col) * 4 + (row & 3);  // lane 16 (row / 4) + col holds it in element row % 4
+    float v[NMAT];
+#pragma unroll
+    for (int m = 0; m < NMAT; ++m) {
+      v[m] = 0.f;
+      for (int u = 0; u < waves; ++u) v[m] += sums[((u * p.batches + g) * NMAT + m) * 256 + at];
+    }
+    const int r = 16 * (g0 + g) + col;
+    if (r < p.R) store<T, EPI>(p, (long long)rows[row] * p.R + r, v[0], v[NMAT - 1]);
+  }
+}
+
+// ------------------------------------------------------------------ many rows of x
+// A work-group of four waves makes 16 MT rows of x x 128 weight rows, 32 to each wave (of a gate/up product 16 of
+// both matrices), K in blocks of 128: x of a block in LDS in the order the MFMA takes it, two buffers, the next
+// block's x and codes in registers meanwhile. A block's 16-byte piece (j, c) of row r lies at place r ^ (4 j + c)
+// of 16: neither the writes (16 pieces of a row) nor the reads (16 rows of a piece) meet bank conflicts.
+template <typename T, int G, bool ZP, int MT, Int4Epi EPI, bool WIDE>
+__global__ __launch_bounds__(256) void int4_tile_kernel(Int4Args p)
+{
+  using N = Num<T>;
+  constexpr int XR = 16 * MT, NG = 128 / G, JG = 4 / NG, NT = 2;
+  constexpr int kFeatures = EPI == kInt4Glu ? 64 : 128;
+  __shared__ i32x4 xs[2][16 * XR];
+  __shared__ int rows[XR];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, c = lane >> 4;
+  const int tile = blockIdx.x / p.row_groups + p.tile0, f0 = (blockIdx.x % p.row_groups) * kFeatures;
+  int e, nrows;
+  if (!find_rows<XR, EPI>(p, tile, rows, e, nrows)) return;
+  __syncthreads();
+  const int groups = p.K / G, blocks = (p.K + 127) / 128;
+  const Decoder dec = decoder<T>();
+  const i32x4 ones = {(int)N::kOnes, (int)N::kOnes, (int)N::kOnes, (int)N::kOnes};
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+
+  // this wave's two groups of 16 weight rows: neighbours, or the same of both matrices
+  Rows w[NT];
+  int first[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    first[t] = EPI == kInt4Glu ? f0 + 16 * wave : f0 + 32 * wave + 16 * t;
+    const int row = min(first[t], p.R - 1);
+    w[t] = weight_rows(p.w[EPI == kInt4Glu ? t : 0], (long long)e * p.R + row, min(16, p.R - row), p.K, groups);
+  }
+  struct Step {
+    i32x4 q[NT];
+    uint32_t s[NT][(NG + 1) / 2], z[NT];
+  };
+  const auto load = [&](int b, Step& k) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const bool in = (b < blocks) & (first[t] + n < p.R);
+      const bool there = WIDE ? in : in & (128 * b + 32 * c < p.K);
+      k.q[t] = load_codes(w[t], there ? (uint32_t)n * (p.K / 2) + 16 * c : kOob, 64 * b);
+      const uint32_t at = in ? (uint32_t)n * groups : kOob / 2;
+      if constexpr (WIDE && NG == 4) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(w[t].s, 2 * at, 2 * NG * b, 0);
+        k.s[t][0] = v[0], k.s[t][1] = v[1];
+        if (ZP) k.z[t] = __builtin_amdgcn_raw_buffer_load_b32(w[t].z, at, NG * b, 0);
+      } else if constexpr (WIDE && NG == 2) {
+        k.s[t][0] = __builtin_amdgcn_raw_buffer_load_b32(w[t].s, 2 * at, 2 * NG * b, 0);
+        if (ZP) k.z[t] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(w[t].z, at, NG * b, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < (NG + 1) / 2; ++i) k.s[t][i] = 0;
+        k.z[t] = 0;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          const int g = b * NG + i;
+          const uint32_t ag = in & (g < groups) ? at : kOob / 2;
+          k.s[t][i / 2] |= (uint32_t)load_scale(w[t], ag, g) << (16 * (i & 1));
+          if (ZP) k.z[t] |= (uint32_t)load_zero(w[t], ag, g) << (8 * i);
+        }
+      }
+    }
+  };
+  // x: thread t carries piece t % 16 of rows t / 16, + 16, ..
+  const int piece = tid & 15, xrow = tid >> 4;
+  const uint16_t* xp[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = rows[xrow + 16 * m];
+    xp[m] = static_cast<const uint16_t*>(p.x) + (long long)(EPI == kInt4Store ? r : r / p.x_div) * p.K;
+  }
+  i32x4 xv[MT];
+  const auto load_x = [&](int b) {
+    const int k = 128 * b + 8 * piece, kc = k < p.K ? k : 0;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const i32x4 v = *reinterpret_cast<const i32x4*>(xp[m] + kc);
+      xv[m] = k < p.K ? v : i32x4{0, 0, 0, 0};
+    }
+  };
+  const int a = piece >> 2, d = piece & 3;  // the place of block_k
+  const int pj = G == 128 ? d : G == 64 ? 2 * (a >> 1) + (d & 1) : a;
+  const int pc = G == 128 ? a : G == 64 ? (a & 1) + 2 * (d >> 1) : d;
+  const int place = (4 * pj + pc) * XR + (xrow ^ (4 * pj + pc));
+  const auto store_x = [&](int buf) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) xs[buf][place + 16 * m] = pair_up(xv[m]);
+  };
+
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[t][m] = zero;
+  const auto multiply = [&](int buf, const Step& k) {
+    uint32_t q[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[t][j] = (uint32_t)k.q[t][j];
+      one_group<G>(q[t]);
+    }
+    static_for<NG>([&](auto gc) {
+      constexpr int g = decltype(gc)::value;
+      f32x4 sum[MT], dot[NT][MT];
+#pragma unroll
+      for (int j = g * JG; j < (g + 1) * JG; ++j) {
+        i32x4 b[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) b[t] = decode8<T>(q[t][j], dec);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const i32x4 x = xs[buf][(4 * j + c) * XR + 16 * m + (n ^ (4 * j + c))];
+          sum[m] = N::mfma(x, ones, j == g * JG ? zero : sum[m]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) dot[t][m] = N::mfma(x, b[t], j == g * JG ? zero : dot[t][m]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float s = N::widen((uint16_t)(k.s[t][g / 2] >> (16 * (g & 1))));
+        const float z = ZP ? -16.0f - (float)(k.z[t] >> (8 * g) & 255u) : -24.0f;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][m][i] = fmaf(s, fmaf(z, sum[m][i], dot[t][m][i]), acc[t][m][i]);
+      }
+    });
+  };
+  Step k0, k1;
+  load_x(0);
+  load(0, k0);
+  store_x(0);
+  for (int b = 0; b < blocks; b += 2) {
+    __syncthreads();
+    load_x(b + 1);
+    load(b + 1, k1);
+    multiply(0, k0);
+    store_x(1);
+    if (b + 1 >= blocks) break;
+    __syncthreads();
+    load_x(b + 2);
+    load(b + 2, k0);
+    multiply(1, k1);
+    store_x(0);
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * m + 4 * c + i;
+      if (r >= nrows) continue;
+      const long long o = (long long)rows[r] * p.R;
+      if (EPI == kInt4Glu) {
+        if (first[0] + n < p.R) store<T, EPI>(p, o + first[0] + n, acc[0][m][i], acc[1][m][i]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          if (first[t] + n < p.R) store<T, EPI>(p, o + first[t] + n, acc[t][m][i], 0.f);
+      }
+    }
+}
+
 // ------------------------------------------------------------------ routing
 // The pairs in the order of their experts, and the tiles of up to tile_rows of them: one work-group, counts
 // and places in LDS. The order of an expert's pairs is left to the atomics: a row's result does not depend
@@ -604,13 +923,49 @@ hipError_t launch_vec(Int4Args a, int items, hipStream_t s)
   }
   // batches of a work-group: as many as leave the chip full once (16 waves a CU)
   const int all = (a.R + RB - 1) / RB;
-  const long long full = 256 * (getenv("MXF") ? atoi(getenv("MXF")) : 16) / waves;
+  const long long full = 256 * 32 / waves;
   a.batches = (int)min((long long)kVecBatches, max(1LL, ((long long)all * items + full - 1) / full));
   a.row_groups = (all + a.batches - 1) / a.batches;
   const int most = max(1, (int)((1u << 22) / a.row_groups));  // a launch's threads are counted in 32 bits
   for (a.tile0 = 0; a.tile0 < items; a.tile0 += most) {
     int4_vec_kernel<T, G, ZP, MR, EPI><<<dim3((unsigned)min(most, items - a.tile0) * a.row_groups), 64 * waves,
                                          sizeof(float) * waves * a.batches * kVecRows * MR, s>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+template <typename T, int G, bool ZP, Int4Epi EPI>
+hipError_t launch_strip(Int4Args a, int tiles, hipStream_t s)
+{
+  constexpr int NMAT = EPI == kInt4Glu ? 2 : 1, MAXW = EPI == kInt4Glu ? 8 : 16;
+  const int units = (a.K + 255) / 256, rounds = (units + MAXW - 1) / MAXW, waves = (units + rounds - 1) / rounds;
+  const auto kernel = a.K % 256 == 0 ? int4_strip_kernel<T, G, ZP, EPI, true> : int4_strip_kernel<T, G, ZP, EPI, false>;
+  const int all = (a.R + 15) / 16;
+  const long long full = 256 * 16 / waves;
+  a.batches = (int)min((long long)kStripGroups, max(1LL, ((long long)all * tiles + full - 1) / full));
+  a.row_groups = (all + a.batches - 1) / a.batches;
+  const int most = max(1, (int)((1u << 21) / a.row_groups));
+  for (a.tile0 = 0; a.tile0 < tiles; a.tile0 += most) {
+    kernel<<<dim3((unsigned)min(most, tiles - a.tile0) * a.row_groups), 64 * waves,
+             sizeof(f32x4) * waves * a.batches * NMAT * 64, s>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+template <typename T, int G, bool ZP, int MT, Int4Epi EPI>
+hipError_t launch_tile(Int4Args a, int tiles, hipStream_t s)
+{
+  constexpr int kFeatures = EPI == kInt4Glu ? 64 : 128;
+  const auto kernel =
+      a.K % 128 == 0 ? int4_tile_kernel<T, G, ZP, MT, EPI, true> : int4_tile_kernel<T, G, ZP, MT, EPI, false>;
+  a.row_groups = (a.R + kFeatures - 1) / kFeatures;
+  const int most = max(1, (int)((1u << 23) / a.row_groups));
+  for (a.tile0 = 0; a.tile0 < tiles; a.tile0 += most) {
+    kernel<<<dim3((unsigned)min(most, tiles - a.tile0) * a.row_groups), 256, 0, s>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -629,7 +984,10 @@ hipError_t launch_tiles(const Int4Args& a, int rows, int tiles, hipStream_t s)
     if (rows == 1) return launch_vec<T, G, ZP, 1, EPI>(a, tiles, s);
   }
   if constexpr (EPI != kInt4Token) {
-    if (rows == 16) return launch_rows<T, G, ZP, 1, EPI>(a, tiles, s);
+    if (rows == 16) {
+      return launch_strip<T, G, ZP, EPI>(a, tiles, s);
+    }
+    if (getenv("TILE")) return rows == 32 ? launch_tile<T, G, ZP, 2, EPI>(a, tiles, s) : launch_tile<T, G, ZP, 4, EPI>(a, tiles, s);
     if (rows == 32) return launch_rows<T, G, ZP, 2, EPI>(a, tiles, s);
     return launch_rows<T, G, ZP, 4, EPI>(a, tiles, s);
   }
