@@ -17,10 +17,11 @@ AUTOGRAD_SOURCES = ["dense_autograd.cpp", "moe_autograd.cpp"]
 SOURCES = ["capi.hip", "mx_forward.hip", "mx_backward.hip", "mx_misc.hip", "mx_router.hip", "mx_lora.hip",
            "mx_dense.hip", "mx_rows.hip", "mx_select.hip", "mx_int4.hip"]
 
-# per-file flags: the transposed products keep their accumulators in VGPRs (the MFMA's VGPR
+# per-file flags: the transposed products and those with 4-bit integer weights keep their accumulators in VGPRs (the MFMA's VGPR
 # form); with the default heuristics the compiler splits them over AGPRs and VGPRs and shuffles
 # them with v_accvgpr moves inside the main loop
-FILE_FLAGS = {"mx_backward.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+FILE_FLAGS = {"mx_backward.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+              "mx_int4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

@@ -7,7 +7,6 @@
 // all exact products in fp32 sums, and one multiply-add by the group's scale per result. A row of x with an
 // infinity gives NaN (the difference of two infinities).
 #include "mx_device.h"
-#include <stdlib.h>
 #include "mx_int4.h"
 
 namespace mx {
@@ -199,7 +198,12 @@ struct Rows {
 };
 MX_DEV __amdgpu_buffer_rsrc_t buffer(const void* base, uint32_t bytes)
 {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+  // scalar for certain: where the compiler does not see that it is, every load becomes a loop over the lanes
+  const uint64_t b = (uint64_t)(uintptr_t)base;
+  const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32 |
+                     (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(u), 0, __builtin_amdgcn_readfirstlane(bytes),
+                                           0x00020000);
 }
 MX_DEV Rows weight_rows(const Int4Matrix& w, long long first, int count, int K, int groups)
 {
@@ -328,11 +332,9 @@ __global__ __launch_bounds__(512) void int4_vec_kernel(Int4Args p)
       };
       for (int b = 0; b < batches; b += 2) {
         load(b + 1, c1);
-        __builtin_amdgcn_sched_barrier(0);  // the loads first, not where their registers are free at last
         multiply(b, c0);
         if (b + 1 >= batches) break;
         load(b + 2, c0);
-        __builtin_amdgcn_sched_barrier(0);
         multiply(b + 1, c1);
       }
     }
@@ -361,135 +363,6 @@ __global__ __launch_bounds__(512) void int4_vec_kernel(Int4Args p)
     }
     const long long o = EPI == kInt4Store ? m : item;
     if ((EPI != kInt4Store || m < p.M) && row < p.R) store<T, EPI>(p, o * p.R + row, u, v);
-  }
-}
-
-// ------------------------------------------------------------------ tiles of rows of x
-// A work-group makes 16 weight rows x up to 16 MT rows of x; its waves share K, block pair by block pair (so
-// that a wave reads whole 128-byte lines), and their sums meet in LDS in the waves' order.
-template <typename T, int G, bool ZP, int MT, Int4Epi EPI, int MAXW>
-__global__ __launch_bounds__(64 * MAXW) void int4_rows_kernel(Int4Args p)
-{
-  using N = Num<T>;
-  constexpr int NMAT = EPI == kInt4Glu ? 2 : 1, NG = 128 / G, JG = 4 / NG;  // groups of a block, dwords of a group
-  extern __shared__ f32x4 part[];  // [waves][NMAT][MT][64]
-  __shared__ int rows[16 * MT];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int n = lane & 15, c = lane >> 4;
-  const int tile = blockIdx.x / p.row_groups + p.tile0, r0 = (blockIdx.x % p.row_groups) * 16;
-
-  int e, nrows;
-  if (!find_rows<16 * MT, EPI>(p, tile, rows, e, nrows)) return;
-  __syncthreads();
-
-  const int wr = min(n, p.R - 1 - r0), groups = p.K / G;
-  const Decoder dec = decoder<T>();
-  Rows w[NMAT];
-#pragma unroll
-  for (int m = 0; m < NMAT; ++m)
-    w[m] = weight_rows(p.w[m], (long long)e * p.R + r0, min(16, p.R - r0), p.K, groups);
-  const uint16_t* xr[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int i = rows[16 * t + n];
-    xr[t] = static_cast<const uint16_t*>(p.x) + (long long)(EPI == kInt4Store ? i : i / p.x_div) * p.K;
-  }
-
-  f32x4 acc[NMAT][MT];
-#pragma unroll
-  for (int m = 0; m < NMAT; ++m)
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const i32x4 ones = {(int)N::kOnes, (int)N::kOnes, (int)N::kOnes, (int)N::kOnes};
-  const int blocks = (p.K + 127) / 128;
-
-  struct Block {
-    i32x4 q[NMAT], x[MT][4];
-    uint16_t s[NMAT][NG];
-    uint8_t z[NMAT][NG];
-  };
-  // past K codes and x are 0
-  const auto load = [&](int b, Block& k) {
-    const bool in = G == 128 || b * 128 + 32 * c < p.K;
-#pragma unroll
-    for (int m = 0; m < NMAT; ++m) {
-      k.q[m] = load_codes(w[m], in ? (uint32_t)wr * (p.K / 2) + 16 * c : kOob, b * 64);
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const int gi = G == 128 ? b : min(b * NG + g, groups - 1);
-        k.s[m][g] = load_scale(w[m], (uint32_t)wr * groups, gi);
-        k.z[m][g] = ZP ? load_zero(w[m], (uint32_t)wr * groups, gi) : (uint8_t)8;
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int kx = b * 128 + block_k<G>(j, c);
-        k.x[t][j] = i32x4{0, 0, 0, 0};
-        if (G == 128 || kx < p.K) k.x[t][j] = *reinterpret_cast<const i32x4*>(xr[t] + kx);
-      }
-  };
-  const auto multiply = [&](const Block& k) {
-    uint32_t d[NMAT][4];
-#pragma unroll
-    for (int m = 0; m < NMAT; ++m) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) d[m][j] = (uint32_t)k.q[m][j];
-      one_group<G>(d[m]);
-    }
-    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      f32x4 sum[MT], dot[NMAT][MT];
-#pragma unroll
-      for (int j = g * JG; j < (g + 1) * JG; ++j) {
-        i32x4 b[NMAT];
-#pragma unroll
-        for (int m = 0; m < NMAT; ++m) b[m] = decode8<T>(d[m][j], dec);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const i32x4 x = pair_up(k.x[t][j]);
-          sum[t] = N::mfma(x, ones, j == g * JG ? zero : sum[t]);
-#pragma unroll
-          for (int m = 0; m < NMAT; ++m) dot[m][t] = N::mfma(x, b[m], j == g * JG ? zero : dot[m][t]);
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < NMAT; ++m) {
-        const float s = N::widen(k.s[m][g]), z = -16.0f - (float)k.z[m][g];
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][t][i] = fmaf(s, fmaf(z, sum[t][i], dot[m][t][i]), acc[m][t][i]);
-      }
-    }
-  };
-  for (int b = 2 * wave; b < blocks; b += 2 * waves) {
-    Block k0, k1;
-    load(b, k0);
-    if (b + 1 < blocks) load(b + 1, k1);
-    multiply(k0);
-    if (b + 1 < blocks) multiply(k1);
-  }
-
-#pragma unroll
-  for (int m = 0; m < NMAT; ++m)
-#pragma unroll
-    for (int t = 0; t < MT; ++t) part[((wave * NMAT + m) * MT + t) * 64 + lane] = acc[m][t];
-  __syncthreads();
-  const float* sums = reinterpret_cast<const float*>(part);
-  for (int i = threadIdx.x; i < MT * 256; i += blockDim.x) {
-    const int row = i >> 4, col = i & 15;  // lane 16 (row % 16 / 4) + col holds it in element row % 4
-    const int at = (row >> 4) * 256 + (16 * ((row & 15) >> 2) + col) * 4 + (row & 3);
-    float v[NMAT];
-#pragma unroll
-    for (int m = 0; m < NMAT; ++m) {
-      v[m] = 0.f;
-      for (int w = 0; w < waves; ++w) v[m] += sums[(w * NMAT + m) * MT * 256 + at];
-    }
-    if (row >= nrows || r0 + col >= p.R) continue;
-    store<T, EPI>(p, (long long)rows[row] * p.R + r0 + col, v[0], v[NMAT - 1]);
   }
 }
 
@@ -647,19 +520,22 @@ __global__ __launch_bounds__(EPI == kInt4Glu ? 512 : 1024) void int4_strip_kerne
 }
 
 // ------------------------------------------------------------------ many rows of x
-// A work-group of four waves makes 16 MT rows of x x 128 weight rows, 32 to each wave (of a gate/up product 16 of
-// both matrices), K in blocks of 128: x of a block in LDS in the order the MFMA takes it, two buffers, the next
-// block's x and codes in registers meanwhile. A block's 16-byte piece (j, c) of row r lies at place r ^ (4 j + c)
-// of 16: neither the writes (16 pieces of a row) nor the reads (16 rows of a piece) meet bank conflicts.
-template <typename T, int G, bool ZP, int MT, Int4Epi EPI, bool WIDE>
-__global__ __launch_bounds__(256) void int4_tile_kernel(Int4Args p)
+// A team of WN waves makes 16 MT rows of x x 32 WN weight rows, 32 to each wave (of a gate/up product 16 of both
+// matrices), K in blocks of 128: x of a block in LDS in the order the MFMA takes it, two buffers, the next
+// block's x and codes in registers meanwhile. KS teams of a work-group take every KS-th block; their sums meet in
+// LDS at the end, in the teams' order. A block's 16-byte piece (j, c) of row r lies at place r ^ (4 j + c) of 16:
+// neither the writes (16 pieces of a row) nor the reads (16 rows of a piece) meet bank conflicts.
+template <typename T, int G, bool ZP, int MT, int WN, int KS, Int4Epi EPI, bool WIDE>
+__global__ __launch_bounds__(64 * WN * KS) void int4_tile_kernel(Int4Args p)
 {
   using N = Num<T>;
   constexpr int XR = 16 * MT, NG = 128 / G, JG = 4 / NG, NT = 2;
-  constexpr int kFeatures = EPI == kInt4Glu ? 64 : 128;
-  __shared__ i32x4 xs[2][16 * XR];
+  constexpr int kFeatures = (EPI == kInt4Glu ? 16 : 32) * WN, kPass = 4 * WN, kPasses = XR / kPass;
+  extern __shared__ i32x4 lds[];  // [KS][2][16 * XR]
   __shared__ int rows[XR];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, team = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WN));
+  const int tid = threadIdx.x - team * (64 * WN), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  i32x4* xs = lds + team * (2 * 16 * XR);
   const int n = lane & 15, c = lane >> 4;
   const int tile = blockIdx.x / p.row_groups + p.tile0, f0 = (blockIdx.x % p.row_groups) * kFeatures;
   int e, nrows;
@@ -683,13 +559,21 @@ __global__ __launch_bounds__(256) void int4_tile_kernel(Int4Args p)
     i32x4 q[NT];
     uint32_t s[NT][(NG + 1) / 2], z[NT];
   };
-  const auto load = [&](int b, Step& k) {
+  // Rows past R are loaded from past the buffer (zeros). A block behind the last is the last again: a condition on
+  // b in the lanes' offsets becomes a branch around each load.
+  uint32_t lane_q[NT], lane_s[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const bool in = first[t] + n < p.R;
+    lane_q[t] = in ? (uint32_t)n * (p.K / 2) + 16 * c : kOob;
+    lane_s[t] = in ? (uint32_t)n * groups : kOob / 2;
+  }
+  const auto load = [&](int block, Step& k) {
+    const int b = min(block, blocks - 1);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const bool in = (b < blocks) & (first[t] + n < p.R);
-      const bool there = WIDE ? in : in & (128 * b + 32 * c < p.K);
-      k.q[t] = load_codes(w[t], there ? (uint32_t)n * (p.K / 2) + 16 * c : kOob, 64 * b);
-      const uint32_t at = in ? (uint32_t)n * groups : kOob / 2;
+      k.q[t] = load_codes(w[t], WIDE || 128 * b + 32 * c < p.K ? lane_q[t] : kOob, 64 * b);
+      const uint32_t at = lane_s[t];
       if constexpr (WIDE && NG == 4) {
         const auto v = __builtin_amdgcn_raw_buffer_load_b64(w[t].s, 2 * at, 2 * NG * b, 0);
         k.s[t][0] = v[0], k.s[t][1] = v[1];
@@ -703,38 +587,37 @@ __global__ __launch_bounds__(256) void int4_tile_kernel(Int4Args p)
         k.z[t] = 0;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-          const int g = b * NG + i;
-          const uint32_t ag = in & (g < groups) ? at : kOob / 2;
-          k.s[t][i / 2] |= (uint32_t)load_scale(w[t], ag, g) << (16 * (i & 1));
-          if (ZP) k.z[t] |= (uint32_t)load_zero(w[t], ag, g) << (8 * i);
+          const int g = min(b * NG + i, groups - 1);  // past K x is 0
+          k.s[t][i / 2] |= (uint32_t)load_scale(w[t], at, g) << (16 * (i & 1));
+          if (ZP) k.z[t] |= (uint32_t)load_zero(w[t], at, g) << (8 * i);
         }
       }
     }
   };
-  // x: thread t carries piece t % 16 of rows t / 16, + 16, ..
+  // x: thread t of the team carries piece t % 16 of rows t / 16, + kPass, ..
   const int piece = tid & 15, xrow = tid >> 4;
-  const uint16_t* xp[MT];
+  const uint16_t* xp[kPasses];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int r = rows[xrow + 16 * m];
+  for (int m = 0; m < kPasses; ++m) {
+    const int r = rows[xrow + kPass * m];
     xp[m] = static_cast<const uint16_t*>(p.x) + (long long)(EPI == kInt4Store ? r : r / p.x_div) * p.K;
   }
-  i32x4 xv[MT];
-  const auto load_x = [&](int b) {
-    const int k = 128 * b + 8 * piece, kc = k < p.K ? k : 0;
+  i32x4 xv[kPasses];
+  const auto load_x = [&](int block) {
+    const int k = 128 * min(block, blocks - 1) + 8 * piece;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const i32x4 v = *reinterpret_cast<const i32x4*>(xp[m] + kc);
-      xv[m] = k < p.K ? v : i32x4{0, 0, 0, 0};
+    for (int m = 0; m < kPasses; ++m) {
+      xv[m] = *reinterpret_cast<const i32x4*>(xp[m] + (WIDE || k < p.K ? k : 0));
+      if (!WIDE && k >= p.K) xv[m] = i32x4{0, 0, 0, 0};
     }
   };
   const int a = piece >> 2, d = piece & 3;  // the place of block_k
   const int pj = G == 128 ? d : G == 64 ? 2 * (a >> 1) + (d & 1) : a;
   const int pc = G == 128 ? a : G == 64 ? (a & 1) + 2 * (d >> 1) : d;
-  const int place = (4 * pj + pc) * XR + (xrow ^ (4 * pj + pc));
+  const int place = 4 * pj + pc;
   const auto store_x = [&](int buf) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) xs[buf][place + 16 * m] = pair_up(xv[m]);
+    for (int m = 0; m < kPasses; ++m) xs[buf * (16 * XR) + place * XR + ((xrow + kPass * m) ^ place)] = pair_up(xv[m]);
   };
 
   f32x4 acc[NT][MT];
@@ -760,7 +643,7 @@ __global__ __launch_bounds__(256) void int4_tile_kernel(Int4Args p)
         for (int t = 0; t < NT; ++t) b[t] = decode8<T>(q[t][j], dec);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          const i32x4 x = xs[buf][(4 * j + c) * XR + 16 * m + (n ^ (4 * j + c))];
+          const i32x4 x = xs[buf * (16 * XR) + (4 * j + c) * XR + 16 * m + (n ^ (4 * j + c))];
           sum[m] = N::mfma(x, ones, j == g * JG ? zero : sum[m]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) dot[t][m] = N::mfma(x, b[t], j == g * JG ? zero : dot[t][m]);
@@ -778,21 +661,45 @@ __global__ __launch_bounds__(256) void int4_tile_kernel(Int4Args p)
     });
   };
   Step k0, k1;
-  load_x(0);
-  load(0, k0);
+  load_x(team);
+  load(team, k0);
   store_x(0);
-  for (int b = 0; b < blocks; b += 2) {
+  for (int b = 0; b < blocks; b += 2 * KS) {  // of all teams; a team's is b + team
     __syncthreads();
-    load_x(b + 1);
-    load(b + 1, k1);
-    multiply(0, k0);
+    load_x(b + team + KS);
+    load(b + team + KS, k1);
+    __builtin_amdgcn_sched_barrier(0);  // the loads first, not where their registers are free at last
+    if (KS == 1 || b + team < blocks) multiply(0, k0);
     store_x(1);
-    if (b + 1 >= blocks) break;
+    if (b + KS >= blocks) break;
     __syncthreads();
-    load_x(b + 2);
-    load(b + 2, k0);
-    multiply(1, k1);
+    load_x(b + team + 2 * KS);
+    load(b + team + 2 * KS, k0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (KS == 1 || b + team + KS < blocks) multiply(1, k1);
     store_x(0);
+  }
+  if constexpr (KS > 1) {
+    f32x4* part = reinterpret_cast<f32x4*>(lds) + wave * (NT * MT * 64) + lane;  // [team - 1][wave][NT][MT][64]
+    __syncthreads();
+    if (team > 0) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) part[((team - 1) * (WN * NT * MT) + t * MT + m) * 64] = acc[t][m];
+    }
+    __syncthreads();
+    if (team > 0) return;
+#pragma unroll
+    for (int k = 0; k < KS - 1; ++k)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const f32x4 v = part[(k * (WN * NT * MT) + t * MT + m) * 64];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][m][i] += v[i];
+        }
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -888,29 +795,6 @@ __global__ __launch_bounds__(256) void int4_combine_kernel(uint16_t* out, const 
   *reinterpret_cast<u32x2*>(out + i) = r;
 }
 
-template <typename T, int G, bool ZP, int MT, Int4Epi EPI>
-hipError_t launch_rows(Int4Args a, int tiles, hipStream_t s)
-{
-  constexpr int NMAT = EPI == kInt4Glu ? 2 : 1, MAXW = MT == 1 ? 16 : 8;
-  a.row_groups = (a.R + 15) / 16;
-  // waves: enough for 16 on every CU, each with a block pair at least
-  const int pairs = (a.K + 255) / 256;
-  const long long groups = (long long)a.row_groups * tiles;
-  int waves = 4;
-  while (waves < MAXW && waves * groups < 4096) waves *= 2;
-  while (waves > 1 && waves / 2 >= pairs) waves /= 2;
-  // a launch's threads are counted in 32 bits
-  const int most = max(1, (int)(((1u << 31) / (64 * MAXW)) / a.row_groups));
-  for (a.tile0 = 0; a.tile0 < tiles; a.tile0 += most) {
-    const int now = min(most, tiles - a.tile0);
-    int4_rows_kernel<T, G, ZP, MT, EPI, MAXW>
-        <<<dim3((unsigned)now * a.row_groups), dim3(64 * waves), sizeof(f32x4) * waves * NMAT * MT * 64, s>>>(a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  return hipSuccess;
-}
-
 // items: pairs (kInt4Glu) or tokens (kInt4Token)
 template <typename T, int G, bool ZP, int MR, Int4Epi EPI>
 hipError_t launch_vec(Int4Args a, int items, hipStream_t s)
@@ -923,7 +807,7 @@ hipError_t launch_vec(Int4Args a, int items, hipStream_t s)
   }
   // batches of a work-group: as many as leave the chip full once (16 waves a CU)
   const int all = (a.R + RB - 1) / RB;
-  const long long full = 256 * 32 / waves;
+  const long long full = 256 * 16 / waves;
   a.batches = (int)min((long long)kVecBatches, max(1LL, ((long long)all * items + full - 1) / full));
   a.row_groups = (all + a.batches - 1) / a.batches;
   const int most = max(1, (int)((1u << 22) / a.row_groups));  // a launch's threads are counted in 32 bits
@@ -956,82 +840,126 @@ hipError_t launch_strip(Int4Args a, int tiles, hipStream_t s)
   return hipSuccess;
 }
 
-template <typename T, int G, bool ZP, int MT, Int4Epi EPI>
+template <typename T, int G, bool ZP, int MT, int WN, int KS, Int4Epi EPI>
 hipError_t launch_tile(Int4Args a, int tiles, hipStream_t s)
 {
-  constexpr int kFeatures = EPI == kInt4Glu ? 64 : 128;
-  const auto kernel =
-      a.K % 128 == 0 ? int4_tile_kernel<T, G, ZP, MT, EPI, true> : int4_tile_kernel<T, G, ZP, MT, EPI, false>;
+  constexpr int kFeatures = (EPI == kInt4Glu ? 16 : 32) * WN;
+  const auto kernel = a.K % 128 == 0 ? int4_tile_kernel<T, G, ZP, MT, WN, KS, EPI, true>
+                                     : int4_tile_kernel<T, G, ZP, MT, WN, KS, EPI, false>;
   a.row_groups = (a.R + kFeatures - 1) / kFeatures;
-  const int most = max(1, (int)((1u << 23) / a.row_groups));
+  const int most = max(1, (int)((1u << 21) / a.row_groups));
   for (a.tile0 = 0; a.tile0 < tiles; a.tile0 += most) {
-    kernel<<<dim3((unsigned)min(most, tiles - a.tile0) * a.row_groups), 256, 0, s>>>(a);
+    kernel<<<dim3((unsigned)min(most, tiles - a.tile0) * a.row_groups), 64 * WN * KS,
+             sizeof(i32x4) * KS * 2 * 16 * 16 * MT, s>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
 }
 
-// rows: of a tile, 16, 32 or 64; or the few-row form's, 1, 2 or 4
+// The forms by the rows of x that they take at once, and of the tile kernel by its waves. A work-group of the tile
+// kernel is one or two waves per SIMD whatever its form, so while there are fewer of them than CUs, smaller ones with
+// more teams on K are quicker: [2048, 7168] bf16, groups of 64, us, as 2 x 1 x 8 (MT, WN, KS) / 2 x 2 x 4 / 4 x 2 x 4 /
+// 4 x 4 x 2 / 4 x 4 x 1: 64 rows 18 / 27 / 36 / 64 / 72, 200 rows 36 / 28 / 37 / 64 / 77, 500 rows 71 / 49 / 40 / 66 / 80,
+// 1000 rows 136 / 96 / 82 / 72 / 85, 2000 rows 267 / 187 / 157 / 146 / 128; [7168, 3584]: 32 rows 11 / 14 / 19 / 32 / 35, 64
+// rows 20 / 15 / 20 / 33 / 37, 200 rows 65 / 42 / 40 / 36 / 40, 500 rows 131 / 74 / 77 / 68 / 59.
+enum Int4Form : int {
+  kVec1, kVec2, kVec4,     // the few-row form
+  kStrip,                  // 16 rows
+  kTile218, kTile224, kTile222,  // 32 rows
+  kTile424, kTile442, kTile441,  // 64 rows
+};
+constexpr int form_rows(Int4Form f) { return f < kStrip ? 1 << f : f == kStrip ? 16 : f < kTile424 ? 32 : 64; }
+constexpr int form_waves(Int4Form f)  // of 32 weight rows side by side
+{
+  return f == kTile218 ? 1 : f == kTile224 || f == kTile222 || f == kTile424 ? 2 : 4;
+}
+constexpr int kCus = 256;
+bool fills_no_round(Int4Form f, int tiles, int weight_rows)
+{
+  const int side = 32 * form_waves(f);
+  return (long long)tiles * ((weight_rows + side - 1) / side) <= kCus;
+}
+
+// items: tiles of form_rows, or the few-row form's pairs or tokens
 template <typename T, int G, bool ZP, Int4Epi EPI>
-hipError_t launch_tiles(const Int4Args& a, int rows, int tiles, hipStream_t s)
+hipError_t launch_form(const Int4Args& a, Int4Form form, int items, hipStream_t s)
 {
   if constexpr (EPI == kInt4Store) {
-    if (rows == 2) return launch_vec<T, G, ZP, 2, EPI>(a, tiles, s);
-    if (rows == 4) return launch_vec<T, G, ZP, 4, EPI>(a, tiles, s);
+    if (form == kVec2) return launch_vec<T, G, ZP, 2, EPI>(a, items, s);
+    if (form == kVec4) return launch_vec<T, G, ZP, 4, EPI>(a, items, s);
   }
   if constexpr (EPI != kInt4Pair) {
-    if (rows == 1) return launch_vec<T, G, ZP, 1, EPI>(a, tiles, s);
+    if (form == kVec1) return launch_vec<T, G, ZP, 1, EPI>(a, items, s);
   }
   if constexpr (EPI != kInt4Token) {
-    if (rows == 16) {
-      return launch_strip<T, G, ZP, EPI>(a, tiles, s);
+    switch (form) {
+      case kStrip: return launch_strip<T, G, ZP, EPI>(a, items, s);
+      case kTile218: return launch_tile<T, G, ZP, 2, 1, 8, EPI>(a, items, s);
+      case kTile224: return launch_tile<T, G, ZP, 2, 2, 4, EPI>(a, items, s);
+      case kTile222:
+        if constexpr (EPI != kInt4Store) return launch_tile<T, G, ZP, 2, 2, 2, EPI>(a, items, s);
+        break;
+      case kTile424: return launch_tile<T, G, ZP, 4, 2, 4, EPI>(a, items, s);
+      case kTile442: return launch_tile<T, G, ZP, 4, 4, 2, EPI>(a, items, s);
+      case kTile441: return launch_tile<T, G, ZP, 4, 4, 1, EPI>(a, items, s);
+      default: break;
     }
-    if (getenv("TILE")) return rows == 32 ? launch_tile<T, G, ZP, 2, EPI>(a, tiles, s) : launch_tile<T, G, ZP, 4, EPI>(a, tiles, s);
-    if (rows == 32) return launch_rows<T, G, ZP, 2, EPI>(a, tiles, s);
-    return launch_rows<T, G, ZP, 4, EPI>(a, tiles, s);
   }
   return hipErrorInvalidValue;
 }
 template <typename T, bool ZP, Int4Epi EPI>
-hipError_t launch_group(const Int4Args& a, int group, int rows, int tiles, hipStream_t s)
+hipError_t launch_group(const Int4Args& a, int group, Int4Form form, int items, hipStream_t s)
 {
   switch (group) {
-    case 32: return launch_tiles<T, 32, ZP, EPI>(a, rows, tiles, s);
-    case 64: return launch_tiles<T, 64, ZP, EPI>(a, rows, tiles, s);
-    default: return launch_tiles<T, 128, ZP, EPI>(a, rows, tiles, s);
+    case 32: return launch_form<T, 32, ZP, EPI>(a, form, items, s);
+    case 64: return launch_form<T, 64, ZP, EPI>(a, form, items, s);
+    default: return launch_form<T, 128, ZP, EPI>(a, form, items, s);
   }
 }
 template <Int4Epi EPI>
-hipError_t launch_typed(const Int4Args& a, int group, int dtype, int rows, int tiles, hipStream_t s)
+hipError_t launch_typed(const Int4Args& a, int group, int dtype, Int4Form form, int items, hipStream_t s)
 {
   const bool zp = a.w[0].z != nullptr;
   if (dtype == 1)
-    return zp ? launch_group<__bf16, true, EPI>(a, group, rows, tiles, s)
-              : launch_group<__bf16, false, EPI>(a, group, rows, tiles, s);
-  return zp ? launch_group<_Float16, true, EPI>(a, group, rows, tiles, s)
-            : launch_group<_Float16, false, EPI>(a, group, rows, tiles, s);
+    return zp ? launch_group<__bf16, true, EPI>(a, group, form, items, s)
+              : launch_group<__bf16, false, EPI>(a, group, form, items, s);
+  return zp ? launch_group<_Float16, true, EPI>(a, group, form, items, s)
+            : launch_group<_Float16, false, EPI>(a, group, form, items, s);
 }
-
-int rows_of(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
 
 template <Int4Epi EPI>
 hipError_t launch_routed(const Int4Args& a, int group, int dtype, hipStream_t s)
 {
-  const int rows = int4_tile_rows(a.pairs.P, a.pairs.E);
-  return launch_typed<EPI>(a, group, dtype, rows, a.tiles ? int4_max_tiles(a.pairs.P, a.pairs.E) : a.pairs.P, s);
+  const int P = a.pairs.P, rows = int4_tile_rows(P, a.pairs.E), tiles = a.tiles ? int4_max_tiles(P, a.pairs.E) : P;
+  // as many tiles as there are likely to be, of weight rows as wide as a dense product's
+  const int likely = P / rows + min(P, a.pairs.E) / 2, wide = EPI == kInt4Glu ? 2 * a.R : a.R;
+  Int4Form form = kStrip;
+  if (rows == 32)
+    form = fills_no_round(kTile218, likely, wide) ? kTile218 : fills_no_round(kTile224, likely, wide) ? kTile224 : kTile222;
+  else if (rows == 64)
+    form = fills_no_round(kTile424, likely, wide) ? kTile424 : fills_no_round(kTile442, likely, wide) ? kTile442 : kTile441;
+  return launch_typed<EPI>(a, group, dtype, form, tiles, s);
 }
 
 }  // namespace
 
 hipError_t launch_int4_gemm(const Int4Args& a, int group, int dtype, hipStream_t s)
 {
-  const int rows = a.M <= kVecMost && a.K >= kVecMinK ? (a.M <= 2 ? a.M : 4) : rows_of(a.M);
-  const int tiles = (int)(((long long)a.M + rows - 1) / rows);
-  return launch_typed<kInt4Store>(a, group, dtype, rows, tiles, s);
+  const auto tiles = [&](Int4Form f) { return (a.M + form_rows(f) - 1) / form_rows(f); };
+  Int4Form form = kTile441;
+  if (a.M <= kVecMost && a.K >= kVecMinK) {
+    form = a.M == 1 ? kVec1 : a.M == 2 ? kVec2 : kVec4;
+  } else if (a.M <= 16) {
+    form = kStrip;
+  } else {
+    for (Int4Form f : {kTile442, kTile424, kTile224, kTile218})
+      if (fills_no_round(f, tiles(f), a.R)) form = f;
+  }
+  return launch_typed<kInt4Store>(a, group, dtype, form, tiles(form), s);
 }
 
-int int4_tile_rows(int P, int E) { return rows_of(P / E); }
+int int4_tile_rows(int P, int E) { return P / E <= 16 ? 16 : P / E <= 32 ? 32 : 64; }
 
 hipError_t launch_int4_route(const Int4Pairs& p, int4* tiles, int* n_tiles, int* order, hipStream_t s)
 {
@@ -1042,7 +970,7 @@ hipError_t launch_int4_route(const Int4Pairs& p, int4* tiles, int* n_tiles, int*
 bool int4_by_token(int N, int D, int F) { return N == 1 && min(D, F) >= kVecMinK; }
 hipError_t launch_int4_glu(const Int4Args& a, int group, int dtype, hipStream_t s)
 {
-  if (a.by_token) return launch_typed<kInt4Glu>(a, group, dtype, 1, a.pairs.P, s);
+  if (a.by_token) return launch_typed<kInt4Glu>(a, group, dtype, kVec1, a.pairs.P, s);
   return launch_routed<kInt4Glu>(a, group, dtype, s);
 }
 hipError_t launch_int4_pairs(const Int4Args& a, int group, int dtype, hipStream_t s)
@@ -1051,7 +979,7 @@ hipError_t launch_int4_pairs(const Int4Args& a, int group, int dtype, hipStream_
 }
 hipError_t launch_int4_token(const Int4Args& a, int group, int dtype, hipStream_t s)
 {
-  return launch_typed<kInt4Token>(a, group, dtype, 1, a.pairs.P / a.pairs.k, s);
+  return launch_typed<kInt4Token>(a, group, dtype, kVec1, a.pairs.P / a.pairs.k, s);
 }
 
 hipError_t launch_int4_combine(void* out, const float* y, const float* topk_w, const Int4Pairs& p, int D, int dtype,
