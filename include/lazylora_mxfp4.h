@@ -345,7 +345,7 @@ int mxfp4_select_topk_backward(void *grad_logits, const int64_t *topk_idx, const
  * W [R, K]: packed [R, K / 2] bytes (low nibble = even element), scales [R, K / group] of the activations'
  * dtype (MXFP4_BF16 or _F16), zeros [R, K / group] bytes or NULL (8 everywhere);
  *   W[r, k] = scales[r, k / group] * (code[r, k] - zeros[r, k / group]).
- * group 32, 64 or 128, K a multiple of it; K and R at most 2^20. packed, x and y 16-byte aligned. Codes enter
+ * group 32, 64 or 128, K a multiple of it; K and R at most 2^20. All pointers 16-byte aligned. Codes enter
  * the products exactly, sums are fp32 and every result is rounded once (an infinity in a row of x gives NaN).
  * No atomics on values: results do not depend on timing.
  *

@@ -1363,9 +1363,8 @@ int mxfp4_int4_gemm(void* y, const void* x, const uint8_t* packed, const void* s
   if (M < 0 || M > (1 << 24)) return fail(MXFP4_EINVAL, "int4_gemm: M must lie in [0, 2^24]%s");
   if (M == 0) return MXFP4_OK;
   if (!y || !x || !packed || !scales) return fail(MXFP4_EINVAL, "int4_gemm: null pointer%s");
-  if (!all_aligned16({y, x, packed}))
-    return fail(MXFP4_EINVAL, "int4_gemm: y, x and packed must be 16-byte aligned%s");
-  if (reinterpret_cast<uintptr_t>(scales) & 1) return fail(MXFP4_EINVAL, "int4_gemm: scales must be 2-byte aligned%s");
+  if (!all_aligned16({y, x, packed, scales, zeros}))
+    return fail(MXFP4_EINVAL, "int4_gemm: pointers must be 16-byte aligned%s");
   mx::Int4Args a = {};
   a.w[0] = {packed, scales, zeros};
   a.x = x;
@@ -1401,8 +1400,8 @@ int mxfp4_int4_moe_forward(void* out, const void* h, int dtype, const void* topk
   for (int m = 0; m < 3; ++m) {
     if (!codes[m] || !scales[m]) return fail(MXFP4_EINVAL, "int4_moe_forward: null weight pointer%s");
     if (zeros && !zeros[m] != !zeros[0]) return fail(MXFP4_EINVAL, "int4_moe_forward: zeros of all matrices or none%s");
-    if (!aligned16(codes[m]) || (reinterpret_cast<uintptr_t>(scales[m]) & 1))
-      return fail(MXFP4_EINVAL, "int4_moe_forward: codes must be 16-byte and scales 2-byte aligned%s");
+    if (!all_aligned16({codes[m], scales[m], zeros ? zeros[m] : nullptr}))
+      return fail(MXFP4_EINVAL, "int4_moe_forward: codes, scales and zeros must be 16-byte aligned%s");
   }
   if (!all_aligned16({out, h}) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return fail(MXFP4_EINVAL, "int4_moe_forward: out and h must be 16-byte, the workspace 256-byte aligned%s");

@@ -23,10 +23,16 @@ from lazylora_amd.native import _ACTS
 GROUPS = (32, 64, 128)
 
 
+def _tidy(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and 16-byte aligned, as the kernels take it."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 class Int4Weight:
     """A matrix [R, K] of 4-bit codes, or E of them stacked: packed uint8 [(E,) R, K / 2], scales bfloat16 or
     float16 [(E,) R, K / group], zeros uint8 of the scales' shape, or None: 8 everywhere (symmetric codes). The
-    tensors are kept as they are where they are contiguous; `shape` is [(E,) R, K]."""
+    tensors are kept as they are where they are contiguous and 16-byte aligned; `shape` is [(E,) R, K]."""
 
     __slots__ = ("packed", "scales", "zeros", "shape", "group")
 
@@ -43,8 +49,7 @@ class Int4Weight:
             raise ValueError(f"zeros must be uint8 {tuple(scales.shape)}, got {zeros.dtype} {tuple(zeros.shape)}")
         if scales.device != packed.device or (zeros is not None and zeros.device != packed.device):
             raise ValueError("codes, scales and zeros must lie on one device")
-        self.packed, self.scales = packed.contiguous(), scales.contiguous()
-        self.zeros = None if zeros is None else zeros.contiguous()
+        self.packed, self.scales, self.zeros = _tidy(packed), _tidy(scales), None if zeros is None else _tidy(zeros)
         self.shape: Tuple[int, ...] = tuple(packed.shape[:-1]) + (K,)
         self.group = K // n
 

@@ -18,8 +18,11 @@ adapters' gradients are accumulated into them by the routed node, as in the refe
 With dense="native" the shared expert runs in 16 bits through the gated feed-forward kernels
 (lazylora_amd.dense.gated_ffn; the checkpoint's dense weights are bfloat16, so bfloat16 holds them
 exactly) and the norm of the routed sum through the norm kernels, forward and backward.
+
+For inference the experts can be an Int4Experts (lazylora_amd.int4), 4-bit integer weights with group scales; and
+the router may have softmax scores or choose among groups of experts (lazylora_amd.router.select_experts).
 """
-from typing import Optional, Sequence, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 import torch.nn.functional as F
@@ -27,6 +30,7 @@ import torch.nn.functional as F
 from lazylora_amd.dense import dropout, gated_ffn
 from lazylora_amd.dense import rms_norm as native_rms_norm
 from lazylora_amd.experts import ExpertLayer
+from lazylora_amd.int4 import Int4Experts, int4_routed
 from lazylora_amd.routed import RoutedExpertsFunction
 from lazylora_amd.router import route
 
@@ -75,12 +79,17 @@ class LatentMoEBlock:
     dense: "torch" (fp32 BLAS) or "native" (the shared expert in dense_dtype, torch.bfloat16 or
     torch.float16, through the feed-forward kernels, and the norm through the norm kernels; the hidden
     and shared widths must be multiples of 8).
+
+    scoring, num_groups, topk_groups and group_score as in select_experts. experts may be an Int4Experts: the
+    routed products then run in its scales' type, without routed adapters, and where a gradient would be
+    recorded a call raises NotImplementedError.
     """
 
-    def __init__(self, experts: ExpertLayer, gate_weight, gate_bias, shared_w1, shared_w3, shared_w2, latent_down,
+    def __init__(self, experts: Union[ExpertLayer, Int4Experts], gate_weight, gate_bias, shared_w1, shared_w3, shared_w2, latent_down,
                  latent_up, latent_norm=None, top_k: int = 16, routed_scaling_factor: float = 1.0,
                  renormalize: bool = True, act: str = "situ", rms_eps: float = 1e-5, lora=None,
-                 dense: str = "torch", dense_dtype: torch.dtype = torch.bfloat16):
+                 dense: str = "torch", dense_dtype: torch.dtype = torch.bfloat16, scoring: str = "sigmoid",
+                 num_groups: int = 1, topk_groups: Optional[int] = None, group_score: str = "top2"):
         if dense not in ("torch", "native"):
             raise ValueError(f'dense must be "torch" or "native", got {dense!r}')
         dev = experts.device
@@ -93,6 +102,9 @@ class LatentMoEBlock:
         self.latent_down, self.latent_up, self.latent_norm = f32(latent_down), f32(latent_up), f32(latent_norm)
         self.top_k, self.routed_scaling_factor, self.renormalize = top_k, routed_scaling_factor, renormalize
         self.act, self.rms_eps, self.lora = act, rms_eps, lora
+        self.scoring, self.num_groups, self.topk_groups, self.group_score = scoring, num_groups, topk_groups, group_score
+        if isinstance(experts, Int4Experts) and self._routed_lora() is not None:
+            raise ValueError("routed adapters need an ExpertLayer: the products with 4-bit integer weights take none")
         H = self.gate_weight.shape[1]
         if self.latent_down.shape != (experts.D, H) or self.latent_up.shape != (H, experts.D):
             raise ValueError(f"latent projections must be [{experts.D}, {H}] and [{H}, {experts.D}]")
@@ -125,6 +137,14 @@ class LatentMoEBlock:
             return y.float()
         return y.float() + delta(s_act.float(), "shared_down_lora", 2)
 
+    def _routed(self, h_latent: torch.Tensor, w: torch.Tensor, idx: torch.Tensor, cached) -> torch.Tensor:
+        """The routed experts' sum, fp32 (`cached`: an earlier call's)."""
+        if not isinstance(self.experts, Int4Experts):
+            return RoutedExpertsFunction.apply(h_latent, w, idx, self.experts, self.act, cached, self._routed_lora())
+        if cached is not None:
+            return cached
+        return int4_routed(h_latent.to(self.experts.dtype), idx, w, self.experts, self.act).float()
+
     def forward(self, h_moe_norm: torch.Tensor, cached: Optional[torch.Tensor] = None, dropout_seed=None
                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """(out in h's dtype and shape, topk_indices, topk_weights) for the normed hidden state.
@@ -135,10 +155,11 @@ class LatentMoEBlock:
         elements. Give every layer and step its own. The routed adapters take no dropout."""
         shape, dtype = h_moe_norm.shape, h_moe_norm.dtype
         x = h_moe_norm.reshape(-1, self.hidden).to(self.experts.device, torch.float32)
-        idx, w = route(x, self.gate_weight, self.gate_bias, self.top_k, self.routed_scaling_factor, self.renormalize)
+        idx, w = route(x, self.gate_weight, self.gate_bias, self.top_k, self.routed_scaling_factor, self.renormalize,
+                       self.scoring, self.num_groups, self.topk_groups, self.group_score)
         shared = self._shared(x, dropout_seed)
         h_latent = F.linear(x, self.latent_down)
-        routed = RoutedExpertsFunction.apply(h_latent, w, idx, self.experts, self.act, cached, self._routed_lora())
+        routed = self._routed(h_latent, w, idx, cached)
         if self.latent_norm is not None:
             norm = native_rms_norm if self.native else rms_norm
             routed = norm(routed, self.latent_norm, self.rms_eps)

@@ -49,6 +49,8 @@ def bound(x, w, y, dt):
 SIZES = [  # M, K, R
     (1, 128, 16), (1, 256, 1), (2, 384, 17), (3, 640, 40), (15, 128, 33), (16, 1024, 16), (17, 512, 20), (31, 256, 18),
     (32, 128, 5), (33, 384, 31), (64, 256, 16), (65, 128, 16), (130, 512, 49), (1, 7168, 24),
+    # each form of the tiles: two by eight waves, two by two by four, four by two by four, four by four by two and by one
+    (64, 1152, 2100), (200, 384, 2100), (300, 384, 2100), (600, 384, 2100), (1100, 128, 2100), (4, 512, 70000),
 ]
 
 
@@ -144,6 +146,11 @@ ROUTED = [  # N, k, E, D, F, group, zeros, dtype, act
     (150, 2, 2, 128, 128, 128, False, "bf16", "swiglu"), (1, 8, 12, 1024, 1152, 64, True, "bf16", "swiglu"),
     (1, 3, 4, 2176, 1024, 128, False, "f16", "situ"), (1, 11, 16, 1024, 1024, 32, False, "bf16", "situ"),
     (2, 8, 12, 1024, 1152, 64, True, "bf16", "swiglu"),
+    # 32 rows to a tile in each form (few, some, many weight rows), then 64
+    (50, 2, 4, 96, 64, 32, True, "f16", "swiglu"), (50, 2, 4, 160, 1024, 32, False, "bf16", "swiglu"),
+    (50, 2, 4, 128, 4096, 64, True, "bf16", "situ"), (50, 2, 4, 4096, 160, 32, False, "f16", "swiglu"),
+    (128, 2, 4, 128, 2048, 128, True, "bf16", "swiglu"), (512, 2, 16, 96, 2048, 32, True, "f16", "swiglu"),
+    (512, 2, 16, 2048, 96, 32, False, "bf16", "situ"),
 ]
 
 
