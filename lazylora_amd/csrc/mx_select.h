@@ -18,7 +18,11 @@ struct SelectArgs {
   int num_groups, topk_groups;
   float scale;
   bool renormalize;
-  int run, per, group_size;  // set by launch_select: lanes of a group, experts of a lane, of a group
+  // set by launch_select: lanes of a group (a power of two), experts of a lane, of a group; every lane of a group has
+  // as many experts as the kernel holds
+  int run, run_log, per, group_size;
+  bool full;
+  long long token0;  // first token of a launch
 };
 struct SelectBwdArgs {
   void* grad_logits;  // [N, E], fully written
@@ -29,6 +33,7 @@ struct SelectBwdArgs {
   bool softmax;
   float scale;
   bool renormalize;
+  long long token0;  // set by launch_select_bwd: first token of a launch
 };
 
 // Experts that a lane holds for these sizes (more than kSelectMaxPer: they do not fit).

@@ -108,19 +108,31 @@ MX_DEV Slots lane_slots(const SelectArgs& a, int lane)
 {
   Slots s;
   s.run = a.run;
-  s.group = lane / a.run;
+  s.group = lane >> a.run_log;
   const int at = (lane & (a.run - 1)) * a.per;
   s.first = s.group * a.group_size + at;
   s.count = s.group < a.num_groups ? max(0, min(a.per, a.group_size - at)) : 0;
   return s;
 }
 
-// The larger two of two pairs, over a run's lanes.
-template <typename K>
-MX_DEV void run_top2(K& a, K& b, int run)
+// The two largest keys of a run's lanes, from each lane's two.
+MX_DEV void merge2(uint32_t& a, uint32_t& b, uint32_t c, uint32_t d)
+{
+  b = max(min(a, c), max(b, d));
+  a = max(a, c);
+}
+MX_DEV void run_top2(uint32_t& a, uint32_t& b, int run)
+{
+  if (run > 1) merge2(a, b, dpp_u<kDppXor1>(a), dpp_u<kDppXor1>(b));
+  if (run > 2) merge2(a, b, dpp_u<kDppXor2>(a), dpp_u<kDppXor2>(b));
+  if (run > 4) merge2(a, b, dpp_u<kDppHalfMirror>(a), dpp_u<kDppHalfMirror>(b));
+  if (run > 8) merge2(a, b, dpp_u<kDppMirror>(a), dpp_u<kDppMirror>(b));
+  for (int off = 16; off < run; off <<= 1) merge2(a, b, __shfl_xor(a, off, 64), __shfl_xor(b, off, 64));
+}
+MX_DEV void run_top2(uint64_t& a, uint64_t& b, int run)
 {
   for (int off = 1; off < run; off <<= 1) {
-    const K c = __shfl_xor(a, off, 64), d = __shfl_xor(b, off, 64);
+    const uint64_t c = __shfl_xor(a, off, 64), d = __shfl_xor(b, off, 64);
     b = max(min(a, c), max(b, d));
     a = max(a, c);
   }
@@ -202,18 +214,28 @@ struct Careful {
 // One wave per token. A round of the selection takes the largest open key of the wave (four butterfly steps
 // and four lane reads), names its holder by a ballot and retires the expert there.
 template <typename T, int PER>
-__global__ __launch_bounds__(256) void select_kernel(SelectArgs a)
+__global__ __launch_bounds__(256, PER <= 4 ? 8 : 1) void select_kernel(SelectArgs a)
 {
   const int lane = threadIdx.x & 63;
-  const long long token = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long token = a.token0 + (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (token >= a.N) return;  // whole waves leave together
   const T* row = static_cast<const T*>(a.logits) + token * a.E;
   const Slots at = lane_slots(a, lane);
 
+  // every lane loads, from its last expert again past its own (an absent group's lanes from the first one), and with
+  // one instruction where all lanes have PER
+  const int base = at.count > 0 ? at.first : 0, last = max(at.count - 1, 0);
   float x[PER];
+  if (a.full) {
+    T raw[PER];
+    __builtin_memcpy(raw, row + base, sizeof(raw));
+    static_for<PER>([&](auto mc) { x[decltype(mc)::value] = load_logit<T>(raw + decltype(mc)::value); });
+  } else {
+    static_for<PER>([&](auto mc) { x[decltype(mc)::value] = load_logit<T>(row + base + min((int)decltype(mc)::value, last)); });
+  }
   static_for<PER>([&](auto mc) {
     constexpr int m = decltype(mc)::value;
-    x[m] = m < at.count ? load_logit<T>(row + at.first + m) : -__builtin_inff();
+    x[m] = m < at.count ? x[m] : -__builtin_inff();
   });
   Score<float> score{a.softmax, 0.f, 1.f};
   float smax = 1.f;  // no score of the row is larger
@@ -228,15 +250,36 @@ __global__ __launch_bounds__(256) void select_kernel(SelectArgs a)
     score.sum = sum == 0.f ? 1.f : sum;
     smax = 1.f / score.sum;
   }
-  // half of this is what a score may be off by: the exponential, the quotient, the sum behind it
+  // The keys' scores take the device's exponential and reciprocal (sigmoid_f, and 2^((l - max) log2 e) / sum): off by
+  // less than half of this, the rounding of the exponent (which moves a score s by s |l - max| 2^-24, at most 0.37 smax
+  // 2^-24), the exponential, the reciprocal and the sum behind it. The weights are computed again in full.
+  const float inv = 1.f / score.sum;
+  const auto quick = [&](float l) {
+    return a.softmax ? __builtin_amdgcn_exp2f((l - score.top) * kLog2e) * inv : sigmoid_f(l);
+  };
   const float s_err = smax * (a.softmax ? 0x1p-20f + (float)(a.per + 16) * 0x1p-23f : 0x1p-20f);
 
   uint32_t key[PER];  // 0: absent, in no kept group or already chosen
+  if (a.bias) {
+    float c[PER];
+    if (a.full)
+      __builtin_memcpy(c, a.bias + base, sizeof(c));
+    else
+      static_for<PER>([&](auto mc) { c[decltype(mc)::value] = a.bias[base + min((int)decltype(mc)::value, last)]; });
+    if (a.softmax)
+      static_for<PER>([&](auto mc) {
+        constexpr int m = decltype(mc)::value;
+        c[m] += __builtin_amdgcn_exp2f((x[m] - score.top) * kLog2e) * inv;
+      });
+    else
+      static_for<PER>([&](auto mc) { c[decltype(mc)::value] += sigmoid_f(x[decltype(mc)::value]); });
+    static_for<PER>([&](auto mc) { key[decltype(mc)::value] = order_key(c[decltype(mc)::value]); });
+  } else {
+    static_for<PER>([&](auto mc) { key[decltype(mc)::value] = order_key(x[decltype(mc)::value]); });
+  }
   static_for<PER>([&](auto mc) {
     constexpr int m = decltype(mc)::value;
-    uint32_t k = 0;
-    if (m < at.count) k = order_key(a.bias ? score(x[m]) + a.bias[at.first + m] : x[m]);
-    key[m] = k;
+    key[m] = m < at.count ? key[m] : 0u;
   });
 
   bool on = at.count > 0;  // the lane's experts can be chosen
@@ -254,7 +297,7 @@ __global__ __launch_bounds__(256) void select_kernel(SelectArgs a)
     uint32_t gk = k1;
     if (a.top2) {
       float c1 = key_value(k1), c2 = key_value(k2);
-      if (scores) c1 = score(c1), c2 = score(c2);
+      if (scores) c1 = quick(c1), c2 = quick(c2);
       if (k2 != 0) {
         gk = order_key(c1 + c2);
         err = 2.f * s_err + 0x1p-21f * (fabsf(c1) + fabsf(c2));
@@ -268,9 +311,13 @@ __global__ __launch_bounds__(256) void select_kernel(SelectArgs a)
     // a group's rank, and whether another group on the other side of the line is too close to tell
     const float gv = key_value(gk);
     int rank = 0;
-    for (int g = 0; g < a.num_groups; ++g) {
-      const uint32_t other = lane_u(gk, g * at.run);
-      rank += other > gk || (other == gk && g < at.group);
+    const int place = lane & (at.run - 1), start = lane - place;
+    for (int g0 = 0; g0 < a.num_groups; g0 += at.run) {  // a run's lanes compare with a group each
+      const int g = g0 + place;
+      const uint32_t other = (uint32_t)__shfl((int)gk, min(g, a.num_groups - 1) << a.run_log, 64);
+      const bool better = (g < a.num_groups) & ((other > gk) | ((other == gk) & (g < at.group)));
+      const uint64_t votes = __builtin_amdgcn_ballot_w64(better) >> start;
+      rank += __popcll(at.run == 64 ? votes : votes & ((1ull << at.run) - 1));
     }
     on = on && rank < a.topk_groups;
     if (a.top2 || a.bias) {
@@ -363,7 +410,7 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelectBwdArgs a)
 {
   extern __shared__ float rows[];
   const int lane = threadIdx.x & 63;
-  const long long token = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long token = a.token0 + (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (token >= a.N) return;
   float* ds_row = rows + (threadIdx.x >> 6) * a.E;
   const T* row = static_cast<const T*>(a.logits) + token * a.E;
@@ -432,29 +479,45 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelectBwdArgs a)
   });
 }
 
+// A launch's threads are counted in 32 bits: so many tokens take one.
+constexpr long long kTokensPerLaunch = 1 << 25;
+template <class Kernel, class Args>
+void launch_tokens(Kernel kernel, Args a, size_t lds, hipStream_t s)
+{
+  for (a.token0 = 0; a.token0 < a.N; a.token0 += kTokensPerLaunch) {
+    const long long now = a.N - a.token0 < kTokensPerLaunch ? a.N - a.token0 : kTokensPerLaunch;
+    kernel<<<dim3((unsigned)((now + 3) / 4)), 256, lds, s>>>(a);
+  }
+}
+template <typename T, int PER>
+void launch_per(SelectArgs a, hipStream_t s)
+{
+  a.full = a.per == PER && a.group_size % PER == 0;
+  launch_tokens(select_kernel<T, PER>, a, 0, s);
+}
 template <typename T>
 hipError_t run_select(const SelectArgs& a, hipStream_t s)
 {
-  const dim3 grid((unsigned)((a.N + 3LL) / 4)), block(256);
-  if (a.per <= 4)
-    select_kernel<T, 4><<<grid, block, 0, s>>>(a);
+  if (a.per <= 1)
+    launch_per<T, 1>(a, s);
+  else if (a.per <= 4)
+    launch_per<T, 4>(a, s);
   else if (a.per <= 16)
-    select_kernel<T, 16><<<grid, block, 0, s>>>(a);
+    launch_per<T, 16>(a, s);
   else
-    select_kernel<T, 64><<<grid, block, 0, s>>>(a);
+    launch_per<T, 64>(a, s);
   return hipGetLastError();
 }
 template <typename T>
 hipError_t run_select_bwd(const SelectBwdArgs& a, hipStream_t s)
 {
-  const dim3 grid((unsigned)((a.N + 3LL) / 4)), block(256);
   const size_t lds = 4 * sizeof(float) * a.E;
   if (a.E <= 4 * 64)
-    select_bwd_kernel<T, 4><<<grid, block, lds, s>>>(a);
+    launch_tokens(select_bwd_kernel<T, 4>, a, lds, s);
   else if (a.E <= 16 * 64)
-    select_bwd_kernel<T, 16><<<grid, block, lds, s>>>(a);
+    launch_tokens(select_bwd_kernel<T, 16>, a, lds, s);
   else
-    select_bwd_kernel<T, 64><<<grid, block, lds, s>>>(a);
+    launch_tokens(select_bwd_kernel<T, 64>, a, lds, s);
   return hipGetLastError();
 }
 
@@ -473,6 +536,7 @@ hipError_t launch_select(SelectArgs a, int dtype, hipStream_t s)
   int runs = 1;
   while (runs < a.num_groups) runs *= 2;
   a.run = kSelectLanes / runs;
+  a.run_log = __builtin_ctz(a.run);
   a.group_size = a.E / a.num_groups;
   a.per = select_per_lane(a.E, a.num_groups);
   switch (dtype) {

@@ -126,6 +126,8 @@ class KimiK3MoERouter(nn.Module):
     """KimiK3MoERouter (lazy_lora/core/moe_router.py:23-135) with the selection on MI355X; scoring and the
     group arguments as in select_experts."""
 
+    scoring, num_groups, topk_groups, group_score = "sigmoid", 1, None, "top2"  # of modules saved without them
+
     def __init__(self, hidden_size: int = 7168, num_experts: int = 896, top_k: int = 16,
                  routed_scaling_factor: float = 1.0, renormalize: bool = True, use_bias: bool = True,
                  device: Optional[Union[str, torch.device]] = None, scoring: str = "sigmoid", num_groups: int = 1,

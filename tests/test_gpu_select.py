@@ -236,6 +236,24 @@ def test_layouts_devices_and_empty_inputs(select):
     assert torch.equal(got[0], select(row, 4)[0])
 
 
+def test_more_tokens_than_one_launch_takes(select):
+    """2^25 tokens to a launch: the ones on both sides of the line, and the last, forward and backward."""
+    N = 2 ** 25 + 5
+    x = torch.zeros(N, 2, device="cuda", dtype=torch.bfloat16)
+    at = torch.tensor([0, 2 ** 25 - 1, 2 ** 25, 2 ** 25 + 1, N - 1], device="cuda")
+    x[at, 1] = 1.0
+    x.requires_grad_(True)
+    idx, w = select(x, 1, scoring="softmax", renormalize=False)
+    want = torch.zeros(N, device="cuda", dtype=torch.int64)
+    want[at] = 1
+    assert torch.equal(idx[:, 0], want)
+    hot = 1 / (1 + np.exp(-1.0))
+    assert (w[at, 0] - hot).abs().max() < 1e-6 and int((w == 0.5).sum()) == N - len(at)
+    g = torch.autograd.grad(w, x, torch.ones_like(w))[0]
+    assert int((g == torch.tensor([0.25, -0.25], device="cuda").bfloat16()).all(1).sum()) == N - len(at)
+    assert (g[at, 1].float() - hot * (1 - hot)).abs().max() < 2e-3
+
+
 def test_refusals(select):
     x = torch.randn(3, 64, device="cuda")
     for kw in ({"top_k": 0}, {"top_k": 65}, {"top_k": 4, "num_groups": 5}, {"top_k": 4, "num_groups": 0},
