@@ -225,12 +225,15 @@ MX_DEV uint8_t load_zero(const Rows& w, uint32_t lane, uint32_t shared)
 }
 
 // ------------------------------------------------------------------ few rows of x
-// Lane i keeps the elements 32 i .. 32 i + 31 of up to MR rows of x in registers and walks the weight rows,
-// kVecRows of them loaded while those before are summed. A wave's load is 1 KiB of one row, x is loaded once
-// for all rows of a work-group (the MFMA form below loads as many bytes of x as of codes for every 16 x 128
-// block), and a product is two instructions for two codes and one dot of two for each row of x. The lanes'
-// sums meet in exchanges of half-waves and quarter-waves, each of which halves how many there are, the waves'
-// in LDS.
+// Lane i keeps the elements 32 i .. 32 i + 31 of up to MR rows of x in registers and walks the weight rows, kVecRows
+// of them loaded while those before are summed. A wave's load is 1 KiB of one row, x is loaded once for all rows of a
+// work-group (with every 16 x 128 block of the codes, as the MFMA takes them, there would be as many bytes of x as of
+// codes), and a product is two instructions for two codes and one dot of two for each row of x. The lanes' sums meet
+// in exchanges of half-waves and quarter-waves, each of which halves how many there are, the waves' in LDS. One row
+// is bound by the codes' bytes behind some 5 us of launch, first loads and last sums: rows of 8192 in groups of 64,
+// us (TB/s): 4096 weight rows 6.9 (2.7), 28672 26 (4.9), 114688 89 (5.8), 229376 171 (6.0). Two rows 8.6 / 30 / 94 /
+// 189; four 10.6 / 42 / 129 / 260, bound by the dots (the 4 x 4 x 4 MFMA in their place, x in its 16 registers
+// whatever its rows: 8.6 / 30 / 121 / 218 with one row, 9.5 / 32 / 127 / 231 with four).
 template <typename T, int G, bool ZP, int MR, Int4Epi EPI>
 __global__ __launch_bounds__(512) void int4_vec_kernel(Int4Args p)
 {
@@ -367,11 +370,20 @@ __global__ __launch_bounds__(512) void int4_vec_kernel(Int4Args p)
 }
 
 // ------------------------------------------------------------------ up to 16 rows of x
-// A wave keeps 256 terms of up to 16 rows of x in registers, as the MFMA takes them, with their sums over each
-// group, and walks groups of 16 weight rows (of a gate/up product: of both matrices), the codes of the next one
-// in flight. The waves of a work-group share K; their sums meet in LDS once, in the waves' order.
+// A wave keeps 256 terms of up to 16 rows of x in registers, as the MFMA takes them, with their sums over each group,
+// and walks groups of 16 weight rows (of a gate/up product: of both matrices), the codes of the next one in flight.
+// The waves of a work-group share K; their sums meet in LDS once, in the waves' order. Bound by the codes' bytes
+// where they are many (256 pairs over 128 experts, 3584 / 1536, gate/up: 0.64 GB in 121 us, 5.3 TB/s), else by the
+// launch: 13 rows of [7168, 3584], groups of 32, 9.0 us, where x from L2 with every block took 17.5 and x staged in
+// LDS for the whole work-group 12.9 to 17.
+// Waves of a work-group at most: as many as their registers let in without spills (two matrices, or a scale loaded by
+// itself for each group of 32, take more).
+constexpr int strip_waves(int group, Int4Epi epi, bool wide)
+{
+  return epi == kInt4Glu || (group == 32 && !wide) ? 8 : 16;
+}
 template <typename T, int G, bool ZP, Int4Epi EPI, bool WIDE>
-__global__ __launch_bounds__(EPI == kInt4Glu ? 512 : 1024) void int4_strip_kernel(Int4Args p)
+__global__ __launch_bounds__(64 * strip_waves(G, EPI, WIDE)) void int4_strip_kernel(Int4Args p)
 {
   using N = Num<T>;
   constexpr int NMAT = EPI == kInt4Glu ? 2 : 1, NG = 128 / G, JG = 4 / NG, NB = kStripGroups;
@@ -389,7 +401,8 @@ __global__ __launch_bounds__(EPI == kInt4Glu ? 512 : 1024) void int4_strip_kerne
   const i32x4 ones = {(int)N::kOnes, (int)N::kOnes, (int)N::kOnes, (int)N::kOnes};
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   const int x_row = rows[n];
-  const uint16_t* xr = static_cast<const uint16_t*>(p.x) + (long long)(EPI == kInt4Store ? x_row : x_row / p.x_div) * p.K;
+  const uint16_t* xr =
+      static_cast<const uint16_t*>(p.x) + (long long)(EPI == kInt4Store ? x_row : x_row / p.x_div) * p.K;
   Rows w[NMAT];
 #pragma unroll
   for (int m = 0; m < NMAT; ++m)
@@ -521,10 +534,15 @@ __global__ __launch_bounds__(EPI == kInt4Glu ? 512 : 1024) void int4_strip_kerne
 
 // ------------------------------------------------------------------ many rows of x
 // A team of WN waves makes 16 MT rows of x x 32 WN weight rows, 32 to each wave (of a gate/up product 16 of both
-// matrices), K in blocks of 128: x of a block in LDS in the order the MFMA takes it, two buffers, the next
-// block's x and codes in registers meanwhile. KS teams of a work-group take every KS-th block; their sums meet in
-// LDS at the end, in the teams' order. A block's 16-byte piece (j, c) of row r lies at place r ^ (4 j + c) of 16:
-// neither the writes (16 pieces of a row) nor the reads (16 rows of a piece) meet bank conflicts.
+// matrices), K in blocks of 128: x of a block in LDS in the order the MFMA takes it, two buffers, the next block's x
+// and codes in registers meanwhile. KS teams of a work-group take every KS-th block; their sums meet in LDS at the
+// end, in the teams' order. A block's 16-byte piece (j, c) of row r lies at place r ^ (4 j + c) of 16: neither the
+// writes (16 pieces of a row) nor the reads (16 rows of a piece) meet bank conflicts. Per block of 64 x 128 products
+// a wave issues 32 MFMAs for the products, 16 for the sums of x, 64 instructions to decode and 64 per group for
+// scales and zero points: about as long on the vector as on the matrix pipe, which is what bounds it (1000 rows of
+// [2048, 7168] in groups of 64, 66 us, 446 TFLOP/s; 2000 pairs over 32 experts of 3584 / 1536, gate/up 147 us, 300
+// TFLOP/s: partly filled tiles). With the accumulators in AGPRs, which the compiler chooses by itself, moves doubled
+// the vector instructions (250 -> 85 us with it all).
 template <typename T, int G, bool ZP, int MT, int WN, int KS, Int4Epi EPI, bool WIDE>
 __global__ __launch_bounds__(64 * WN * KS) void int4_tile_kernel(Int4Args p)
 {
@@ -823,8 +841,9 @@ hipError_t launch_vec(Int4Args a, int items, hipStream_t s)
 template <typename T, int G, bool ZP, Int4Epi EPI>
 hipError_t launch_strip(Int4Args a, int tiles, hipStream_t s)
 {
-  constexpr int NMAT = EPI == kInt4Glu ? 2 : 1, MAXW = EPI == kInt4Glu ? 8 : 16;
-  const int units = (a.K + 255) / 256, rounds = (units + MAXW - 1) / MAXW, waves = (units + rounds - 1) / rounds;
+  constexpr int NMAT = EPI == kInt4Glu ? 2 : 1;
+  const int most_waves = strip_waves(G, EPI, a.K % 256 == 0);
+  const int units = (a.K + 255) / 256, rounds = (units + most_waves - 1) / most_waves, waves = (units + rounds - 1) / rounds;
   const auto kernel = a.K % 256 == 0 ? int4_strip_kernel<T, G, ZP, EPI, true> : int4_strip_kernel<T, G, ZP, EPI, false>;
   const int all = (a.R + 15) / 16;
   const long long full = 256 * 16 / waves;
@@ -859,10 +878,10 @@ hipError_t launch_tile(Int4Args a, int tiles, hipStream_t s)
 
 // The forms by the rows of x that they take at once, and of the tile kernel by its waves. A work-group of the tile
 // kernel is one or two waves per SIMD whatever its form, so while there are fewer of them than CUs, smaller ones with
-// more teams on K are quicker: [2048, 7168] bf16, groups of 64, us, as 2 x 1 x 8 (MT, WN, KS) / 2 x 2 x 4 / 4 x 2 x 4 /
-// 4 x 4 x 2 / 4 x 4 x 1: 64 rows 18 / 27 / 36 / 64 / 72, 200 rows 36 / 28 / 37 / 64 / 77, 500 rows 71 / 49 / 40 / 66 / 80,
-// 1000 rows 136 / 96 / 82 / 72 / 85, 2000 rows 267 / 187 / 157 / 146 / 128; [7168, 3584]: 32 rows 11 / 14 / 19 / 32 / 35, 64
-// rows 20 / 15 / 20 / 33 / 37, 200 rows 65 / 42 / 40 / 36 / 40, 500 rows 131 / 74 / 77 / 68 / 59.
+// more teams on K are quicker: [2048, 7168] bf16, groups of 64, us, as 2 x 1 x 8 (MT, WN, KS) / 2 x 2 x 4 / 4 x 2 x 4
+// / 4 x 4 x 2 / 4 x 4 x 1: 64 rows 18 / 27 / 36 / 64 / 72, 200 rows 36 / 28 / 37 / 64 / 77, 500 rows 71 / 49 / 40 /
+// 66 / 80, 1000 rows 136 / 96 / 82 / 72 / 85, 2000 rows 267 / 187 / 157 / 146 / 128; [7168, 3584]: 32 rows 11 / 14 /
+// 19 / 32 / 35, 64 rows 20 / 15 / 20 / 33 / 37, 200 rows 65 / 42 / 40 / 36 / 40, 500 rows 131 / 74 / 77 / 68 / 59.
 enum Int4Form : int {
   kVec1, kVec2, kVec4,     // the few-row form
   kStrip,                  // 16 rows

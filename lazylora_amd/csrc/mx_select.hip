@@ -211,8 +211,11 @@ struct Careful {
   }
 };
 
-// One wave per token. A round of the selection takes the largest open key of the wave (four butterfly steps
-// and four lane reads), names its holder by a ballot and retires the expert there.
+// One wave per token, bound by instructions: a round costs some 22 of them and is a serial chain, so as many waves as
+// there can be (eight per SIMD with 64 registers) run side by side. 8192 tokens, top-8 of 256 in 8 groups, sigmoid
+// and bias: 11 us (9 MB of logits would take 1.8); without groups and bias 8.0; 1024 tokens, top-16 of 896 in 7
+// groups, softmax and bias: 14 us; one token 3.6. A round of the selection takes the largest open key of the wave
+// (four butterfly steps and four lane reads), names its holder by a ballot and retires the expert there.
 template <typename T, int PER>
 __global__ __launch_bounds__(256, PER <= 4 ? 8 : 1) void select_kernel(SelectArgs a)
 {
@@ -251,8 +254,8 @@ __global__ __launch_bounds__(256, PER <= 4 ? 8 : 1) void select_kernel(SelectArg
     smax = 1.f / score.sum;
   }
   // The keys' scores take the device's exponential and reciprocal (sigmoid_f, and 2^((l - max) log2 e) / sum): off by
-  // less than half of this, the rounding of the exponent (which moves a score s by s |l - max| 2^-24, at most 0.37 smax
-  // 2^-24), the exponential, the reciprocal and the sum behind it. The weights are computed again in full.
+  // less than half of this, the rounding of the exponent (which moves a score s by s |l - max| 2^-24, at most 0.37
+  // smax 2^-24), the exponential, the reciprocal and the sum behind it. The weights are computed again in full.
   const float inv = 1.f / score.sum;
   const auto quick = [&](float l) {
     return a.softmax ? __builtin_amdgcn_exp2f((l - score.top) * kLog2e) * inv : sigmoid_f(l);
@@ -404,7 +407,7 @@ __global__ __launch_bounds__(256, PER <= 4 ? 8 : 1) void select_kernel(SelectArg
 //   sigmoid: dl_e = ds_e s_e (1 - s_e) at the chosen experts, 0 elsewhere;
 //   softmax: dl_e = s_e (ds_e - d) with d = sum_j ds_j s_j, at every expert. Renormalised, d is
 //   c (sum g s) 1e-20 / S^2: written so, not as the difference of nearly equal sums.
-// A token's ds meet its experts through a row of LDS.
+// A token's ds meet its experts through a row of LDS. 4099 tokens of 64 experts 4.5 us, 1024 of 896 7.7.
 template <typename T, int PER>
 __global__ __launch_bounds__(256) void select_bwd_kernel(SelectBwdArgs a)
 {

@@ -253,6 +253,56 @@ def test_rows_outside_the_call_stay():
         assert (buf[M * R:] == 7).all()
 
 
+@pytest.mark.parametrize("N,k,E,D,F", [(1, 8, 12, 1024, 1152), (5, 8, 12, 128, 64), (40, 4, 12, 160, 96), (300, 4, 6, 128, 96)])
+def test_workspace_and_output_bounds(N, k, E, D, F):
+    """A routed call writes its output and its workspace and nothing behind them, on each path."""
+    import ctypes
+    from lazylora_amd.native import kernel
+    lib = kernel().lib
+    gen = gen_of(N, k, D)
+    ex = layer(gen, E, D, F, 32, True, torch.bfloat16)
+    h = torch.randn(N, D, device="cuda", generator=gen).bfloat16()
+    idx = torch.randint(-1, E, (N, k), device="cuda", generator=gen)
+    w = torch.rand(N, k, device="cuda", generator=gen)
+    out = torch.full((N * D + 512,), 7.0, device="cuda", dtype=torch.bfloat16)
+    n = lib.mxfp4_int4_moe_workspace_size(N, k, E, D, F)
+    ws = torch.full((n + 4096,), 0xA5, device="cuda", dtype=torch.uint8)
+    arr = lambda name: (ctypes.c_void_p * 3)(*[getattr(m, name).data_ptr() for m in (ex.w1, ex.w3, ex.w2)])
+    rc = lib.mxfp4_int4_moe_forward(out.data_ptr(), h.data_ptr(), 1, idx.data_ptr(), 3, w.data_ptr(), N, k, arr("packed"),
+                                    arr("scales"), arr("zeros"), E, D, F, 32, 0, ws.data_ptr(), n,
+                                    torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert (out[N * D:] == 7).all() and (ws[n:] == 0xA5).all()
+    from lazylora_amd.int4 import int4_routed
+    assert torch.equal(out[: N * D].view(N, D), int4_routed(h, idx, w, ex))
+
+
+def test_two_streams_at_once():
+    """Calls of different sizes on two streams, each with its own workspace, give what they give alone."""
+    from lazylora_amd.int4 import int4_gemm, int4_routed
+    gen = gen_of(31)
+    ex = layer(gen, 16, 256, 128, 64, True, torch.bfloat16)
+    wt = weight(gen, (), 512, 256, 64, False, torch.bfloat16)
+    calls = []
+    for N in (1, 3, 33, 200):
+        h = torch.randn(N, 256, device="cuda", generator=gen).bfloat16()
+        idx = torch.randn(N, 16, device="cuda", generator=gen).topk(4, -1).indices
+        w = torch.rand(N, 4, device="cuda", generator=gen)
+        calls.append(lambda h=h, idx=idx, w=w: (int4_routed(h, idx, w, ex), int4_gemm(h, wt)))
+    want = [c() for c in calls]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for r in range(6):
+        for i, c in enumerate(calls):
+            with torch.cuda.stream(streams[(i + r) % 2]):
+                got.append((i, c()))
+    torch.cuda.synchronize()
+    for i, g in got:
+        assert torch.equal(g[0], want[i][0]) and torch.equal(g[1], want[i][1])
+
+
 def test_non_finite_rows():
     """An infinity or NaN stays in its row."""
     from lazylora_amd.int4 import int4_gemm
