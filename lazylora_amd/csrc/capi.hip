@@ -1412,7 +1412,7 @@ int mxfp4_int4_moe_forward(void* out, const void* h, int dtype, const void* topk
   mx::Int4Args a = {};
   a.pairs = {topk_idx, idx_dtype == MXFP4_I64, N * k, k, E};
   a.act = act_kind;
-  a.by_token = mx::int4_by_token(N, D, F);
+  a.by_token = mx::int4_by_token(N, k, E, D, F);
   if (!a.by_token && a.pairs.P > mx::kInt4ScanPairs) {
     int* n_tiles = reinterpret_cast<int*>(base);
     int4* tiles = reinterpret_cast<int4*>(base + ws.tiles);

@@ -51,7 +51,7 @@ constexpr int kInt4ScanPairs = 64;  // up to so many pairs the products find the
 hipError_t launch_int4_route(const Int4Pairs& p, int4* tiles, int* n_tiles, int* order, hipStream_t s);
 // Whether a call of N tokens runs without routing, each pair by itself: launch_int4_glu with by_token, then
 // launch_int4_token.
-bool int4_by_token(int N, int D, int F);
+bool int4_by_token(int N, int k, int E, int D, int F);
 // h [P, R] = GLU(x W1^T, x W3^T) of each pair's expert.
 hipError_t launch_int4_glu(const Int4Args& a, int group, int dtype, hipStream_t s);
 // y [P, R] fp32 = x W^T of each pair's expert.

@@ -428,7 +428,8 @@ __global__ __launch_bounds__(64 * strip_waves(G, EPI, WIDE)) void int4_strip_ker
       if constexpr (WIDE) {
         const int at = in ? lane_s : kOob / 2, shared = row * groups + u * (2 * NG);
         if constexpr (NG == 4) {
-          const i32x4 v = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(w[m].s, 2 * at, 2 * shared, 0));
+          const i32x4 v =
+              __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(w[m].s, 2 * at, 2 * shared, 0));
 #pragma unroll
           for (int i = 0; i < 4; ++i) t.s[m][i] = v[i];
           if (ZP) {
@@ -843,7 +844,8 @@ hipError_t launch_strip(Int4Args a, int tiles, hipStream_t s)
 {
   constexpr int NMAT = EPI == kInt4Glu ? 2 : 1;
   const int most_waves = strip_waves(G, EPI, a.K % 256 == 0);
-  const int units = (a.K + 255) / 256, rounds = (units + most_waves - 1) / most_waves, waves = (units + rounds - 1) / rounds;
+  const int units = (a.K + 255) / 256, rounds = (units + most_waves - 1) / most_waves;
+  const int waves = (units + rounds - 1) / rounds;
   const auto kernel = a.K % 256 == 0 ? int4_strip_kernel<T, G, ZP, EPI, true> : int4_strip_kernel<T, G, ZP, EPI, false>;
   const int all = (a.R + 15) / 16;
   const long long full = 256 * 16 / waves;
@@ -954,10 +956,13 @@ hipError_t launch_routed(const Int4Args& a, int group, int dtype, hipStream_t s)
   // as many tiles as there are likely to be, of weight rows as wide as a dense product's
   const int likely = P / rows + min(P, a.pairs.E) / 2, wide = EPI == kInt4Glu ? 2 * a.R : a.R;
   Int4Form form = kStrip;
-  if (rows == 32)
-    form = fills_no_round(kTile218, likely, wide) ? kTile218 : fills_no_round(kTile224, likely, wide) ? kTile224 : kTile222;
-  else if (rows == 64)
-    form = fills_no_round(kTile424, likely, wide) ? kTile424 : fills_no_round(kTile442, likely, wide) ? kTile442 : kTile441;
+  if (rows == 32) {
+    form = fills_no_round(kTile224, likely, wide) ? kTile224 : kTile222;
+    if (fills_no_round(kTile218, likely, wide)) form = kTile218;
+  } else if (rows == 64) {
+    form = fills_no_round(kTile442, likely, wide) ? kTile442 : kTile441;
+    if (fills_no_round(kTile424, likely, wide)) form = kTile424;
+  }
   return launch_typed<EPI>(a, group, dtype, form, tiles, s);
 }
 
@@ -986,7 +991,15 @@ hipError_t launch_int4_route(const Int4Pairs& p, int4* tiles, int* n_tiles, int*
   return hipGetLastError();
 }
 
-bool int4_by_token(int N, int D, int F) { return N == 1 && min(D, F) >= kVecMinK; }
+// A few tokens' pairs have an expert each, as a rule, and go by themselves in two launches, where one row's products
+// read 1 KiB pieces; an expert that several of them name is read again, mostly from the caches. By tokens / by
+// experts, us: 8 of 64 experts, 7168 / 2048, 2 tokens 72 / 112, 4 121 / 168, 8 222 / 250, 16 439 / 301; 8 of 128,
+// 3584 / 1536, 2 32 / 50, 8 82 / 114, 16 161 / 156; 4 of 32, 2048 / 1024, 2 13 / 22, 8 24 / 31, 16 38 / 36; 2 of 8,
+// 4096 / 1024, 2 12 / 20, 8 (two pairs for each expert) 23 / 24, 16 36 / 30.
+bool int4_by_token(int N, int k, int E, int D, int F)
+{
+  return min(D, F) >= kVecMinK && (N == 1 || (N <= 8 && N * k <= 2 * E));
+}
 hipError_t launch_int4_glu(const Int4Args& a, int group, int dtype, hipStream_t s)
 {
   if (a.by_token) return launch_typed<kInt4Glu>(a, group, dtype, kVec1, a.pairs.P, s);

@@ -146,6 +146,9 @@ ROUTED = [  # N, k, E, D, F, group, zeros, dtype, act
     (150, 2, 2, 128, 128, 128, False, "bf16", "swiglu"), (1, 8, 12, 1024, 1152, 64, True, "bf16", "swiglu"),
     (1, 3, 4, 2176, 1024, 128, False, "f16", "situ"), (1, 11, 16, 1024, 1024, 32, False, "bf16", "situ"),
     (2, 8, 12, 1024, 1152, 64, True, "bf16", "swiglu"),
+    # by tokens up to 8 (pairs that share experts among them), by experts past 8 and where the pairs are many for the experts
+    (3, 8, 12, 1024, 1024, 64, True, "f16", "swiglu"), (8, 3, 12, 1280, 1024, 128, False, "bf16", "situ"),
+    (8, 4, 12, 1024, 1056, 32, True, "bf16", "swiglu"), (9, 2, 12, 1024, 1024, 64, False, "f16", "swiglu"),
     # 32 rows to a tile in each form (few, some, many weight rows), then 64
     (50, 2, 4, 96, 64, 32, True, "f16", "swiglu"), (50, 2, 4, 160, 1024, 32, False, "bf16", "swiglu"),
     (50, 2, 4, 128, 4096, 64, True, "bf16", "situ"), (50, 2, 4, 4096, 160, 32, False, "f16", "swiglu"),
