@@ -215,9 +215,13 @@ MX_DEV i32x4 load_codes(const Rows& w, uint32_t lane, uint32_t shared)
 {
   return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(w.q, (int)lane, (int)shared, 0));
 }
+// The byte offset of a scale, from its number: doubled without a sign, so that kOob / 2 becomes kOob (in an int that
+// overflows, and what the compiler may then assume of the number is that it is smaller).
+constexpr int scale_bytes(uint32_t number) { return (int)(2 * number); }
+static_assert((uint32_t)scale_bytes(kOob / 2) == kOob, "past every buffer");
 MX_DEV uint16_t load_scale(const Rows& w, uint32_t lane, uint32_t shared)
 {
-  return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(w.s, (int)(2 * lane), (int)(2 * shared), 0);
+  return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(w.s, scale_bytes(lane), scale_bytes(shared), 0);
 }
 MX_DEV uint8_t load_zero(const Rows& w, uint32_t lane, uint32_t shared)
 {
@@ -426,23 +430,23 @@ __global__ __launch_bounds__(64 * strip_waves(G, EPI, WIDE)) void int4_strip_ker
         t.q[m][b] = load_codes(w[m], there ? lane_q : kOob, row * (p.K / 2) + 128 * u + 64 * b);
       }
       if constexpr (WIDE) {
-        const int at = in ? lane_s : kOob / 2, shared = row * groups + u * (2 * NG);
+        const uint32_t at = in ? lane_s : kOob / 2, shared = row * groups + u * (2 * NG);
         if constexpr (NG == 4) {
-          const i32x4 v =
-              __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(w[m].s, 2 * at, 2 * shared, 0));
+          const i32x4 v = __builtin_bit_cast(
+              i32x4, __builtin_amdgcn_raw_buffer_load_b128(w[m].s, scale_bytes(at), scale_bytes(shared), 0));
 #pragma unroll
           for (int i = 0; i < 4; ++i) t.s[m][i] = v[i];
           if (ZP) {
-            const auto y = __builtin_amdgcn_raw_buffer_load_b64(w[m].z, at, shared, 0);
+            const auto y = __builtin_amdgcn_raw_buffer_load_b64(w[m].z, (int)at, (int)shared, 0);
             t.z[m][0] = y[0], t.z[m][1] = y[1];
           }
         } else if constexpr (NG == 2) {
-          const auto v = __builtin_amdgcn_raw_buffer_load_b64(w[m].s, 2 * at, 2 * shared, 0);
+          const auto v = __builtin_amdgcn_raw_buffer_load_b64(w[m].s, scale_bytes(at), scale_bytes(shared), 0);
           t.s[m][0] = v[0], t.s[m][1] = v[1];
-          if (ZP) t.z[m][0] = __builtin_amdgcn_raw_buffer_load_b32(w[m].z, at, shared, 0);
+          if (ZP) t.z[m][0] = __builtin_amdgcn_raw_buffer_load_b32(w[m].z, (int)at, (int)shared, 0);
         } else {
-          t.s[m][0] = __builtin_amdgcn_raw_buffer_load_b32(w[m].s, 2 * at, 2 * shared, 0);
-          if (ZP) t.z[m][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(w[m].z, at, shared, 0);
+          t.s[m][0] = __builtin_amdgcn_raw_buffer_load_b32(w[m].s, scale_bytes(at), scale_bytes(shared), 0);
+          if (ZP) t.z[m][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(w[m].z, (int)at, (int)shared, 0);
         }
       } else {
 #pragma unroll
@@ -594,12 +598,12 @@ __global__ __launch_bounds__(64 * WN * KS) void int4_tile_kernel(Int4Args p)
       k.q[t] = load_codes(w[t], WIDE || 128 * b + 32 * c < p.K ? lane_q[t] : kOob, 64 * b);
       const uint32_t at = lane_s[t];
       if constexpr (WIDE && NG == 4) {
-        const auto v = __builtin_amdgcn_raw_buffer_load_b64(w[t].s, 2 * at, 2 * NG * b, 0);
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(w[t].s, scale_bytes(at), scale_bytes(NG * b), 0);
         k.s[t][0] = v[0], k.s[t][1] = v[1];
-        if (ZP) k.z[t] = __builtin_amdgcn_raw_buffer_load_b32(w[t].z, at, NG * b, 0);
+        if (ZP) k.z[t] = __builtin_amdgcn_raw_buffer_load_b32(w[t].z, (int)at, NG * b, 0);
       } else if constexpr (WIDE && NG == 2) {
-        k.s[t][0] = __builtin_amdgcn_raw_buffer_load_b32(w[t].s, 2 * at, 2 * NG * b, 0);
-        if (ZP) k.z[t] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(w[t].z, at, NG * b, 0);
+        k.s[t][0] = __builtin_amdgcn_raw_buffer_load_b32(w[t].s, scale_bytes(at), scale_bytes(NG * b), 0);
+        if (ZP) k.z[t] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(w[t].z, (int)at, NG * b, 0);
       } else {
 #pragma unroll
         for (int i = 0; i < (NG + 1) / 2; ++i) k.s[t][i] = 0;
