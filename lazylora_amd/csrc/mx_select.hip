@@ -311,9 +311,7 @@ __global__ __launch_bounds__(256, PER <= 4 ? 8 : 1) void select_kernel(SelectArg
     } else if (a.bias) {
       err = s_err + 0x1p-22f * fabsf(key_value(k1));
     }
-    // a group's rank, and whether another group on the other side of the line is too close to tell
-    const float gv = key_value(gk);
-    int rank = 0;
+    int rank = 0;  // a group's
     const int place = lane & (at.run - 1), start = lane - place;
     for (int g0 = 0; g0 < a.num_groups; g0 += at.run) {  // a run's lanes compare with a group each
       const int g = g0 + place;
@@ -323,13 +321,14 @@ __global__ __launch_bounds__(256, PER <= 4 ? 8 : 1) void select_kernel(SelectArg
       rank += __popcll(at.run == 64 ? votes : votes & ((1ull << at.run) - 1));
     }
     on = on && rank < a.topk_groups;
-    if (a.top2 || a.bias) {
-      // the last kept group's value against the others'
-      const uint64_t edge = __builtin_amdgcn_ballot_w64(rank == a.topk_groups - 1 && at.group < a.num_groups);
-      const int el = __builtin_ctzll(edge | (1ull << 63));
-      const float ev = lane_f(gv, el), ee = lane_f(err, el);
-      const bool close = at.group < a.num_groups && rank >= a.topk_groups && ev - gv <= ee + err;
-      if (__builtin_amdgcn_ballot_w64(close) != 0) on = Careful<T>(a, row, at, score.top, lane).group_on();
+    if ((a.top2 || a.bias) && a.topk_groups < a.num_groups) {
+      // The kept groups' least possible value against the others' largest: any kept group may be the one whose error
+      // (of a sum of two that cancel, say) kept it.
+      const float gv = key_value(gk);
+      const bool here = at.group < a.num_groups, kept = rank < a.topk_groups, finite = fabsf(gv) < __builtin_inff();
+      const uint32_t lo = finite ? order_key(gv - err) : 0u, hi = finite ? order_key(gv + err) : 0xFFFFFFFFu;
+      const uint32_t low = ~wave_max(here & kept ? ~lo : 0u), high = wave_max(here & !kept ? hi : 0u);
+      if (low <= high) on = Careful<T>(a, row, at, score.top, lane).group_on();
     }
     static_for<PER>([&](auto mc) { key[decltype(mc)::value] = on ? key[decltype(mc)::value] : 0u; });
   }
