@@ -296,20 +296,21 @@ __global__ __launch_bounds__(256, PER <= 4 ? 8 : 1) void select_kernel(SelectArg
       k1 = max(k1, key[m]);
     });
     run_top2(k1, k2, at.run);
-    float err = 0.f;
+    // the group's value, its error, and whether it is infinite or NaN because a choice in it is
+    const auto endless = [](float v) { return !(fabsf(v) < __builtin_inff()); };
+    float c1 = key_value(k1), c2 = key_value(k2);
+    if (scores) c1 = quick(c1), c2 = quick(c2);
     uint32_t gk = k1;
+    bool exact = endless(c1);
+    float err = s_err + 0x1p-22f * fabsf(c1);
     if (a.top2) {
-      float c1 = key_value(k1), c2 = key_value(k2);
-      if (scores) c1 = quick(c1), c2 = quick(c2);
       if (k2 != 0) {
         gk = order_key(c1 + c2);
+        exact |= endless(c2);
         err = 2.f * s_err + 0x1p-21f * (fabsf(c1) + fabsf(c2));
-      } else if (k1 != 0) {
+      } else {
         gk = order_key(c1);
-        err = s_err + 0x1p-22f * fabsf(c1);
       }
-    } else if (a.bias) {
-      err = s_err + 0x1p-22f * fabsf(key_value(k1));
     }
     int rank = 0;  // a group's
     const int place = lane & (at.run - 1), start = lane - place;
@@ -323,12 +324,15 @@ __global__ __launch_bounds__(256, PER <= 4 ? 8 : 1) void select_kernel(SelectArg
     on = on && rank < a.topk_groups;
     if ((a.top2 || a.bias) && a.topk_groups < a.num_groups) {
       // The kept groups' least possible value against the others' largest: any kept group may be the one whose error
-      // (of a sum of two that cancel, say) kept it.
+      // (of a sum of two that cancel, say) kept it. An infinity or NaN among the choices is exact, and equal ones go
+      // by their number; a sum of finite ones that 32 bits cannot hold lies past 2^127.
       const float gv = key_value(gk);
-      const bool here = at.group < a.num_groups, kept = rank < a.topk_groups, finite = fabsf(gv) < __builtin_inff();
-      const uint32_t lo = finite ? order_key(gv - err) : 0u, hi = finite ? order_key(gv + err) : 0xFFFFFFFFu;
-      const uint32_t low = ~wave_max(here & kept ? ~lo : 0u), high = wave_max(here & !kept ? hi : 0u);
-      if (low <= high) on = Careful<T>(a, row, at, score.top, lane).group_on();
+      const bool here = at.group < a.num_groups, kept = rank < a.topk_groups;
+      const float below = gv == __builtin_inff() ? 0x1p127f : gv - err, above = gv == -__builtin_inff() ? -0x1p127f : gv + err;
+      const uint32_t low = ~wave_max(here & kept ? ~(exact ? gk : order_key(below)) : 0u);
+      const uint32_t high = wave_max(here & !kept ? exact ? gk : order_key(above) : 0u);
+      if (low < high || (low == high && fabsf(key_value(low)) < __builtin_inff()))
+        on = Careful<T>(a, row, at, score.top, lane).group_on();
     }
     static_for<PER>([&](auto mc) { key[decltype(mc)::value] = on ? key[decltype(mc)::value] : 0u; });
   }
@@ -362,7 +366,7 @@ __global__ __launch_bounds__(256, PER <= 4 ? 8 : 1) void select_kernel(SelectArg
     const float v = key_value(mine_key);
     const float err = s_err + 0x1p-22f * fabsf(v);
     const float next = key_value((uint32_t)__shfl_down((int)mine_key, 1, 64));
-    const bool pair = lane < a.top_k - 1 && v - next <= err;
+    const bool pair = lane < a.top_k - 1 && v - next <= err && fabsf(v) < __builtin_inff();
     const float vl = lane_f(v, a.top_k - 1), el = lane_f(err, a.top_k - 1);
     const uint32_t line = vl - el == vl - el && fabsf(vl) < __builtin_inff() ? order_key(vl - el) : 0xFFFFFFFFu;
     if (__builtin_amdgcn_ballot_w64(pair) != 0 || __builtin_amdgcn_ballot_w64(best >= line) != 0) {
