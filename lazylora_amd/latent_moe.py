@@ -142,7 +142,11 @@ class LatentMoEBlock:
         if not isinstance(self.experts, Int4Experts):
             return RoutedExpertsFunction.apply(h_latent, w, idx, self.experts, self.act, cached, self._routed_lora())
         if cached is not None:
-            return cached
+            # nothing recorded with the call that made it, and nothing here, would carry a gradient to h_latent or w
+            if torch.is_grad_enabled() and (h_latent.requires_grad or w.requires_grad):
+                raise NotImplementedError("the products with 4-bit integer weights have no backward pass: call the block "
+                                          "under torch.no_grad() or on detached tensors, with cached as without")
+            return cached.to(torch.float32)
         return int4_routed(h_latent.to(self.experts.dtype), idx, w, self.experts, self.act).float()
 
     def forward(self, h_moe_norm: torch.Tensor, cached: Optional[torch.Tensor] = None, dropout_seed=None
