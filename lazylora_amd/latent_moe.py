@@ -103,8 +103,7 @@ class LatentMoEBlock:
         self.top_k, self.routed_scaling_factor, self.renormalize = top_k, routed_scaling_factor, renormalize
         self.act, self.rms_eps, self.lora = act, rms_eps, lora
         self.scoring, self.num_groups, self.topk_groups, self.group_score = scoring, num_groups, topk_groups, group_score
-        if isinstance(experts, Int4Experts) and self._routed_lora() is not None:
-            raise ValueError("routed adapters need an ExpertLayer: the products with 4-bit integer weights take none")
+        self._check_adapters()
         H = self.gate_weight.shape[1]
         if self.latent_down.shape != (experts.D, H) or self.latent_up.shape != (H, experts.D):
             raise ValueError(f"latent projections must be [{experts.D}, {H}] and [{H}, {experts.D}]")
@@ -137,10 +136,15 @@ class LatentMoEBlock:
             return y.float()
         return y.float() + delta(s_act.float(), "shared_down_lora", 2)
 
+    def _check_adapters(self) -> None:
+        if isinstance(self.experts, Int4Experts) and self._routed_lora() is not None:
+            raise ValueError("routed adapters need an ExpertLayer: the products with 4-bit integer weights take none")
+
     def _routed(self, h_latent: torch.Tensor, w: torch.Tensor, idx: torch.Tensor, cached) -> torch.Tensor:
         """The routed experts' sum, fp32 (`cached`: an earlier call's)."""
         if not isinstance(self.experts, Int4Experts):
             return RoutedExpertsFunction.apply(h_latent, w, idx, self.experts, self.act, cached, self._routed_lora())
+        self._check_adapters()
         if cached is not None:
             # nothing recorded with the call that made it, and nothing here, would carry a gradient to h_latent or w
             if torch.is_grad_enabled() and (h_latent.requires_grad or w.requires_grad):

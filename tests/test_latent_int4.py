@@ -46,3 +46,18 @@ def test_cached_sum_without_a_gradient(block):
     # in any floating type, as with an ExpertLayer
     low = cached.bfloat16()
     torch.testing.assert_close(block(x, cached=low)[0], block._shared(x, None) + low.float() @ block.latent_up.T)
+
+
+def test_routed_adapters_are_refused_whenever_they_come(block):
+    """`lora` may be set on a block that is there already: routed adapters are not left out of the sum in silence."""
+    class Adapter:
+        lora_A, lora_B, scaling, dropout_rate = torch.zeros(4, Dl), torch.zeros(F, 4), 1.0, 0.0
+
+    class Bundle:
+        gate_lora = up_lora = down_lora = Adapter()
+
+    block.lora = Bundle()
+    with torch.no_grad(), pytest.raises(ValueError, match="adapters"):
+        block(torch.randn(3, H))
+    with torch.no_grad(), pytest.raises(ValueError, match="adapters"):
+        block(torch.randn(3, H), cached=torch.randn(3, Dl))
