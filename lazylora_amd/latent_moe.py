@@ -32,7 +32,7 @@ from lazylora_amd.dense import rms_norm as native_rms_norm
 from lazylora_amd.experts import ExpertLayer
 from lazylora_amd.int4 import Int4Experts, int4_routed
 from lazylora_amd.routed import RoutedExpertsFunction
-from lazylora_amd.router import route
+from lazylora_amd.router import check_options, route
 
 SITU_BETA, SITU_LINEAR_BETA = 4.0, 25.0  # lazy_lora/core/situ_activation.py:22-23
 
@@ -92,6 +92,7 @@ class LatentMoEBlock:
                  num_groups: int = 1, topk_groups: Optional[int] = None, group_score: str = "top2"):
         if dense not in ("torch", "native"):
             raise ValueError(f'dense must be "torch" or "native", got {dense!r}')
+        check_options(scoring, group_score)
         dev = experts.device
         f32 = lambda t: None if t is None else torch.as_tensor(t).to(dev, torch.float32)
         self.experts = experts

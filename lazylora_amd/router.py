@@ -60,6 +60,13 @@ class _Select(torch.autograd.Function):
         return grad_logits, None, None, None, None
 
 
+def check_options(scoring: str, group_score: str) -> None:
+    if not (isinstance(scoring, str) and scoring in SCORINGS):
+        raise ValueError(f"unknown scoring {scoring!r}")
+    if not (isinstance(group_score, str) and group_score in GROUP_SCORES):
+        raise ValueError(f"unknown group score {group_score!r}")
+
+
 def select_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor] = None, scoring: str = "sigmoid",
                    num_groups: int = 1, topk_groups: Optional[int] = None, group_score: str = "top2",
                    renormalize: bool = True, routed_scaling_factor: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -77,10 +84,7 @@ def select_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor
     softmax row of -inf alone has weights 0. E <= 4096 (where num_groups is no power of two, 64 * 64 experts
     for the next power of two of groups), num_groups <= 64, top_k <= min(64, experts of the kept groups).
     Second derivatives, forward-mode differentiation and tracing raise, as in lazylora_amd.dense."""
-    if scoring not in SCORINGS:
-        raise ValueError(f"unknown scoring {scoring!r}")
-    if group_score not in GROUP_SCORES:
-        raise ValueError(f"unknown group score {group_score!r}")
+    check_options(scoring, group_score)
     return _module().select_experts(logits, bias, top_k, SCORINGS[scoring], num_groups,
                             num_groups if topk_groups is None else topk_groups, GROUP_SCORES[group_score],
                             routed_scaling_factor, renormalize)
@@ -94,6 +98,7 @@ def route(x: Union[torch.Tensor, np.ndarray], weight: Union[torch.Tensor, np.nda
     weight [E, hidden] (moe_router.py:81-99). NumPy in, NumPy out; torch tensors come back on
     x's device. scoring, num_groups, topk_groups and group_score as in select_experts, which makes the
     selection unless they are the reference's (sigmoid, one group)."""
+    check_options(scoring, group_score)
     as_numpy = isinstance(x, np.ndarray)
     xt = torch.from_numpy(np.asarray(x, np.float32)) if as_numpy else x
     if xt.is_cuda:
@@ -132,6 +137,7 @@ class KimiK3MoERouter(nn.Module):
                  routed_scaling_factor: float = 1.0, renormalize: bool = True, use_bias: bool = True,
                  device: Optional[Union[str, torch.device]] = None, scoring: str = "sigmoid", num_groups: int = 1,
                  topk_groups: Optional[int] = None, group_score: str = "top2"):
+        check_options(scoring, group_score)
         super().__init__()
         self.weight = nn.Parameter(torch.empty(num_experts, hidden_size, device=device))
         self.bias = nn.Parameter(torch.zeros(num_experts, device=device)) if use_bias else None
