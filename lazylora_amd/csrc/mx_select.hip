@@ -6,9 +6,10 @@
 // descending order, equal ones and equal groups by the lower number first; weights s, renormalised by
 // their sum + 1e-20 and scaled.
 //
-// Which experts are chosen is that of exact arithmetic, not of its 32-bit rounding: sums of 32-bit
-// scores and biases that lie closer than their error are decided in 64 bits. Without that some token in a
-// thousand (top-16 of 896) would get its experts in another order than the formula gives.
+// Without a bias the order is that of the logits. With one, and between groups by sums of two, it is that of
+// 64-bit scores and sums on the 32-bit bias: 32-bit values that lie closer than their error are decided in 64
+// bits. Without that some token in a thousand (top-16 of 896) would get its experts in another order than the
+// formula gives. What 64 bits hold as equal (sigmoid(38) and sigmoid(45), say) is equal and goes by the number.
 #include "mx_device.h"
 #include "mx_select.h"
 

@@ -74,14 +74,14 @@ def select_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor
     bfloat16 or float16, on the HIP device), differentiable in the logits.
 
     Scores are sigmoid(logits) or softmax(logits) (`scoring`); the choice goes by score + bias (bias [E] of any
-    floating type, for the choice only: no gradient), the weights are the chosen scores, divided by their sum +
+    floating type, float64 too taken as float32; for the choice only: no gradient), the weights are the chosen scores, divided by their sum +
     1e-20 with `renormalize` (and top_k > 1), times routed_scaling_factor. With num_groups > 1 the experts form
     that many equal runs and only the topk_groups best of them (None: all) can be chosen from, by the sum of
     each group's two largest values of score + bias (group_score "top2") or by its largest ("max").
 
-    Indices are in descending order of score + bias, as exact arithmetic on the given numbers has it (without a
-    bias: of the logits); equal values go to the lower id, equal groups to the lower number, NaN comes first. A
-    softmax row of -inf alone has weights 0. E <= 4096 (where num_groups is no power of two, 64 * 64 experts
+    Indices are in descending order of score + bias in 64 bits (without a bias: of the logits), and so are the
+    groups; values that are equal there, as sigmoid(38) and sigmoid(45) under one bias are, go to the lower id,
+    equal groups to the lower number, NaN comes first. A softmax row of -inf alone has weights 0. E <= 4096 (where num_groups is no power of two, 64 * 64 experts
     for the next power of two of groups), num_groups <= 64, top_k <= min(64, experts of the kept groups).
     Second derivatives, forward-mode differentiation and tracing raise, as in lazylora_amd.dense."""
     check_options(scoring, group_score)

@@ -101,3 +101,19 @@ def test_infinite_groups_on_both_sides(select, group_score):
                 bias[8 * g:8 * g + rng.integers(1, 9)] = value
             run(select, x, "f32", bias, top_k=6, num_groups=8, topk_groups=4, group_score=group_score)
             run(select, x, "f32", bias, top_k=6, scoring="softmax", num_groups=8, topk_groups=4, group_score=group_score)
+
+
+def test_saturated_scores(select):
+    """Scores that 64 bits hold as equal: without a bias the order is the logits', with one the ids' (written down
+    here, not computed); a 64-bit bias counts as its 32-bit value."""
+    x = torch.tensor([[45.0, 38.0, 50.0, 40.0, -60.0, -42.0, -50.0, 0.0]], device="cuda")
+    pick = lambda b, k=8: select(x, k, b, renormalize=False)[0][0].tolist()
+    assert pick(None) == [2, 0, 3, 1, 7, 5, 6, 4]
+    assert pick(torch.zeros(8, device="cuda")) == [0, 1, 2, 3, 7, 5, 6, 4]  # small scores differ, those next to 1 do not
+    assert pick(torch.full((8,), 0.02, device="cuda")) == [0, 1, 2, 3, 7, 4, 5, 6]
+    # 1 - 9.4e-14 and 1 - 3.4e-14 differ in 64 bits, though not in 32
+    y = torch.tensor([[30.0, 31.0, 30.5, -1.0]], device="cuda")
+    assert select(y, 3, torch.zeros(4, device="cuda"))[0][0].tolist() == [1, 2, 0]
+    b = torch.zeros(8, device="cuda", dtype=torch.float64)
+    b[3] = 2.0 ** -30
+    assert pick(1 + b) == pick(torch.ones(8, device="cuda")) and pick(b)[0] == 3
