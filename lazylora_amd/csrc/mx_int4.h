@@ -38,7 +38,6 @@ struct Int4Args {
   // set by the launcher: work-groups over the weight rows, the first row tile (pair, token) of this launch; of the
   // few-row form the batches of weight rows of a work-group and the waves that share a row of K
   int row_groups, tile0, batches, team;
-  bool wide;  // the scales of 256 codes can be loaded at once
 };
 
 // y [M, R] = x [M, K] W^T (dtype MXFP4_BF16 or _F16).
