@@ -346,7 +346,9 @@ int mxfp4_select_topk_backward(void *grad_logits, const int64_t *topk_idx, const
  * dtype (MXFP4_BF16 or _F16), zeros [R, K / group] bytes or NULL (8 everywhere);
  *   W[r, k] = scales[r, k / group] * (code[r, k] - zeros[r, k / group]).
  * group 32, 64 or 128, K a multiple of it; K and R at most 2^20. All pointers 16-byte aligned. Codes enter
- * the products exactly, sums are fp32 and every result is rounded once (an infinity in a row of x gives NaN).
+ * the products exactly, sums are fp32 and every result is rounded once. An infinity in a row of x gives NaN; finite
+ * rows stay finite while the sum of |x| max(31, 16 + zero) over a group is below 2^127 (every |x| below 2^111, always in
+ * MXFP4_F16), and scaled below fp32's largest number. A scale that is not finite gives such results in its row of W.
  * No atomics on values: results do not depend on timing.
  *
  * y [M, R] = x [M, K] . W^T, M at most 2^24. */
@@ -355,7 +357,8 @@ int mxfp4_int4_gemm(void *y, const void *x, const uint8_t *packed, const void *s
 
 /* The routed expert layer over such weights:
  *   out[t] = sum over slots of topk_w[t, j] W2_e . GLU(W1_e . h[t], W3_e . h[t]), e = topk_idx[t, j],
- * h and out [N, D] of dtype, the GLU's results rounded to dtype in between. codes, scales and zeros: host
+ * h and out [N, D] of dtype, the GLU's results rounded to dtype in between (in MXFP4_F16 one past 65504 becomes an
+ * infinity, and the token's row NaN: SwiGLU in MXFP4_BF16 or SiTU, which is below 100, do not reach that). codes, scales and zeros: host
  * arrays of 3 device pointers, W1 and W3 [E, F, D] and W2 [E, D, F] stacked expert-major (zeros may be NULL, or
  * hold three NULLs). topk_idx [N, k] MXFP4_I32 or _I64, ids outside [0, E) contribute nothing; topk_w [N, k] fp32.
  * D and F multiples of group, E at most 4096, N k at most 2^24, N D at most 2^32. The 256-byte aligned

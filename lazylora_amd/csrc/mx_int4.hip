@@ -5,7 +5,9 @@
 // an operand of ones, x itself over a group; then
 //   sum x (q - z) = sum x (16 + q) - (16 + z) sum x,
 // all exact products in fp32 sums, and one multiply-add by the group's scale per result. A row of x with an
-// infinity gives NaN (the difference of two infinities).
+// infinity gives NaN (the difference of two infinities), and so does one whose sums pass 32 bits: a group's
+// sum of |x| max(31, 16 + z) has to stay below 2^127, which float16 cannot reach and bfloat16 only where |x|
+// passes 2^111 in all 128 places (any zero point). An infinite or NaN scale gives such results in its weight row.
 #include "mx_device.h"
 #include "mx_int4.h"
 

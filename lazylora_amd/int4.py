@@ -88,14 +88,16 @@ class Int4Experts:
 
 def int4_gemm(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
     """y [..., R] = x [..., K] W^T, x and y of the scales' type (bfloat16 or float16). A row of x with an infinity
-    gives NaN."""
+    gives NaN, and so does one with numbers past fp32's range in the sum of |x| max(31, 16 + zero) over a group (none
+    below 2^111 is, and no float16). Scales have to be finite."""
     return _module().int4_gemm(x, weight.packed, weight.scales, weight.zeros)
 
 
 def int4_routed(h: torch.Tensor, topk_indices: torch.Tensor, topk_weights: torch.Tensor, experts: Int4Experts,
                 act: str = "swiglu") -> torch.Tensor:
     """sum over the slots j of topk_weights[t, j] * W2_e GLU(W1_e h[t], W3_e h[t]), e = topk_indices[t, j], for h
-    [N, D] of the scales' type; the result is of that type too, and so are the GLU's results in between.
+    [N, D] of the scales' type; the result is of that type too, and so are the GLU's results in between (a SwiGLU
+    value past float16's 65504 is an infinity, and the token's result NaN; bfloat16 and "situ" do not reach that).
     topk_indices int32 or int64 [N, k], as the router gives them (ids outside [0, E) contribute nothing),
     topk_weights [N, k] of any floating type; act "swiglu" or "situ"."""
     if act not in _ACTS:

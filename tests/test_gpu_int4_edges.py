@@ -60,3 +60,49 @@ def test_routed_waves_without_a_last_unit(group, dtype):
             np.add.at(tol, t, ws[t, j, None] * (hidden + sums))
         tol += eps / 2 * (np.abs(want) + tol) + torch.finfo(dt).tiny
         assert (np.abs(got - want) <= tol).all(), zeros
+
+
+# every form: one, two and four rows, 16 rows, and the tiles'
+FORMS = [(1, 1152, 40), (2, 1152, 40), (4, 1152, 40), (6, 1152, 40), (20, 1152, 40), (64, 1152, 2100), (200, 384, 2100),
+         (300, 384, 2100), (600, 384, 2100), (1100, 128, 2100)]
+
+
+@pytest.mark.parametrize("M,K,R", FORMS)
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_largest_numbers(M, K, R, group):
+    """Rows of numbers up to 2^112 with every zero point: a group's sums stay in 32 bits, whatever the signs."""
+    from lazylora_amd.int4 import Int4Weight, int4_gemm
+    gen, dt = gen_of(M, K, group), torch.bfloat16
+    x = (2.0 ** 111 * (1 + torch.rand(M, K, device="cuda", generator=gen))).to(dt)
+    x[x > 2.0 ** 112] = 2.0 ** 112
+    x[M // 2:] *= 1 - 2 * torch.randint(0, 2, (M - M // 2, K), device="cuda", generator=gen)
+    packed = torch.randint(0, 256, (R, K // 2), device="cuda", generator=gen, dtype=torch.uint8)
+    scales = (2.0 ** torch.randint(-120, -110, (R, K // group), device="cuda", generator=gen).float()).to(dt)
+    zeros = torch.randint(0, 256, scales.shape, device="cuda", generator=gen, dtype=torch.uint8)
+    zeros[0] = 255
+    w = Int4Weight(packed, scales, zeros)
+    xs = x.double().cpu().numpy()
+    want = xs @ dense64(w).T
+    # as bound(), with 31 of a code and 16 + z of the sum
+    each = (47 + zeros.double().cpu().numpy()) * scales.double().cpu().numpy()
+    tol = ((K / 4 + 16) * 2.0 ** -24 * (np.abs(xs) @ np.repeat(each, group, -1).T) + torch.finfo(dt).eps / 2 * np.abs(want)
+           + torch.finfo(dt).tiny)
+    assert (np.abs(int4_gemm(x, w).double().cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.parametrize("M,K,R", FORMS)
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_scales_that_are_not_finite(M, K, R, value):
+    """Their rows of weights give infinities or NaN, the others what they give without them."""
+    from lazylora_amd.int4 import int4_gemm
+    gen = gen_of(M, K, R)
+    for k in (K, K + 32):  # also in a last block that is not full
+        x = torch.randn(M, k, device="cuda", generator=gen).half()
+        w = weight(gen, (), R, k, 32, True, torch.float16)
+        want = int4_gemm(x, w)
+        rows = torch.tensor([0, R // 2, R - 1], device="cuda")
+        w.scales[rows, torch.tensor([0, 1, k // 32 - 1], device="cuda")] = value
+        got = int4_gemm(x, w)
+        clean = torch.ones(R, dtype=torch.bool, device="cuda")
+        clean[rows] = False
+        assert not torch.isfinite(got[:, rows]).any() and torch.equal(got[:, clean], want[:, clean])
