@@ -64,8 +64,9 @@ inline bool records(at::ArrayRef<Tensor> ts)
   return false;
 }
 // A launch computes values and records nothing: it would drop a tensor's forward-mode tangent, which says that
-// the derivative along it is zero, and a tracer would see the outputs allocated but not filled. Every call and
-// every backward pass looks for both first.
+// the derivative along it is zero, and a tracer would see the outputs allocated but not filled. The tensors of a
+// function transform (vmap, batched gradients, torch.func.grad, functionalize) have no memory to launch over. Every
+// call and every backward pass looks for these first.
 inline void check_modes(at::ArrayRef<Tensor> ts)
 {
   using c10::impl::TorchDispatchModeTLS;
@@ -75,6 +76,12 @@ inline void check_modes(at::ArrayRef<Tensor> ts)
                        TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
   TORCH_CHECK_NOT_IMPLEMENTED(!traced, "the operators of this package cannot be traced (torch.jit.trace, make_fx, "
                                        "torch.export): a trace would not hold their launches");
+  constexpr c10::DispatchKeySet transformed({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                             c10::DispatchKey::Functionalize});
+  for (const Tensor& t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t.key_set().has_any(transformed),
+                                "the operators of this package cannot be transformed (torch.func.vmap, grad, functionalize, "
+                                "batched gradients)");
   for (const Tensor& t : ts)
     TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
                                 "the operators of this package have no forward-mode derivative (an input or upstream gradient "
