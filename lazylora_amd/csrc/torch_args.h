@@ -76,8 +76,9 @@ inline void check_modes(at::ArrayRef<Tensor> ts)
                        TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
   TORCH_CHECK_NOT_IMPLEMENTED(!traced, "the operators of this package cannot be traced (torch.jit.trace, make_fx, "
                                        "torch.export): a trace would not hold their launches");
-  constexpr c10::DispatchKeySet transformed({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
-                                             c10::DispatchKey::Functionalize});
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet transformed({DispatchKey::Batched, DispatchKey::FuncTorchBatched,
+                                             DispatchKey::FuncTorchGradWrapper, DispatchKey::Functionalize});
   for (const Tensor& t : ts)
     TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t.key_set().has_any(transformed),
                                 "the operators of this package cannot be transformed (torch.func.vmap, grad, functionalize, "
