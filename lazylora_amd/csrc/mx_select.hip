@@ -407,11 +407,17 @@ __global__ __launch_bounds__(256, PER <= 4 ? 8 : 1) void select_kernel(SelectArg
 
 // The gradient of the weights with respect to the logits, one wave per token. With chosen scores s_j, S =
 // sum s_j + 1e-20, upstream g and the factor c:
-//   ds_j = c (g_j - sum_i g_i s_i / S) / S   (renormalised),   c g_j   (otherwise);
+//   ds_j = c (sum_i s_i (g_j - g_i) + 1e-20 g_j) / S^2   (renormalised),   c g_j   (otherwise);
 //   sigmoid: dl_e = ds_e s_e (1 - s_e) at the chosen experts, 0 elsewhere;
 //   softmax: dl_e = s_e (ds_e - d) with d = sum_j ds_j s_j, at every expert. Renormalised, d is
-//   c (sum g s) 1e-20 / S^2: written so, not as the difference of nearly equal sums.
-// A token's ds meet its experts through a row of LDS. 4099 tokens of 64 experts 4.5 us, 1024 of 896 7.7.
+//   c (sum g s) 1e-20 / S^2; otherwise ds_j - d at a chosen expert is
+//   c (sum_i s_i (g_j - g_i) + g_j times the scores not chosen).
+// The sums go over differences of the upstream gradients: where one expert has nearly all of the score its own
+// gradient is as small as the others' scores, and g_j - sum_i g_i s_i / S would leave the rounding of g_j.
+// A token's ds meet its experts through a row of LDS, -0 where an expert is not chosen. 4099 tokens of 64 experts
+// 4.5 us, 1024 of 896 7.7.
+constexpr float kNotChosen = -0.f;
+MX_DEV bool not_chosen(float v) { return f_bits(v) == 0x80000000u; }
 template <typename T, int PER>
 __global__ __launch_bounds__(256) void select_bwd_kernel(SelectBwdArgs a)
 {
@@ -430,7 +436,7 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelectBwdArgs a)
     x[m] = -__builtin_inff();
     if (e < a.E) {
       x[m] = load_logit<T>(row + e);
-      ds_row[e] = 0.f;
+      ds_row[e] = kNotChosen;
     }
   });
   Score<float> score{a.softmax, 0.f, 1.f};
@@ -455,14 +461,28 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelectBwdArgs a)
     }
   }
   const float gs = wave_sum(g * s);
-  float ds = g, d = gs;
+  float diff = 0.f;  // sum_i s_i (g - g_i)
+  for (int i = 0; i < a.top_k; ++i) diff = fmaf(lane_f(s, i), g - lane_f(g, i), diff);
+  float ds = g, d = gs;  // of softmax ds - d at the chosen experts
   if (a.renormalize) {
     const float den = wave_sum(s) + 1e-20f;
-    ds = (g - gs / den) / den;
     d = gs * (1e-20f / den) / den;
+    ds = fmaf(1e-20f, g, diff) / den / den;
+    if (a.softmax) ds -= d;
+  } else if (a.softmax) {
+    wave_lds_fence();
+    if (e >= 0) ds_row[e] = 0.f;
+    wave_lds_fence();
+    float left = 0.f;
+    static_for<PER>([&](auto mc) {
+      constexpr int m = decltype(mc)::value;
+      const int i = lane + 64 * m;
+      if (i < a.E && not_chosen(ds_row[i])) left += expf(x[m] - score.top);
+    });
+    ds = fmaf(g, wave_sum(left) / score.sum, diff);
   }
   wave_lds_fence();
-  if (e >= 0) ds_row[e] = ds;
+  if (e >= 0) ds_row[e] = ds + 0.f;  // never -0
   wave_lds_fence();
   static_for<PER>([&](auto mc) {
     constexpr int m = decltype(mc)::value;
@@ -471,7 +491,7 @@ __global__ __launch_bounds__(256) void select_bwd_kernel(SelectBwdArgs a)
       const float t = ds_row[i];
       float v;
       if (a.softmax) {
-        v = score(x[m]) * (t - d);
+        v = score(x[m]) * (not_chosen(t) ? -d : t);
       } else {
         // 1 - s as the other side's sigmoid, without the cancellation of 1 - s
         v = t == 0.f ? 0.f : t * score(x[m]) * score(-x[m]);

@@ -117,3 +117,60 @@ def test_saturated_scores(select):
     b = torch.zeros(8, device="cuda", dtype=torch.float64)
     b[3] = 2.0 ** -30
     assert pick(1 + b) == pick(torch.ones(8, device="cuda")) and pick(b)[0] == 3
+
+
+def grads64(x, g, idx, scoring, renormalize, scale):
+    """(dL/dlogits, size of what is added) in 64 bits, with the differences of the upstream gradients taken before they
+    are weighted: dL/ds_j of the renormalised weights is (sum_i s_i (g_j - g_i) + 1e-20 g_j) / S^2, and softmax's own
+    term likewise over all experts."""
+    N, E = x.shape
+    if scoring == "sigmoid":
+        s, rest = 1 / (1 + np.exp(-x)), 1 / (1 + np.exp(x))
+    else:
+        e = np.exp(x - x.max(1, keepdims=True))
+        s = e / e.sum(1, keepdims=True)
+    dx, size = np.zeros((N, E)), np.zeros((N, E))
+    for t in range(N):
+        c, u = s[t, idx[t]], scale * g[t]
+        out = np.ones(E, bool)
+        out[idx[t]] = False
+        diff = u[:, None] - u[None, :]
+        both = np.abs(u[:, None]) + np.abs(u[None, :])
+        np.fill_diagonal(both, 0)
+        a, b = (diff * c).sum(1), (both * c).sum(1)
+        if renormalize:
+            S = c.sum() + 1e-20
+            a, b, d = (a + 1e-20 * u) / S ** 2, (b + 1e-20 * np.abs(u)) / S ** 2, (u * c).sum() * 1e-20 / S ** 2
+        elif scoring == "sigmoid":
+            a, b, d = u, np.abs(u), 0.0
+        else:
+            left = s[t, out].sum()
+            a, b, d = a + u * left, b + np.abs(u) * left, (u * c).sum()
+        if scoring == "sigmoid":
+            dx[t, idx[t]], size[t, idx[t]] = (v * c * rest[t, idx[t]] for v in (a, b))
+        else:
+            dx[t], size[t] = -s[t] * d, s[t] * np.abs(u * c).sum() * (1e-20 / S ** 2 if renormalize else 1)
+            dx[t, idx[t]], size[t, idx[t]] = c * (a - d if renormalize else a), c * (b + abs(d) * renormalize)
+    return dx, size
+
+
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("E,top_k", [(8, 1), (8, 2), (64, 6), (300, 16), (1024, 64), (4096, 5)])
+def test_gradients_of_confident_routers(select, scoring, renormalize, E, top_k):
+    """Rows in which one expert has nearly all of the score: its gradient is as small as the others' scores, and is
+    right to 32 bits of that, not of the upstream gradient."""
+    rng = np.random.default_rng(E + top_k)
+    x = rng.standard_normal((24, E)).astype(np.float32)
+    for t in range(24):
+        x[t] -= 0.75 * t * (scoring == "sigmoid")
+        x[t, rng.integers(E)] += 0.75 * t
+    g = rng.standard_normal((24, top_k)).astype(np.float32)
+    logits = torch.from_numpy(x).cuda().requires_grad_(True)
+    idx, w = select(logits, top_k, scoring=scoring, renormalize=renormalize, routed_scaling_factor=2.5)
+    got = torch.autograd.grad(w, logits, torch.from_numpy(g).cuda())[0].double().cpu().numpy()
+    want, size = grads64(x.astype(np.float64), g.astype(np.float64), idx.cpu().numpy(), scoring, renormalize and top_k > 1, 2.5)
+    # scores as in W_TOL (their exponents' rounding up to 2^-24 times the distance of a logit from the largest, 32 where
+    # they matter), three of them in a product, the sums of 64 and of 4096 / 64 terms in a row
+    tol = 1024 * 2.0 ** -24
+    assert (np.abs(got - want) <= tol * size + 1e-30).all(), (np.abs(got - want) / (size + 1e-30)).max()
