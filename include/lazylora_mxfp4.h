@@ -323,7 +323,8 @@ int mxfp4_dropout(void *y, const void *x, long long n, double p, uint64_t seed,
  *   divided by (their sum + 1e-20) when renormalize != 0 and top_k > 1, then times routed_scaling_factor.
  * Without a bias the order is that of the logits; with one, and between sums of two, that of scores and sums
  * in 64 bits, not of their 32-bit rounding. Values and groups that are equal so (sigmoid(38) and sigmoid(45)
- * under one bias: both 1 in 64 bits) go to the lower number, NaN comes before every number. A softmax row of nothing but -inf has scores 0; one with +inf has scores NaN.
+ * under one bias: both 1 in 64 bits) go to the lower number, NaN comes before every number. A softmax row of
+ * nothing but -inf has scores 0; one with +inf has scores NaN.
  * logits [N, E] of MXFP4_F32, _BF16 or _F16, bias [E] fp32. E <= 4096, num_groups <= 64 and a divisor of E,
  * top_k <= min(64, topk_groups E / num_groups); where num_groups is no power of two, E / num_groups at most
  * 64 times 64 / (the next power of two). */

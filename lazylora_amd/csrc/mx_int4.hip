@@ -239,7 +239,8 @@ MX_DEV uint8_t load_zero(const Rows& w, uint32_t lane, uint32_t shared)
 // is bound by the codes' bytes behind some 5 us of launch, first loads and last sums: rows of 8192 in groups of 64,
 // us (TB/s): 4096 weight rows 6.9 (2.7), 28672 26 (4.9), 114688 89 (5.8), 229376 171 (6.0). Two rows 8.6 / 30 / 94 /
 // 189; four 10.6 / 42 / 129 / 260, bound by the dots (the 4 x 4 x 4 MFMA in their place, x in its 16 registers
-// whatever its rows: 8.6 / 30 / 121 / 218 with one row, 9.5 / 32 / 127 / 231 with four).
+// whatever its rows: 8.6 / 30 / 121 / 218 with one row, 9.5 / 32 / 127 / 231 with four; not kept as a second form
+// for three and four rows alone).
 template <typename T, int G, bool ZP, int MR, Int4Epi EPI>
 __global__ __launch_bounds__(512) void int4_vec_kernel(Int4Args p)
 {

@@ -214,8 +214,8 @@ struct Careful {
 
 // One wave per token, bound by instructions: a round costs some 22 of them and is a serial chain, so as many waves as
 // there can be (eight per SIMD with 64 registers) run side by side. 8192 tokens, top-8 of 256 in 8 groups, sigmoid
-// and bias: 11 us (9 MB of logits would take 1.8); without groups and bias 8.0; 1024 tokens, top-16 of 896 in 7
-// groups, softmax and bias: 14 us; one token 3.6. A round of the selection takes the largest open key of the wave
+// and bias: 11 to 12 us (9 MB of logits would take 1.8); without groups and bias 7.3; 1024 tokens, top-16 of 896 in 7
+// groups, softmax and bias: 14 to 17 us; one token 3.7. A round of the selection takes the largest open key of the wave
 // (four butterfly steps and four lane reads), names its holder by a ballot and retires the expert there.
 template <typename T, int PER>
 __global__ __launch_bounds__(256, PER <= 4 ? 8 : 1) void select_kernel(SelectArgs a)
