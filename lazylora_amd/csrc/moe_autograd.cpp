@@ -68,9 +68,16 @@ struct Select : torch::autograd::Function<Select> {
     variable_list out(9);
     if (!grads[1].defined() || !ctx->needs_input_grad(0)) return out;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &idx = saved[1];
+    // what a saved-tensor hook hands back may lie elsewhere and otherwise than what was saved
+    const Tensor x = logits_arg(saved[0]);
+    const Tensor &si = saved[1], &g = grads[1];
+    const auto lead = [](const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); };
+    TORCH_CHECK_VALUE(si.scalar_type() == at::kLong && g.scalar_type() == at::kFloat && si.device() == x.device() &&
+                          g.device() == x.device() && si.sizes() == g.sizes() && lead(x) == lead(si),
+                      "the saved logits ", x.sizes(), " and indices ", si.scalar_type(), " ", si.sizes(), " on ",
+                      si.device(), " do not fit a gradient ", g.scalar_type(), " ", g.sizes(), " on ", g.device());
     const c10::DeviceGuard guard(x.device());
-    const Tensor gw = laid_out(grads[1]);
+    const Tensor idx = laid_out(si), gw = laid_out(g);
     out[0] = at::empty_like(x);
     const int64_t E = x.size(-1), N = x.numel() / E;
     check(mxfp4_select_topk_backward(N ? out[0].data_ptr() : nullptr, N ? idx.data_ptr<int64_t>() : nullptr,

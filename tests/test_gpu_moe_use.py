@@ -111,3 +111,29 @@ def test_a_prompt_of_thousands_of_tokens():
     assert (err <= 0.75 * eps * size * 1.5 + eps / 2 * np.abs(want) + torch.finfo(dt).tiny).all()
     # the order in which the routing places pairs does not change a result
     assert all(torch.equal(int4_routed(h, idx, w, ex), out) for _ in range(5))
+
+
+def test_saved_tensor_hooks():
+    """Saved logits and indices that come back from a hook strided, in another type or on the host."""
+    from lazylora_amd.router import select_experts
+    x = torch.randn(7, 32, device="cuda").requires_grad_(True)
+    dw = torch.randn(7, 4, device="cuda")
+    run = lambda: select_experts(x, 4, scoring="softmax", num_groups=4, topk_groups=2)[1]
+    want = torch.autograd.grad(run(), x, dw)[0]
+
+    def strided(t):
+        wide = torch.full((*t.shape, 2), -1, device=t.device, dtype=t.dtype)
+        wide[..., 0] = t.detach()
+        return wide[..., 0]
+
+    with torch.autograd.graph.saved_tensors_hooks(strided, lambda t: t):
+        w = run()
+    assert torch.equal(torch.autograd.grad(w, x, dw)[0], want)
+    with torch.autograd.graph.save_on_cpu():
+        w = run()
+    assert torch.equal(torch.autograd.grad(w, x, dw)[0], want)
+    for bad in (lambda t: t.cpu(), lambda t: t[:3], lambda t: t[:, :2], lambda t: t.double() if t.is_floating_point() else t.int()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), bad):
+            w = run()
+        with pytest.raises(ValueError):
+            torch.autograd.grad(w, x, dw)
