@@ -11,8 +11,9 @@ They run in hand-written kernels (csrc/mx_dense.hip, csrc/mx_rows.hip), as autog
 tensors they do not take; nothing falls back to torch. Sums, statistics and activation functions are
 fp32 whatever the tensors' type, and each result is rounded once. Results do not depend on timing (no
 atomics). Without a gradient to record a call saves nothing; a second derivative raises. So do
-forward-mode differentiation and tracing (torch.jit.trace, make_fx; NotImplementedError): a launch
-would drop a tangent and leave no trace. torch.compile breaks its graph at a call.
+forward-mode differentiation, tracing (torch.jit.trace, make_fx) and function transforms (torch.func.vmap,
+grad, batched gradients; all NotImplementedError): a launch would drop a tangent, leave no trace and find no
+memory. torch.compile breaks its graph at a call.
 """
 from typing import Optional, Tuple, Union
 
@@ -27,7 +28,7 @@ def _module():
     """The autograd module; RuntimeError where the native library is off or unavailable."""
     global _ext
     if kernel() is None:
-        raise RuntimeError("the MI355X dense operators are unavailable: LAZYLORA_NO_NATIVE=1 is set, or the native "
+        raise RuntimeError("the MI355X operators are unavailable: LAZYLORA_NO_NATIVE=1 is set, or the native "
                            "library failed to load, or no HIP device is visible (set LAZYLORA_NATIVE_STRICT=1 to see "
                            "the underlying error)")
     if _ext is None:

@@ -82,7 +82,7 @@ class LatentMoEBlock:
 
     scoring, num_groups, topk_groups and group_score as in select_experts. experts may be an Int4Experts: the
     routed products then run in its scales' type, without routed adapters, and where a gradient would be
-    recorded a call raises NotImplementedError.
+    recorded a call raises NotImplementedError, with a cached sum as without.
     """
 
     def __init__(self, experts: Union[ExpertLayer, Int4Experts], gate_weight, gate_bias, shared_w1, shared_w3, shared_w2, latent_down,

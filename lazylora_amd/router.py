@@ -83,7 +83,7 @@ def select_experts(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor
     groups; values that are equal there, as sigmoid(38) and sigmoid(45) under one bias are, go to the lower id,
     equal groups to the lower number, NaN comes first. A softmax row of -inf alone has weights 0. E <= 4096 (where num_groups is no power of two, 64 * 64 experts
     for the next power of two of groups), num_groups <= 64, top_k <= min(64, experts of the kept groups).
-    Second derivatives, forward-mode differentiation and tracing raise, as in lazylora_amd.dense."""
+    Second derivatives, forward-mode differentiation, tracing and function transforms raise, as in lazylora_amd.dense."""
     check_options(scoring, group_score)
     return _module().select_experts(logits, bias, top_k, SCORINGS[scoring], num_groups,
                             num_groups if topk_groups is None else topk_groups, GROUP_SCORES[group_score],
