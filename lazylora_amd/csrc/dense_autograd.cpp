@@ -62,8 +62,14 @@ struct Norm : torch::autograd::Function<Norm> {
   {
     check_modes(grads);
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
-    const NormSizes n = norm_sizes(x);
+    // what a saved-tensor hook hands back may lie elsewhere and otherwise than what was saved
+    const NormSizes n = norm_sizes(saved[0]);
+    const Tensor x = laid_out(saved[0]), w = vector_arg(saved[1], "the saved weight", n, x),
+                 stats = arg(saved[2], "the saved statistics", {2, n.M}, x, at::kFloat);
+    TORCH_CHECK_VALUE(grads[0].sizes() == x.sizes() && grads[0].scalar_type() == x.scalar_type() &&
+                          grads[0].device() == x.device(),
+                      "the saved x ", x.scalar_type(), " ", x.sizes(), " does not fit a gradient ", grads[0].scalar_type(),
+                      " ", grads[0].sizes());
     const c10::DeviceGuard guard(x.device());
     const int64_t wtype = ctx->saved_data["wtype"].toInt(), btype = ctx->saved_data["btype"].toInt();
     const bool has_w = wtype >= 0, has_b = btype >= 0;  // the inputs are numbered without the absent ones
@@ -92,6 +98,11 @@ Tensor norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, dou
 }
 
 // ---------------------------------------------------------------- dropout
+void check_seed(const Tensor& seed, const Tensor& x)
+{
+  TORCH_CHECK_VALUE(!seed.defined() || (seed.scalar_type() == at::kLong && seed.numel() == 1 && seed.device() == x.device()),
+                    "a seed tensor must hold one int64 on x's device");
+}
 Tensor dropout_run(const Tensor& t, double p, uint64_t seed, const Tensor& seed_dev, uint64_t stream)
 {
   const c10::DeviceGuard guard(t.device());
@@ -117,6 +128,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   {
     check_modes(grads);
     const Tensor seed_dev = ctx->get_saved_variables()[0];
+    check_seed(seed_dev, grads[0]);
     return once({dropout_run(grads[0], ctx->saved_data["p"].toDouble(), (uint64_t)ctx->saved_data["seed"].toInt(),
                              seed_dev, (uint64_t)ctx->saved_data["stream"].toInt()),
                  Tensor(), Tensor(), Tensor(), Tensor()});
@@ -130,8 +142,7 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, const OptTensor& seed_d
                     "x must be a float32, bfloat16 or float16 tensor on the HIP device");
   TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "p must lie in [0, 1], got ", p);
   const Tensor sd = given(seed_dev);
-  TORCH_CHECK_VALUE(!sd.defined() || (sd.scalar_type() == at::kLong && sd.numel() == 1 && sd.device() == x.device()),
-                    "a seed tensor must hold one int64 on x's device");
+  check_seed(sd, x);
   if (records({x})) return Dropout::apply(x, p, (int64_t)seed, seed_dev, (int64_t)stream);
   return dropout_run(x, p, seed, sd, stream);
 }
@@ -211,14 +222,33 @@ struct Ffn : torch::autograd::Function<Ffn> {
   {
     check_modes(grads);
     variable_list out(8);
-    const Tensor gh = grads.size() > 1 && grads[1].defined() ? tidy(grads[1]) : Tensor();
-    if (!grads[0].defined() && !gh.defined()) return out;
+    const bool hidden = grads.size() > 1 && grads[1].defined();
+    if (!grads[0].defined() && !hidden) return out;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &wd = saved[3], &h = saved[4], &gu = saved[5];
-    const c10::DeviceGuard guard(wg.device());
-    const int M = (int)gu.size(0), F = (int)wg.size(0), D = (int)wg.size(1), Do = (int)wd.size(0);
-    const Tensor gy = grads[0].defined() ? tidy(grads[0]) : at::zeros({M, Do}, wg.options());
     auto shape = ctx->saved_data["lead"].toIntVector();
+    // what a saved-tensor hook hands back may lie elsewhere and otherwise than what was saved
+    const Tensor& like = saved[1];
+    TORCH_CHECK_VALUE(like.is_cuda() && like.dim() == 2 && saved[3].dim() == 2 && saved[5].dim() == 2 &&
+                          (like.scalar_type() == at::kBFloat16 || like.scalar_type() == at::kHalf),
+                      "the saved weights must be bfloat16 or float16 matrices on the HIP device, got ", like.scalar_type(),
+                      " ", like.sizes(), " on ", like.device());
+    const c10::DeviceGuard guard(like.device());
+    const int M = (int)saved[5].size(0), F = (int)like.size(0), D = (int)shape.back(), Do = (int)saved[3].size(0);
+    const auto dt = like.scalar_type();
+    const auto rows = [&](const Tensor& t, const char* name, int64_t width) {
+      if (!t.defined()) return t;
+      shape.back() = width;
+      const Tensor r = arg(t, name, shape, like, dt);
+      shape.back() = D;
+      return r;
+    };
+    const Tensor x = rows(saved[0], "the saved x", D), h = rows(saved[4], "the saved hidden values", F),
+                 wg = arg(like, "the saved w_gate", {F, D}, like, dt), wu = arg(saved[2], "the saved w_up", {F, D}, like, dt),
+                 wd = arg(saved[3], "the saved w_down", {Do, F}, like, dt),
+                 gu = arg(saved[5], "the saved products", {c10::multiply_integers(shape.begin(), shape.end() - 1), 2LL * F},
+                          like, at::kFloat),
+                 gh = hidden ? rows(grads[1], "the gradient of the hidden values", F) : Tensor(),
+                 gy = grads[0].defined() ? rows(grads[0], "the gradient", Do) : at::zeros({M, Do}, wg.options());
     Tensor dx;
     if (ctx->needs_input_grad(0)) dx = at::empty(shape, wg.options());
     const bool has_gd = ctx->saved_data["gate_delta"].toBool(), has_ud = ctx->saved_data["up_delta"].toBool();
